@@ -232,10 +232,10 @@ def _own_norm(ops, s):
 def _own_ffn(ops, s):
     act, train = s["case"]["act"], "dy" in s
     w = (s["w_gate"], s["w_up"], s["w_down"])
-    y, gate, up = ops.gated_ffn_fwd(s["x"], *w, s["b_gate"], s["b_up"], s["b_down"], act=act, keep=train)
+    y, kept = ops.gated_ffn_fwd(s["x"], *w, s["b_gate"], s["b_up"], s["b_down"], act=act, keep=train)
     if not train:
         return {"y": y}
-    g = ops.gated_ffn_bwd(s["x"], *w, s["dy"], gate, up, s["b_gate"], s["b_up"], s["b_down"], act=act)
+    g = ops.gated_ffn_bwd(s["x"], *w, s["dy"], kept, s["b_gate"], s["b_up"], s["b_down"], act=act)
     out = {"y": y, "dx": g[0], "dw_gate": g[1], "dw_up": g[2], "dw_down": g[3]}
     if s["b_gate"] is not None:
         out.update(db_gate=g[4], db_up=g[5], db_down=g[6])
