@@ -403,6 +403,65 @@ int mragan_patch_combine(const float* pred, int X, int Y, int Z, int px, int py,
 int mragan_crop_patches(const float* vol, int X, int Y, int Z, const int* starts, int n, int px, int py, int pz,
                         float* out, void* stream);
 
+/* ---- layers of a token block on channels-last tensors -----------------------------------------
+ * Activations are [rows][C] with the channels contiguous (an NDHWC volume is N·D·H·W rows) and may
+ * be fp32, bf16 or fp16 (mragan_dtype); statistics, states and every sum are fp32.  These entry
+ * points are additions: the version number above is unchanged by them. */
+enum mragan_dtype { MRAGAN_DT_F32 = 0, MRAGAN_DT_BF16 = 1, MRAGAN_DT_F16 = 2 };
+
+/* LayerNorm over the channels: y = (x − μ)·rstd·weight + bias, rstd = (mean((x − μ)²) + eps)^−½.
+ * weight / bias ([C], type wdtype: dtype or fp32) may be NULL (1 / 0); mean and rstd ([rows]) are
+ * outputs the backward reads.  bwd: dx, dweight, dbias (types as x and weight) may each be NULL to
+ * skip it; dweight and dbias are reduced over the rows in a fixed order.  No tensor may overlap an
+ * output, except that bwd's dx may be dy. */
+int mragan_layer_norm_fwd(const void* x, int64_t rows, int C, int dtype, const void* weight, const void* bias, int wdtype,
+                          float eps, void* y, float* mean, float* rstd, void* stream);
+size_t mragan_layer_norm_bwd_workspace(int64_t rows, int C, int dtype);
+int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, const void* dy, int64_t rows, int C,
+                          int dtype, const void* weight, int wdtype, void* dx, void* dweight, void* dbias, void* ws,
+                          size_t ws_bytes, void* stream);
+
+/* Gated feed-forward block on x [M][C] with weights w_gate, w_up [F][C] and w_down [O][F]:
+ *   g = x·w_gateᵀ + b_gate,  u = x·w_upᵀ + b_up,  h = act(g)·u,  y = h·w_downᵀ + b_down   ([M][O])
+ * act: mragan_act or one of the two below (GELU is the erf form).  Biases may be NULL.  One dtype
+ * throughout; 16-byte aligned contiguous tensors.  fp32 tensors are multiplied in the process
+ * mode of mragan_set_conv_precision (f32 here: three bf16 planes per operand, six products, fp32
+ * accumulation, ≤ 2⁻²² relative error per product); 16-bit tensors as they are, and what the
+ * products take from each other (h, dg, du, `kept`) is rounded to that type.  kept [3][M][F]
+ * (dtype) holds h, act'(g)·u and act(g): fwd writes it when given, bwd reads it, or recomputes it
+ * from x when NULL.  bwd: any gradient may be NULL to skip it. */
+enum mragan_gate_act { MRAGAN_ACT_SILU = 5, MRAGAN_ACT_GELU = 6 };
+size_t mragan_gated_ffn_workspace(int64_t M, int C, int F, int O, int dtype, int backward, int recompute);
+int mragan_gated_ffn_fwd(const void* x, int64_t M, int C, int F, int O, int dtype, const void* w_gate, const void* w_up,
+                         const void* w_down, const void* b_gate, const void* b_up, const void* b_down, int act, void* y,
+                         void* kept, void* ws, size_t ws_bytes, void* stream);
+int mragan_gated_ffn_bwd(const void* x, int64_t M, int C, int F, int O, int dtype, const void* w_gate, const void* w_up,
+                         const void* w_down, const void* b_gate, const void* b_up, int act, const void* dy,
+                         const void* kept, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* db_gate, void* db_up,
+                         void* db_down, void* ws, size_t ws_bytes, void* stream);
+
+/* Gated linear recurrence over the T positions of B sequences of C channels:
+ *   a_t = σ(decay_t),  h_t = a_t·h_{t−1} + σ(−decay_t)·x_t,  y_t = h_t·silu(gate_t)   (y = h: gate NULL)
+ * from h_{−1} = h0 ([B][C] fp32, NULL = 0), or from the last position to the first with reverse = 1.
+ * x, decay, gate, dy: element (b, t, c) at b·stride_b + t·stride_t + c (strides in elements, any
+ * value: slices of one projection, expanded tensors); y, dx, ddecay, dgate: contiguous [B][T][C].
+ * last [B][C] fp32: the state after the last step.  carry [B][mragan_linear_recurrence_carries(T, C)][C]
+ * fp32: states at fixed steps that the backward restarts from (NULL in an inference call).
+ * decay = +inf leaves the state as it is (a padded position), −inf restarts from x_t; x and h
+ * have to be finite there (0·inf is NaN).  bwd: dlast may be NULL (0), dx / ddecay / dgate / dh0 too
+ * (skipped); dgate needs gate. */
+int64_t mragan_linear_recurrence_carries(int64_t T, int C);
+size_t mragan_linear_recurrence_workspace(int64_t B, int64_t T, int C, int backward);
+int mragan_linear_recurrence_fwd(const void* x, int64_t x_sb, int64_t x_st, const void* decay, int64_t d_sb, int64_t d_st,
+                                 const void* gate, int64_t g_sb, int64_t g_st, const float* h0, int64_t B, int64_t T, int C,
+                                 int dtype, int reverse, void* y, float* last, float* carry, void* ws, size_t ws_bytes,
+                                 void* stream);
+int mragan_linear_recurrence_bwd(const void* x, int64_t x_sb, int64_t x_st, const void* decay, int64_t d_sb, int64_t d_st,
+                                 const void* gate, int64_t g_sb, int64_t g_st, const float* carry, const void* dy,
+                                 int64_t dy_sb, int64_t dy_st, const float* dlast, int64_t B, int64_t T, int C, int dtype,
+                                 int reverse, void* dx, void* ddecay, void* dgate, float* dh0, void* ws, size_t ws_bytes,
+                                 void* stream);
+
 /* diagnostics: the kernel families launched by this thread since the last reset, ';'-joined
  * (e.g. "conv_wgrad3_x3;wgrad_reduce"); reset = 1 clears the log after copying it.  (ABI 7) */
 const char* mragan_launch_log(int reset);

@@ -2,6 +2,7 @@
 extension machinery: plain hipcc, one object per .hip file, parallel compile."""
 import concurrent.futures as cf
 import os
+import re
 import subprocess
 import sys
 
@@ -30,6 +31,18 @@ def _needs(obj, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _includes(path, seen=None):
+    """The in-tree headers `path` includes, directly or through another."""
+    seen = set() if seen is None else seen
+    with open(path) as f:
+        for name in re.findall(r'^\s*#include "([^"]+)"', f.read(), flags=re.M):
+            h = os.path.normpath(os.path.join(os.path.dirname(path), name))
+            if h not in seen and os.path.exists(h):
+                seen.add(h)
+                _includes(h, seen)
+    return sorted(seen)
+
+
 def _check_no_scratch(src, remarks):
     """Every kernel must run out of registers: a private-memory (scratch) spill in an MFMA loop
     costs 20× (measured: a 2-byte/lane spill turned a 60 µs conv into 1.6 ms).  Fail the build."""
@@ -49,14 +62,12 @@ def _check_no_scratch(src, remarks):
 def build(verbose=False, jobs=None):
     os.makedirs(LIB, exist_ok=True)
     os.makedirs(OBJ, exist_ok=True)
-    headers = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
-    headers.append(os.path.join(HERE, "..", "include", "mragan_hip.h"))
     objs, cmds = [], []
     for s in sources():
         src = os.path.join(CSRC, s)
         obj = os.path.join(OBJ, s.replace(".hip", ".o"))
         objs.append(obj)
-        if _needs(obj, [src] + headers):
+        if _needs(obj, [src, os.path.abspath(__file__)] + _includes(src)):   # this file: the flags
             cmds.append(["hipcc", *FLAGS, "-Rpass-analysis=kernel-resource-usage", "-c", src, "-o", obj])
     with cf.ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 1)) as ex:
         for cmd, r in zip(cmds, ex.map(lambda c: subprocess.run(c, capture_output=True, text=True), cmds)):

@@ -1,0 +1,478 @@
+// LayerNorm over the channels of channels-last rows, forward and backward.
+//
+//   fwd   μ = mean_c x,  rstd = (mean_c (x − μ)² + eps)^−½,  y = (x − μ)·rstd·w + b
+//   bwd   p = dy·w,  x̂ = (x − μ)·rstd,  dx = rstd·(p − mean_c p − x̂·mean_c(p·x̂)),
+//         dw = Σ_rows dy·x̂,  db = Σ_rows dy
+//
+// Both directions are bound by HBM: fwd reads x and writes y, bwd reads x and dy and writes dx, once
+// each.  So a row lives in the registers of the G lanes that own it (G = 4 … 64 lanes of a wave, or a
+// block of 256 / 1024 threads), every sum is taken from there (the variance as the mean of squared
+// deviations, exact for rows far from zero), a block walks over rows with the next row's loads in
+// flight, and w and b are loaded once per block.  The weight's gradient is summed per lane over the
+// rows of its block in fp32, then over the block's row groups in LDS, then over the blocks by a
+// second launch: a fixed order, no atomics.
+#include "token_ops.h"
+
+namespace mragan {
+namespace {
+
+constexpr int kThreads = 256;
+
+// 16 bytes of T; rows of any channel count start at any element, so the access is typed with the
+// element's alignment (gfx950 takes global accesses of any alignment; aligned ones cost the same)
+template <typename T>
+struct RowVec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+template <typename T>
+__device__ __forceinline__ RowVec<T> row_load(const T* row, int col, int C) {
+  RowVec<T> r;
+  if (col + RowVec<T>::N <= C) {
+    __builtin_memcpy(&r, row + col, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < RowVec<T>::N; i++) r.v[i] = col + i < C ? row[col + i] : (T)0.f;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void row_store(T* row, int col, int C, const RowVec<T>& r) {
+  if (col + RowVec<T>::N <= C) {
+    __builtin_memcpy(row + col, &r, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < RowVec<T>::N; i++)
+      if (col + i < C) row[col + i] = r.v[i];
+  }
+}
+
+// N consecutive parameters from p (fp32 or T): `dflt` where p is null or past the row
+template <int N, typename W>
+__device__ __forceinline__ void param_load(const W* p, int col, int C, float dflt, float (&out)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) out[i] = dflt;
+  if (!p) return;
+  if (col + N <= C) {
+    W t[N];
+    __builtin_memcpy(t, p + col, N * sizeof(W));
+#pragma unroll
+    for (int i = 0; i < N; i++) out[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (col + i < C) out[i] = (float)p[col + i];
+  }
+}
+
+// sum over the G lanes of a row; G > 64: over the block's waves through `red` (one slot per wave),
+// which the caller must not reuse before its next barrier
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  if constexpr (G <= 64) {
+    return group_sum<G>(v);
+  } else {
+    v = group_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < G / 64; i++) s += red[i];
+    return s;
+  }
+}
+
+template <typename T, typename W, int G, int NV>
+__global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(const T* x, int64_t rows, int C, const W* w,
+                                                                             const W* b, float eps, T* y, float* mean,
+                                                                             float* rstd) {
+  constexpr int N = RowVec<T>::N, BT = G > kThreads ? G : kThreads;
+  __shared__ float red[2][16];
+  const int lane = threadIdx.x % G;
+  const int64_t step = (int64_t)gridDim.x * (BT / G);
+  int64_t row = (int64_t)blockIdx.x * (BT / G) + threadIdx.x / G;
+  const float inv = 1.f / (float)C;
+  RowVec<T> cur[NV], nxt[NV];
+  if (row < rows) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) cur[i] = row_load(x + row * C, (i * G + lane) * N, C);
+  }
+  for (; row < rows; row += step) {
+    if (row + step < rows) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) nxt[i] = row_load(x + (row + step) * C, (i * G + lane) * N, C);
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) s += (float)cur[i].v[j];          // lanes past the row hold zeros
+    const float mu = row_sum<G>(s, red[0]) * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const float d = (float)cur[i].v[j] - mu;
+        if ((i * G + lane) * N + j < C) q += d * d;
+      }
+    const float r = rsqrtf(row_sum<G>(q, red[1]) * inv + eps);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int col = (i * G + lane) * N;
+      float wv[N], bv[N];
+      param_load<N>(w, col, C, 1.f, wv);
+      param_load<N>(b, col, C, 0.f, bv);
+      RowVec<T> o;
+#pragma unroll
+      for (int j = 0; j < N; j++) o.v[j] = (T)(((float)cur[i].v[j] - mu) * r * wv[j] + bv[j]);
+      row_store(y + row * C, col, C, o);
+    }
+    if (lane == 0) {
+      mean[row] = mu;
+      rstd[row] = r;
+    }
+    if constexpr (G > 64) __syncthreads();                           // red is read before the next row writes it
+#pragma unroll
+    for (int i = 0; i < NV; i++) cur[i] = nxt[i];
+  }
+}
+
+// part: [gridDim.x][2][C] fp32 sums of this block's rows (Σ dy·x̂, Σ dy), or null
+template <typename T, typename W, int G, int NV>
+__global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(const T* x, const float* mean, const float* rstd,
+                                                                             const T* dy, int64_t rows, int C, const W* w,
+                                                                             T* dx, float* part) {
+  constexpr int N = RowVec<T>::N, BT = G > kThreads ? G : kThreads, E = NV * N;
+  __shared__ float red[2][16];
+  __shared__ float acc_s[G <= 64 ? BT / 64 : 1][G <= 64 ? G * E + 1 : 1];
+  const int lane = threadIdx.x % G;
+  const int64_t step = (int64_t)gridDim.x * (BT / G);
+  int64_t row = (int64_t)blockIdx.x * (BT / G) + threadIdx.x / G;
+  const float inv = 1.f / (float)C;
+  float wv[NV][N], aw[NV][N], ab[NV][N];
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    param_load<N>(w, (i * G + lane) * N, C, 1.f, wv[i]);
+#pragma unroll
+    for (int j = 0; j < N; j++) aw[i][j] = ab[i][j] = 0.f;
+  }
+  RowVec<T> cx[NV], cd[NV], nx[NV], nd[NV];
+  float mu = 0.f, r = 0.f, nmu = 0.f, nr = 0.f;
+  if (row < rows) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      cx[i] = row_load(x + row * C, (i * G + lane) * N, C);
+      cd[i] = row_load(dy + row * C, (i * G + lane) * N, C);
+    }
+    mu = mean[row];
+    r = rstd[row];
+  }
+  for (; row < rows; row += step) {
+    if (row + step < rows) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        nx[i] = row_load(x + (row + step) * C, (i * G + lane) * N, C);
+        nd[i] = row_load(dy + (row + step) * C, (i * G + lane) * N, C);
+      }
+      nmu = mean[row + step];
+      nr = rstd[row + step];
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) {                                  // dy is zero past the row
+        const float d = (float)cd[i].v[j], xh = ((float)cx[i].v[j] - mu) * r, p = d * wv[i][j];
+        s1 += p;
+        s2 += p * xh;
+        aw[i][j] += d * xh;
+        ab[i][j] += d;
+      }
+    if (dx) {
+      const float m1 = row_sum<G>(s1, red[0]) * inv, m2 = row_sum<G>(s2, red[1]) * inv;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        RowVec<T> o;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+          const float xh = ((float)cx[i].v[j] - mu) * r, p = (float)cd[i].v[j] * wv[i][j];
+          o.v[j] = (T)(r * (p - m1 - xh * m2));
+        }
+        row_store(dx + row * C, (i * G + lane) * N, C, o);
+      }
+      if constexpr (G > 64) __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      cx[i] = nx[i];
+      cd[i] = nd[i];
+    }
+    mu = nmu;
+    r = nr;
+  }
+  if (!part) return;
+  float* out = part + (int64_t)blockIdx.x * 2 * C;
+  if constexpr (G > 64) {                                            // one row group: nothing to join
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const int col = (i * G + lane) * N + j;
+        if (col < C) {
+          out[col] = aw[i][j];
+          out[C + col] = ab[i][j];
+        }
+      }
+  } else {
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {                                    // dw, then db through the same LDS
+      if (k) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+          float v = k ? ab[i][j] : aw[i][j];
+          // the row groups of a wave: lanes that differ in the bits above G
+          if constexpr (G <= 4) v += __shfl_xor(v, 4);
+          if constexpr (G <= 8) v += __shfl_xor(v, 8);
+          if constexpr (G <= 16) v += __shfl_xor(v, 16);
+          if constexpr (G <= 32) v += __shfl_xor(v, 32);
+          if ((threadIdx.x & 63) < G) acc_s[wave][(i * G + lane) * N + j] = v;
+        }
+      __syncthreads();
+      for (int col = threadIdx.x; col < C; col += BT) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < BT / 64; q++) v += acc_s[q][col];
+        out[k * C + col] = v;
+      }
+    }
+  }
+}
+
+// Σ over the nb blocks' partials: a block takes 32 of the 2C columns with 32 threads each
+template <typename W>
+__global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* part, int nb, int C, W* dw, W* db) {
+  __shared__ float s[32][33];
+  const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5;
+  const int64_t col = (int64_t)blockIdx.x * 32 + cl, n = 2 * (int64_t)C;
+  float v = 0.f;
+  if (col < n)
+    for (int k = slot; k < nb; k += 32) v += part[k * n + col];
+  s[slot][cl] = v;
+  __syncthreads();
+  if (slot == 0 && col < n) {
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; k++) v += s[k][cl];
+    if (col < C) {
+      if (dw) dw[col] = (W)v;
+    } else if (db) {
+      db[col - C] = (W)v;
+    }
+  }
+}
+
+// Rows of more channels than the registers of a block hold (C > kMaxRow): the block walks the row
+// in memory, once per sum; the parameter gradients take a column per thread over all rows.
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* x, int C, const W* w, const W* b, float eps, T* y,
+                                                           float* mean, float* rstd) {
+  __shared__ float red[2][16];
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * C;
+  float s = 0.f, q = 0.f;
+  for (int c = threadIdx.x; c < C; c += 1024) s += (float)xr[c];
+  const float mu = row_sum<1024>(s, red[0]) / (float)C;
+  for (int c = threadIdx.x; c < C; c += 1024) {
+    const float d = (float)xr[c] - mu;
+    q += d * d;
+  }
+  const float r = rsqrtf(row_sum<1024>(q, red[1]) / (float)C + eps);
+  for (int c = threadIdx.x; c < C; c += 1024)
+    y[row * C + c] = (T)(((float)xr[c] - mu) * r * (w ? (float)w[c] : 1.f) + (b ? (float)b[c] : 0.f));
+  if (threadIdx.x == 0) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+}
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* x, const float* mean, const float* rstd, const T* dy, int C,
+                                                           const W* w, T* dx) {
+  __shared__ float red[2][16];
+  const int64_t row = blockIdx.x;
+  const float mu = mean[row], r = rstd[row];
+  float s1 = 0.f, s2 = 0.f;
+  for (int c = threadIdx.x; c < C; c += 1024) {
+    const float p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
+    s1 += p;
+    s2 += p * ((float)x[row * C + c] - mu) * r;
+  }
+  const float m1 = row_sum<1024>(s1, red[0]) / (float)C, m2 = row_sum<1024>(s2, red[1]) / (float)C;
+  for (int c = threadIdx.x; c < C; c += 1024) {
+    const float xh = ((float)x[row * C + c] - mu) * r, p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
+    dx[row * C + c] = (T)(r * (p - m1 - xh * m2));
+  }
+}
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void ln_param_long_kernel(const T* x, const float* mean, const float* rstd, const T* dy,
+                                                            int64_t rows, int C, W* dw, W* db) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= C) return;
+  float sw = 0.f, sb = 0.f;
+  for (int64_t k = 0; k < rows; k++) {
+    const float d = (float)dy[k * C + c];
+    sw += d * (((float)x[k * C + c] - mean[k]) * rstd[k]);
+    sb += d;
+  }
+  if (dw) dw[c] = (W)sw;
+  if (db) db[c] = (W)sb;
+}
+
+// The largest row that a block holds: 16 channels a thread of 512 (backward: their 256 registers also
+// carry the next row, the weight and two accumulators), 32 a thread of 256 (forward).
+constexpr int kMaxRow = 8192;
+// Most blocks of a backward launch: four on each of the 256 CUs, whose partial sums the second launch reads
+constexpr int kMaxBwdBlocks = 1024;
+
+// Lanes per row and 16-byte vectors per lane.  A wave or a part of one per row as long as `most`
+// channels a lane suffice, else the block.  Few rows (≤ 1024: fewer waves than the chip's SIMDs hold
+// one each of) of more than 64 vectors take a block each, so that more CUs share the loads.
+struct Shape {
+  int G, NV;
+};
+Shape pick(int64_t rows, int C, int N, int most) {
+  const int V = ceil_div(C, N);
+  for (int g = 4; g <= 64; g *= 2)
+    if (V <= g) return {g, 1};
+  for (int g : {64, 256}) {
+    if (g == 64 && rows <= 1024) continue;
+    for (int nv = 1; nv * N <= most; nv *= 2)
+      if (V <= g * nv) return {g, nv};
+  }
+  return {512, 16 / N};
+}
+
+template <typename T, typename W>
+int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, float eps, void* y, float* mean, float* rstd,
+           hipStream_t st) {
+  constexpr int N = RowVec<T>::N;
+  const T* xt = static_cast<const T*>(x);
+  const W *wt = static_cast<const W*>(w), *bt = static_cast<const W*>(b);
+  T* yt = static_cast<T*>(y);
+  if (C > kMaxRow) {
+    ln_fwd_long_kernel<T, W><<<(unsigned)rows, 1024, 0, st>>>(xt, C, wt, bt, eps, yt, mean, rstd);
+    return check_launch("layer_norm_fwd_long");
+  }
+  const Shape s = pick(rows, C, N, 32);
+  const int64_t per = kThreads / s.G, blocks = (rows + per - 1) / per, most = 2048;
+  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+#define LN_RUN(G_, NV_)                                                                                                  \
+  if constexpr (NV_ * N <= 32) {                                                                                         \
+    if (s.G == G_ && s.NV == NV_) {                                                                                      \
+      ln_fwd_kernel<T, W, G_, NV_><<<grid, kThreads, 0, st>>>(xt, rows, C, wt, bt, eps, yt, mean, rstd); \
+      return check_launch("layer_norm_fwd");                                                                             \
+    }                                                                                                                    \
+  }
+  LN_RUN(4, 1) LN_RUN(8, 1) LN_RUN(16, 1) LN_RUN(32, 1) LN_RUN(64, 1) LN_RUN(64, 2) LN_RUN(64, 4) LN_RUN(64, 8)
+  LN_RUN(256, 1) LN_RUN(256, 2) LN_RUN(256, 4) LN_RUN(256, 8)
+#undef LN_RUN
+  set_error("layer_norm_fwd: no kernel for C = %d", C);
+  return kUnsupported;
+}
+
+Shape bwd_shape(int64_t rows, int C, int N) { return pick(rows, C, N, 16); }
+int bwd_blocks(int64_t rows, int C, int N) {
+  const Shape s = bwd_shape(rows, C, N);
+  const int per = s.G > kThreads ? 1 : kThreads / s.G;
+  const int64_t blocks = (rows + per - 1) / per, most = s.G > kThreads ? kMaxBwdBlocks / 2 : kMaxBwdBlocks;
+  return (int)(blocks < most ? blocks : most);
+}
+
+template <typename T, typename W>
+int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, int64_t rows, int C, const void* w, void* dx,
+           void* dw, void* db, float* part, hipStream_t st) {
+  constexpr int N = RowVec<T>::N;
+  const T *xt = static_cast<const T*>(x), *dyt = static_cast<const T*>(dy);
+  const W* wt = static_cast<const W*>(w);
+  T* dxt = static_cast<T*>(dx);
+  W *dwt = static_cast<W*>(dw), *dbt = static_cast<W*>(db);
+  const bool params = dw || db;
+  if (C > kMaxRow) {
+    if (dx) {
+      ln_bwd_long_kernel<T, W><<<(unsigned)rows, 1024, 0, st>>>(xt, mean, rstd, dyt, C, wt, dxt);
+      if (int rc = check_launch("layer_norm_bwd_long")) return rc;
+    }
+    if (params) {
+      ln_param_long_kernel<T, W><<<ceil_div(C, 256), 256, 0, st>>>(xt, mean, rstd, dyt, rows, C, dwt, dbt);
+      return check_launch("layer_norm_param_long");
+    }
+    return kOk;
+  }
+  const Shape s = bwd_shape(rows, C, N);
+  const unsigned grid = bwd_blocks(rows, C, N);
+  if (!params) part = nullptr;
+  int rc = kUnsupported;
+#define LN_RUN(G_, NV_)                                                                                                 \
+  if constexpr (NV_ * N <= 16) {                                                                                        \
+    if (s.G == G_ && s.NV == NV_) {                                                                                     \
+      ln_bwd_kernel<T, W, G_, NV_><<<grid, G_ > kThreads ? G_ : kThreads, 0, st>>>(xt, mean, rstd, dyt, rows, C, wt, dxt, part); \
+      rc = check_launch("layer_norm_bwd");                                                                              \
+    }                                                                                                                   \
+  }
+  LN_RUN(4, 1) LN_RUN(8, 1) LN_RUN(16, 1) LN_RUN(32, 1) LN_RUN(64, 1) LN_RUN(64, 2) LN_RUN(64, 4)
+  LN_RUN(256, 1) LN_RUN(256, 2) LN_RUN(256, 4) LN_RUN(512, 16 / N)
+#undef LN_RUN
+  if (rc) return rc;
+  if (params) {
+    ln_param_reduce_kernel<W><<<ceil_div(2 * (int64_t)C, 32), 1024, 0, st>>>(part, (int)grid, C, dwt, dbt);
+    return check_launch("layer_norm_param_reduce");
+  }
+  return kOk;
+}
+
+template <typename W>
+__global__ void ln_zero_kernel(W* dw, W* db, int C) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= C) return;
+  if (dw) dw[c] = (W)0.f;
+  if (db) db[c] = (W)0.f;
+}
+
+}  // namespace
+
+size_t layer_norm_bwd_ws_bytes(int64_t rows, int C, int dtype) {
+  if (C > kMaxRow || rows == 0) return 0;
+  return (size_t)bwd_blocks(rows, C, dtype == kF32 ? 4 : 8) * 2 * C * sizeof(float);
+}
+
+int layer_norm_fwd(const void* x, int64_t rows, int C, int dtype, const void* w, const void* b, int wdtype, float eps, void* y,
+                   float* mean, float* rstd, hipStream_t st) {
+  if (rows == 0) return kOk;
+  MRAGAN_DTYPE_DISPATCH(dtype, T, {
+    if (wdtype == kF32) return ln_fwd<T, float>(x, rows, C, w, b, eps, y, mean, rstd, st);
+    return ln_fwd<T, T>(x, rows, C, w, b, eps, y, mean, rstd, st);
+  })
+  return kOk;
+}
+
+int layer_norm_bwd(const void* x, const float* mean, const float* rstd, const void* dy, int64_t rows, int C, int dtype,
+                   const void* w, int wdtype, void* dx, void* dw, void* db, float* part, hipStream_t st) {
+  if (rows == 0) {                                                   // empty sums
+    if (!dw && !db) return kOk;
+    MRAGAN_DTYPE_DISPATCH(wdtype, W, {
+      ln_zero_kernel<W><<<ceil_div(C, 256), 256, 0, st>>>(static_cast<W*>(dw), static_cast<W*>(db), C);
+    })
+    return check_launch("layer_norm_zero");
+  }
+  MRAGAN_DTYPE_DISPATCH(dtype, T, {
+    if (wdtype == kF32) return ln_bwd<T, float>(x, mean, rstd, dy, rows, C, w, dx, dw, db, part, st);
+    return ln_bwd<T, T>(x, mean, rstd, dy, rows, C, w, dx, dw, db, part, st);
+  })
+  return kOk;
+}
+
+}  // namespace mragan

@@ -116,6 +116,20 @@ SIGNATURES = {
     # ABI 19: the interior + shell data-gradient rule as a query
     "mragan_conv3d_dgrad_split": (i32, [i32] * 6),
     "mragan_conv3d_wgrad_op16_pair": (i32, [vp, i32, vp, vp, i32, vp] + [i32] * 11 + [vp, i32, vp, sz, vp]),
+    # token-block layers (additions without a version change)
+    "mragan_layer_norm_fwd": (i32, [vp, i64, i32, i32, vp, vp, i32, f32, vp, vp, vp, vp]),
+    "mragan_layer_norm_bwd_workspace": (sz, [i64, i32, i32]),
+    "mragan_layer_norm_bwd": (i32, [vp, vp, vp, vp, i64, i32, i32, vp, i32, vp, vp, vp, vp, sz, vp]),
+    "mragan_gated_ffn_workspace": (sz, [i64, i32, i32, i32, i32, i32, i32]),
+    "mragan_gated_ffn_fwd": (i32, [vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, sz, vp]),
+    "mragan_gated_ffn_bwd": (i32, [vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                   vp, sz, vp]),
+    "mragan_linear_recurrence_carries": (i64, [i64, i32]),
+    "mragan_linear_recurrence_workspace": (sz, [i64, i64, i32, i32]),
+    "mragan_linear_recurrence_fwd": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i32, i32, vp, vp, vp,
+                                           vp, sz, vp]),
+    "mragan_linear_recurrence_bwd": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp, i64, i64, vp, i64, i64, i32, i32,
+                                           i32, vp, vp, vp, vp, vp, sz, vp]),
     "mragan_conv3d_presplit_bwd_stats": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, i32, i32, i32, i32, vp, i32, i32, i32,
                                                i32, vp, sz, vp, vp, vp, i32, vp, sz, vp, vp]),
 }

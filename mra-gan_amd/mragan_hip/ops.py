@@ -1093,3 +1093,253 @@ def crop_patches(vol: torch.Tensor, starts: torch.Tensor, patch, out: Optional[t
     X, Y, Z = vol.shape
     call("mragan_crop_patches", _ptr(vol), X, Y, Z, _ptr(starts.contiguous()), n, px, py, pz, _ptr(out), _stream())
     return out
+
+
+# ---- layers of a token block --------------------------------------------------------------------
+# LayerNorm, gated feed-forward block and gated linear recurrence on channels-last tensors of any of
+# three element types.  Unlike the calls above these take their device and stream from their first
+# tensor (a tensor of another device than the current one runs there, on that device's current
+# stream), and their scratch memory from torch's allocator per call: two streams, or two captured
+# graphs, never share it.  Outputs are new tensors.
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+GATE_ACT = dict(ACT, silu=5, gelu=6)
+
+
+def _token_dtype(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in _DTYPE:
+        raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a device tensor (HIP); got {t.device}")
+    return _DTYPE[t.dtype]
+
+
+def _like(t: Optional[torch.Tensor], name: str, ref: torch.Tensor, shape, dtype=None):
+    """t of this shape, of ref's device and (unless given) type; None passes."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != (dtype or ref.dtype):
+        raise ValueError(f"{name}: expected {dtype or ref.dtype}, got {t.dtype}")
+    if t.device != ref.device:
+        raise ValueError(f"{name}: expected a tensor on {ref.device}, got {t.device}")
+    return t
+
+
+def _dense(t: Optional[torch.Tensor]):
+    """Contiguous, and on the 16-byte boundary that the products' loads need (a view may start off one)."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+def _scratch(nbytes: int, ref: torch.Tensor):
+    return torch.empty(nbytes, dtype=torch.uint8, device=ref.device) if nbytes else None
+
+
+def _call_on(ref: torch.Tensor, name: str, *args):
+    """The library call on ref's device and that device's current stream."""
+    if ref.device.index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(ref.device):
+            call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _ln_params(x, weight, bias):
+    """Code of the weight's and bias's common type: x's, or float32."""
+    C = x.shape[-1]
+    wd = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+    if wd not in (x.dtype, torch.float32):
+        raise ValueError(f"layer_norm: weight and bias must be {x.dtype} or float32, got {wd}")
+    _like(weight, "layer_norm.weight", x, (C,), wd)
+    _like(bias, "layer_norm.bias", x, (C,), wd)
+    return wd
+
+
+def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                   eps: float = 1e-5):
+    """LayerNorm over the last dimension of x [..., C] (any leading shape).  weight / bias [C]: x's type or
+    float32.  Returns (y, mean, rstd), mean and rstd float32 of x's leading shape."""
+    dt = _token_dtype(x, "layer_norm.x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm: expected [..., C] with C ≥ 1, got shape {tuple(x.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
+    wd = _ln_params(x, weight, bias)
+    x, C = x.contiguous(), x.shape[-1]
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty_like(x)
+    mean = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    fn = lambda: _call_on(x, "mragan_layer_norm_fwd", _ptr(x), mean.numel(), C, dt, _ptr(weight), _ptr(bias), _DTYPE[wd], eps,
+                          _ptr(y), _ptr(mean), _ptr(rstd))
+    _timed(lambda: dict(op="ln_fwd", cls=f"layer_norm_fwd C{C} [{mean.numel()}] {x.dtype}",
+                        bytes=2.0 * x.numel() * x.element_size()), fn)
+    return y, mean, rstd
+
+
+def layer_norm_bwd(x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, dy: torch.Tensor,
+                   weight: Optional[torch.Tensor] = None, bias=False):
+    """Gradients (dx, dweight, dbias) of layer_norm_fwd.  dweight is None without a weight.  bias: True (dbias of
+    the weight's type, or x's), a dtype, or False (None)."""
+    dt = _token_dtype(x, "layer_norm_bwd.x")
+    lead, C = x.shape[:-1], x.shape[-1]
+    wd = _ln_params(x, weight, None)
+    if isinstance(bias, torch.dtype):
+        if weight is not None and bias != wd or bias not in (x.dtype, torch.float32):
+            raise ValueError(f"layer_norm_bwd: bias gradient of {bias} beside x of {x.dtype}, weight of {wd}")
+        wd = bias
+    _like(dy, "layer_norm_bwd.dy", x, x.shape)
+    _like(mean, "layer_norm_bwd.mean", x, lead, torch.float32)
+    _like(rstd, "layer_norm_bwd.rstd", x, lead, torch.float32)
+    x, dy, mean, rstd = x.contiguous(), dy.contiguous(), mean.contiguous(), rstd.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    dx = torch.empty_like(x)
+    dw = None if weight is None else torch.empty(C, device=x.device, dtype=wd)
+    db = torch.empty(C, device=x.device, dtype=wd) if bias else None
+    nbytes = query("mragan_layer_norm_bwd_workspace", mean.numel(), C, dt) if dw is not None or bias else 0
+    ws = _scratch(nbytes, x)
+    fn = lambda: _call_on(x, "mragan_layer_norm_bwd", _ptr(x), _ptr(mean), _ptr(rstd), _ptr(dy), mean.numel(), C, dt,
+                          _ptr(weight), _DTYPE[wd], _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+    _timed(lambda: dict(op="ln_bwd", cls=f"layer_norm_bwd C{C} [{mean.numel()}] {x.dtype}",
+                        bytes=3.0 * x.numel() * x.element_size()), fn)
+    return dx, dw, db
+
+
+def _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
+    dt = _token_dtype(x, "gated_ffn.x")
+    if act not in GATE_ACT:
+        raise ValueError(f"gated_ffn: act must be one of {sorted(k for k in GATE_ACT if k)}, got {act!r}")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_down.dim() != 2:
+        raise ValueError(f"gated_ffn: expected x [..., C], w_gate, w_up [F, C], w_down [O, F]; got {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    C, F, O = x.shape[-1], w_gate.shape[0], w_down.shape[0]
+    if min(C, F, O) < 1:
+        raise ValueError("gated_ffn: a dimension of length 0")
+    for t, name, shape in ((w_gate, "w_gate", (F, C)), (w_up, "w_up", (F, C)), (w_down, "w_down", (O, F)),
+                           (b_gate, "b_gate", (F,)), (b_up, "b_up", (F,)), (b_down, "b_down", (O,))):
+        _like(t, "gated_ffn." + name, x, shape)
+    return dt, C, F, O
+
+
+def gated_ffn_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                  b_gate: Optional[torch.Tensor] = None, b_up: Optional[torch.Tensor] = None,
+                  b_down: Optional[torch.Tensor] = None, act: str = "silu", keep: bool = False):
+    """y = (act(x·w_gateᵀ + b_gate) · (x·w_upᵀ + b_up))·w_downᵀ + b_down for x [..., C], w_gate, w_up [F, C],
+    w_down [O, F], one type throughout; act: silu, gelu or one of ACT.  float32 tensors are multiplied in
+    set_conv_precision's mode.  Returns (y [..., O], kept): kept [3, rows, F] spares the backward the first
+    two products (keep=True), else None."""
+    dt, C, F, O = _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+    x, w_gate, w_up, w_down, b_gate, b_up, b_down = map(_dense, (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
+    M = x.numel() // C
+    y = torch.empty(x.shape[:-1] + (O,), device=x.device, dtype=x.dtype)
+    kept = torch.empty((3, M, F), device=x.device, dtype=x.dtype) if keep else None
+    nbytes = query("mragan_gated_ffn_workspace", M, C, F, O, dt, 0, 0)
+    ws = _scratch(nbytes, x)
+    fn = lambda: _call_on(x, "mragan_gated_ffn_fwd", _ptr(x), M, C, F, O, dt, _ptr(w_gate), _ptr(w_up), _ptr(w_down),
+                          _ptr(b_gate), _ptr(b_up), _ptr(b_down), GATE_ACT[act], _ptr(y), _ptr(kept) if M else None, _ptr(ws),
+                          nbytes)
+    _timed(lambda: dict(op="ffn_fwd", cls=f"gated_ffn_fwd {C}->{F}->{O} [{M}] {x.dtype}", flops=2.0 * M * F * (2 * C + O)), fn)
+    return y, kept
+
+
+def gated_ffn_bwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, dy: torch.Tensor,
+                  kept: Optional[torch.Tensor] = None, b_gate: Optional[torch.Tensor] = None,
+                  b_up: Optional[torch.Tensor] = None, b_down: Optional[torch.Tensor] = None, act: str = "silu",
+                  need: Sequence[bool] = (True,) * 7):
+    """Gradients (dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down) of gated_ffn_fwd, None for an absent bias and
+    where `need` is False.  kept: gated_ffn_fwd's, or None (recomputed from x)."""
+    dt, C, F, O = _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+    _like(dy, "gated_ffn_bwd.dy", x, x.shape[:-1] + (O,))
+    M = x.numel() // C
+    _like(kept, "gated_ffn_bwd.kept", x, (3, M, F))
+    like = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    grads = [torch.empty(t.shape, device=x.device, dtype=x.dtype) if n and t is not None else None for t, n in zip(like, need)]
+    if M == 0:                                             # no rows: empty sums
+        return tuple(None if g is None else g.zero_() for g in grads)
+    x, w_gate, w_up, w_down, b_gate, b_up, dy, kept = map(_dense, (x, w_gate, w_up, w_down, b_gate, b_up, dy, kept))
+    nbytes = query("mragan_gated_ffn_workspace", M, C, F, O, dt, 1, int(kept is None))
+    ws = _scratch(nbytes, x)
+    fn = lambda: _call_on(x, "mragan_gated_ffn_bwd", _ptr(x), M, C, F, O, dt, _ptr(w_gate), _ptr(w_up), _ptr(w_down),
+                          _ptr(b_gate), _ptr(b_up), GATE_ACT[act], _ptr(dy), _ptr(kept), *map(_ptr, grads), _ptr(ws), nbytes)
+    _timed(lambda: dict(op="ffn_bwd", cls=f"gated_ffn_bwd {C}->{F}->{O} [{M}] {x.dtype}",
+                        flops=4.0 * M * F * (2 * C + O) + (0 if kept is not None else 4.0 * M * F * C)), fn)
+    return tuple(grads)
+
+
+def _sequence(t: Optional[torch.Tensor], name: str, ref: torch.Tensor):
+    """(tensor, batch stride, time stride): t as it is where its channels are contiguous, else a copy."""
+    if t is None:
+        return None, 0, 0
+    _like(t, name, ref, ref.shape)
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        t = t.contiguous()
+    return t, t.stride(0), t.stride(1)
+
+
+def _recurrence_check(x):
+    dt = _token_dtype(x, "linear_recurrence.x")
+    if x.dim() != 3 or x.shape[2] < 1:
+        raise ValueError(f"linear_recurrence: expected [B, T, C] with C ≥ 1, got shape {tuple(x.shape)}")
+    return dt, x.shape[0], x.shape[1], x.shape[2]
+
+
+def linear_recurrence_fwd(x: torch.Tensor, decay: torch.Tensor, gate: Optional[torch.Tensor] = None,
+                          h0: Optional[torch.Tensor] = None, reverse: bool = False):
+    """h_t = σ(decay_t)·h_{t−1} + σ(−decay_t)·x_t along dimension 1 of [B, T, C] from h0 ([B, C] float32, default 0),
+    y = h·silu(gate) (y = h without a gate); reverse: from the last position to the first.  x, decay and gate
+    may be strided (slices of one projection, expanded tensors).  Returns (y, last, carry): last [B, C] float32,
+    the state after the last step (the next call's h0); carry: states the backward restarts from."""
+    dt, B, T, C = _recurrence_check(x)
+    xs = _sequence(x, "linear_recurrence.x", x)
+    ds = _sequence(decay, "linear_recurrence.decay", x)
+    gs = _sequence(gate, "linear_recurrence.gate", x)
+    _like(h0, "linear_recurrence.h0", x, (B, C), torch.float32)
+    h0 = None if h0 is None else h0.contiguous()
+    y = torch.empty((B, T, C), device=x.device, dtype=x.dtype)
+    carry = torch.empty((B, query("mragan_linear_recurrence_carries", T, C), C), device=x.device, dtype=torch.float32)
+    if T == 0 or B == 0:
+        last = torch.zeros((B, C), device=x.device, dtype=torch.float32) if h0 is None else h0.clone()
+        return y, last, carry
+    last = torch.empty((B, C), device=x.device, dtype=torch.float32)
+    nbytes = query("mragan_linear_recurrence_workspace", B, T, C, 0)
+    ws = _scratch(nbytes, x)
+    fn = lambda: _call_on(x, "mragan_linear_recurrence_fwd", _ptr(xs[0]), xs[1], xs[2], _ptr(ds[0]), ds[1], ds[2], _ptr(gs[0]),
+                          gs[1], gs[2], _ptr(h0), B, T, C, dt, int(reverse), _ptr(y), _ptr(last), _ptr(carry), _ptr(ws), nbytes)
+    _timed(lambda: dict(op="recur_fwd", cls=f"linear_recurrence_fwd [{B}x{T}x{C}] {x.dtype}",
+                        bytes=(3.0 + (gate is not None)) * y.numel() * y.element_size()), fn)
+    return y, last, carry
+
+
+def linear_recurrence_bwd(x: torch.Tensor, decay: torch.Tensor, carry: torch.Tensor, dy: torch.Tensor,
+                          gate: Optional[torch.Tensor] = None, dlast: Optional[torch.Tensor] = None, reverse: bool = False,
+                          need: Sequence[bool] = (True,) * 4):
+    """Gradients (dx, ddecay, dgate, dh0) of linear_recurrence_fwd, contiguous (dh0 float32), from dy and, if the
+    final state was used, dlast [B, C] float32; None without a gate and where `need` is False."""
+    dt, B, T, C = _recurrence_check(x)
+    xs = _sequence(x, "linear_recurrence_bwd.x", x)
+    ds = _sequence(decay, "linear_recurrence_bwd.decay", x)
+    gs = _sequence(gate, "linear_recurrence_bwd.gate", x)
+    ys = _sequence(dy, "linear_recurrence_bwd.dy", x)
+    _like(carry, "linear_recurrence_bwd.carry", x, (B, query("mragan_linear_recurrence_carries", T, C), C), torch.float32)
+    _like(dlast, "linear_recurrence_bwd.dlast", x, (B, C), torch.float32)
+    carry = carry.contiguous()
+    dlast = None if dlast is None else dlast.contiguous()
+    new = lambda n: torch.empty((B, T, C), device=x.device, dtype=x.dtype) if n else None
+    dx, dd, dz = new(need[0]), new(need[1]), new(need[2] and gate is not None)
+    if T == 0 or B == 0:
+        dh0 = (torch.zeros((B, C), device=x.device, dtype=torch.float32) if dlast is None else dlast.clone()) if need[3] else None
+        return dx, dd, dz, dh0
+    dh0 = torch.empty((B, C), device=x.device, dtype=torch.float32) if need[3] else None
+    nbytes = query("mragan_linear_recurrence_workspace", B, T, C, 1)
+    ws = _scratch(nbytes, x)
+    fn = lambda: _call_on(x, "mragan_linear_recurrence_bwd", _ptr(xs[0]), xs[1], xs[2], _ptr(ds[0]), ds[1], ds[2], _ptr(gs[0]),
+                          gs[1], gs[2], _ptr(carry), _ptr(ys[0]), ys[1], ys[2], _ptr(dlast), B, T, C, dt, int(reverse), _ptr(dx),
+                          _ptr(dd), _ptr(dz), _ptr(dh0), _ptr(ws), nbytes)
+    n = sum(t is not None for t in (gate, dx, dd, dz)) + 3.0
+    _timed(lambda: dict(op="recur_bwd", cls=f"linear_recurrence_bwd [{B}x{T}x{C}] {x.dtype}",
+                        bytes=n * x.numel() * x.element_size()), fn)
+    return dx, dd, dz, dh0

@@ -18,6 +18,13 @@ argument must be float32 on the input's device (checked: the kernels take raw po
   mragan::gan_loss         GANLoss (BCE on D's sigmoid output, or MSE)      networks3D.py:130-150
   mragan::adam_            torch.optim.Adam step on a flat parameter buffer cycle_gan_model.py:107-110
 
+Layers of a token block over the same channels-last activations (no counterpart in the reference's
+networks), on float32, bfloat16 or float16 tensors:
+
+  mragan::layer_norm         nn.LayerNorm over the channels
+  mragan::gated_ffn          act(x·Wgᵀ)·(x·Wuᵀ)·Wdᵀ (+ biases), nn.Linear weight layouts
+  mragan::linear_recurrence  h_t = σ(d_t)·h_{t−1} + σ(−d_t)·x_t, y_t = h_t·silu(z_t) along [B, T, C]
+
 The loss ops' gradients are the kernels' (sign(a − b)/n, dGANLoss/dp) times the incoming gradient;
 they need the process-wide loss scale at 1 (ops.set_loss_scale), which they check.
 """
@@ -269,4 +276,98 @@ def _(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, step, grad_scale)
     return None
 
 
-OPS: List[str] = ["conv3d", "instance_norm", "replication_pad", "l1_loss", "gan_loss", "adam_"]
+@torch.library.custom_op("mragan::layer_norm", mutates_args=(), device_types="cuda")
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+               eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, mean, rstd) over x's last dimension; weight / bias of x's type or float32.  Differentiable in y."""
+    return ops.layer_norm_fwd(x, weight, bias, eps)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps):
+    return (x.new_empty(x.shape), x.new_empty(x.shape[:-1], dtype=torch.float32),
+            x.new_empty(x.shape[:-1], dtype=torch.float32))
+
+
+def _ln_setup(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    _, mean, rstd = output
+    ctx.save_for_backward(x, weight, mean, rstd)
+    ctx.bias = bias.dtype if bias is not None else False
+    ctx.mark_non_differentiable(mean, rstd)
+
+
+def _ln_backward(ctx, dy, _dmean, _drstd):
+    x, weight, mean, rstd = ctx.saved_tensors
+    return ops.layer_norm_bwd(x, mean, rstd, dy, weight, bias=ctx.bias) + (None,)
+
+
+layer_norm.register_autograd(_ln_backward, setup_context=_ln_setup)
+
+
+@torch.library.custom_op("mragan::gated_ffn", mutates_args=(), device_types="cuda")
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              b_gate: Optional[torch.Tensor], b_up: Optional[torch.Tensor], b_down: Optional[torch.Tensor], act: str,
+              keep: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, kept).  keep: hold the inner products for the backward ([3, rows, F]); else kept is empty and a backward
+    computes them again (inference, or less memory for a third more work)."""
+    y, kept = ops.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep)
+    return y, x.new_empty(0) if kept is None else kept
+
+
+@gated_ffn.register_fake
+def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
+    rows = x.numel() // x.shape[-1]
+    return (x.new_empty(x.shape[:-1] + (w_down.shape[0],)),
+            x.new_empty((3, rows, w_gate.shape[0])) if keep else x.new_empty(0))
+
+
+def _ffn_setup(ctx, inputs, output):
+    ctx.act, ctx.keep = inputs[7:]
+    ctx.save_for_backward(*inputs[:7], output[1] if ctx.keep else None)
+    ctx.mark_non_differentiable(output[1])
+
+
+def _ffn_backward(ctx, dy, _dkept):
+    x, wg, wu, wd, bg, bu, bd, kept = ctx.saved_tensors
+    return ops.gated_ffn_bwd(x, wg, wu, wd, dy, kept, bg, bu, bd, ctx.act, need=ctx.needs_input_grad[:7]) + (None, None)
+
+
+gated_ffn.register_autograd(_ffn_backward, setup_context=_ffn_setup)
+
+
+@torch.library.custom_op("mragan::linear_recurrence", mutates_args=(), device_types="cuda")
+def linear_recurrence(x: torch.Tensor, decay: torch.Tensor, gate: Optional[torch.Tensor], h0: Optional[torch.Tensor],
+                      reverse: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, last, carry).  Differentiable in y and last."""
+    return ops.linear_recurrence_fwd(x, decay, gate, h0, reverse)
+
+
+@linear_recurrence.register_fake
+def _(x, decay, gate, h0, reverse):
+    B, T, C = x.shape
+    n = ops.query("mragan_linear_recurrence_carries", T, C)
+    return (x.new_empty((B, T, C)), x.new_empty((B, C), dtype=torch.float32), x.new_empty((B, n, C), dtype=torch.float32))
+
+
+def _recur_setup(ctx, inputs, output):
+    x, decay, gate, _, ctx.reverse = inputs
+    ctx.save_for_backward(x, decay, gate, output[2])
+    ctx.mark_non_differentiable(output[2])
+    ctx.set_materialize_grads(False)                   # an unused output has no gradient
+
+
+def _recur_backward(ctx, dy, dlast, _dcarry):
+    x, decay, gate, carry = ctx.saved_tensors
+    if dy is None:
+        if dlast is None:
+            return None, None, None, None, None
+        dy = x.new_zeros(1).expand(x.shape)
+    return ops.linear_recurrence_bwd(x, decay, carry, dy, gate, dlast, ctx.reverse, need=ctx.needs_input_grad[:4]) + (None,)
+
+
+linear_recurrence.register_autograd(_recur_backward, setup_context=_recur_setup)
+
+
+OPS: List[str] = ["conv3d", "instance_norm", "replication_pad", "l1_loss", "gan_loss", "adam_", "layer_norm", "gated_ffn",
+                  "linear_recurrence"]
