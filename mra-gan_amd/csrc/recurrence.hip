@@ -5,12 +5,14 @@
 //   dx_t = G_t·i_t,  dd_t = G_t·(h_{t−1} − x_t)·a_t·i_t,  dz_t = dy_t·h_t·silu'(z_t)
 //
 // Both recursions are products of affine maps s ↦ P·s + E, which compose associatively, so time is
-// split: a lane takes S steps of kVC channels in order, the LT time lanes of a block join their
-// (P, E) through LDS (a chunk of kChunk = LT·S steps), and a block walks over the chunks with the
-// state of 64 channels in fp32.  HBM is the bound: each tensor is read or written once.  Where B and
-// C give too few blocks to fill the chip, the chunks are also split into segments over blocks: a
-// first launch reduces each segment to its (P, E), the second starts each segment from the fold
-// of the ones before it (its inputs then come a second time, as a rule from the 256 MB cache).
+// split: a lane takes S = 8 steps of two channels in order, the two time lanes of a wave join their
+// maps in registers and the eight waves of a block through LDS (a chunk of 128 steps), and a block
+// walks over the chunks with the fp32 state of 64 channels in registers, the next chunk's loads in
+// flight.  HBM is the bound: each tensor is read or written once.  Where B and C give too few blocks
+// to fill the chip, the chunks are also split into segments over blocks: a first launch reduces each
+// segment to its (P, E), the second starts each segment from the fold of the ones before it (its
+// inputs then come a second time, as a rule from the 256 MB cache).
+// Steps behind the end of a sequence and channels behind C enter as d = +inf, x = 0: the identity.
 // The forward leaves the fp32 state entering each chunk; the backward recomputes the states of a
 // chunk from it in registers and walks the chunks backwards, so that no state is read or written.
 #include "token_ops.h"
@@ -18,11 +20,15 @@
 namespace mragan {
 namespace {
 
-constexpr int kVC = 4;          // channels a lane
-constexpr int kChunk = 128;     // steps between two carried states
-constexpr int kLC = 16;         // channel lanes: 64 channels, 128 bytes of a 16-bit row
+constexpr int kVC = 2;                    // channels a lane
+constexpr int kLC = 32;                   // channel lanes: 64 channels, 128 bytes of a 16-bit row
 constexpr int kCT = kLC * kVC;
-constexpr int kShort = 16;      // sequences up to this long: a thread walks the whole sequence
+constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kLT = kWaves * 2;           // time lanes
+constexpr int kS = 8;                     // steps of a time lane
+constexpr int kChunk = kLT * kS;          // 128 steps between two carried states
+constexpr int kShort = 16;                // sequences up to this long: a thread walks the whole sequence
+constexpr int kShortVC = 4;               // of this many channels
 
 template <typename T>
 struct Strided {                // element (b, t, c) at p[b·sb + t·st + c]
@@ -30,44 +36,35 @@ struct Strided {                // element (b, t, c) at p[b·sb + t·st + c]
   int64_t sb, st;
 };
 
-// kVC channels of one step; lanes past C hold zeros
-template <typename T>
-struct Quad {
-  T v[kVC];
-};
-template <typename T>
-__device__ __forceinline__ Quad<T> quad_load(const T* p, int n) {    // n: channels left, ≥ 1
-  Quad<T> r;
-  if (n >= kVC) {
+// N channels of one step; those past the row's end (n channels left) read `fill` and are not written
+template <int N, typename T>
+__device__ __forceinline__ Words<T, N> group_load(const T* p, int n, float fill = 0.f) {
+  Words<T, N> r;
+  if (n >= N) {
     __builtin_memcpy(&r, p, sizeof(r));
   } else {
 #pragma unroll
-    for (int i = 0; i < kVC; i++) r.v[i] = i < n ? p[i] : (T)0.f;
+    for (int i = 0; i < N; i++) r.set(i, i < n ? (float)p[i] : fill);
   }
   return r;
 }
-template <typename T>
-__device__ __forceinline__ void quad_store(T* p, int n, const Quad<T>& r) {
-  if (n >= kVC) {
+template <int N, typename T>
+__device__ __forceinline__ void group_store(T* p, int n, const Words<T, N>& r) {
+  if (n >= N) {
     __builtin_memcpy(p, &r, sizeof(r));
   } else {
 #pragma unroll
-    for (int i = 0; i < kVC; i++)
-      if (i < n) p[i] = r.v[i];
+    for (int i = 0; i < N; i++)
+      if (i < n) p[i] = (T)r.get(i);
   }
 }
 
-__device__ __forceinline__ float silu(float z) {
-  float s, n;
-  sigmoid_pair(z, s, n);
-  return z * s;
-}
-// z·σ(z) and its derivative σ(z)·(1 + z·σ(−z))
+__device__ __forceinline__ float silu(float z) { return z * __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+// z·σ(z) and its derivative σ(z)·(1 + z·(1 − σ(z)))
 __device__ __forceinline__ void silu_pair(float z, float& f, float& df) {
-  float s, n;
-  sigmoid_pair(z, s, n);
+  const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
   f = z * s;
-  df = s * (1.f + z * n);
+  df = s * (1.f + z * (1.f - s));
 }
 
 struct Geo {
@@ -79,10 +76,10 @@ struct Geo {
   __device__ __forceinline__ int64_t at(int64_t t) const { return reverse ? T - 1 - t : t; }
 };
 
-// this block's (sequence, segment, first channel)
+// this block's (sequence, segment, first channel) and this thread's channels and time lane
 struct Place {
   int64_t b, k0, k1;
-  int seg, c0;
+  int seg, c0, wave, half, lt, cl, c, n;
 };
 __device__ __forceinline__ Place place(const Geo& g) {
   Place p;
@@ -93,46 +90,103 @@ __device__ __forceinline__ Place place(const Geo& g) {
   p.b = id / g.segs;
   p.k0 = p.seg * g.per_seg;
   p.k1 = p.k0 + g.per_seg < g.chunks ? p.k0 + g.per_seg : g.chunks;
+  p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  p.half = (threadIdx.x >> 5) & 1;
+  p.lt = p.wave * 2 + p.half;
+  p.cl = (threadIdx.x % kLC) * kVC;
+  p.c = p.c0 + p.cl;
+  p.n = g.C - p.c;
   return p;
+}
+
+// Where this lane's steps of chunk k lie: a wave-uniform address per step (of the chunk's lowest
+// position in memory, which a chunk cut off by the sequence's end may place before the tensor) plus
+// one 32-bit offset of the lane — per-lane 64-bit addresses of every step and tensor would fill the
+// registers.  Steps behind the end and channels behind C read as `fill` and are not written.
+template <typename T>
+struct Steps {
+  T* base;
+  unsigned off;
+  int64_t st;
+  __device__ __forceinline__ Steps(T* q, int64_t sb, int64_t st_, const Geo& g, const Place& p, int64_t k) : st(st_) {
+    const int64_t low = g.reverse ? g.T - (k + 1) * kChunk : k * kChunk;
+    base = q + (p.b * sb + low * st + p.c0);
+    off = (unsigned)(g.reverse ? kChunk - (p.lt + 1) * kS : p.lt * kS) * (unsigned)st + p.cl;
+  }
+  __device__ __forceinline__ T* at(const Geo& g, int s) const { return base + (g.reverse ? kS - 1 - s : s) * st + off; }
+};
+template <typename T>
+__device__ __forceinline__ void load_steps(const Strided<T>& q, const Geo& g, const Place& p, int64_t k, bool whole, float fill,
+                                           Words<T, kVC> (&r)[kS]) {
+  const Steps<const T> a(q.p, q.sb, q.st, g, p, k);
+  if (whole) {
+#pragma unroll
+    for (int s = 0; s < kS; s++) __builtin_memcpy(&r[s], a.at(g, s), sizeof(r[s]));
+  } else {
+    const int64_t left = g.T - (k * kChunk + p.lt * kS);
+#pragma unroll
+    for (int s = 0; s < kS; s++)
+      if (s < left && p.n > 0) {
+        r[s] = group_load<kVC>(a.at(g, s), p.n, fill);
+      } else {
+#pragma unroll
+        for (int v = 0; v < kVC; v++) r[s].set(v, fill);
+      }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_step(const Steps<T>& a, const Geo& g, const Place& p, int64_t k, bool whole, int s,
+                                           const Words<T, kVC>& r) {
+  if (whole) __builtin_memcpy(a.at(g, s), &r, sizeof(r));
+  else if (k * kChunk + p.lt * kS + s < g.T && p.n > 0) group_store<kVC>(a.at(g, s), p.n, r);
+}
+__device__ __forceinline__ bool whole_chunk(const Geo& g, const Place& p, int64_t k) {
+  return (k + 1) * kChunk <= g.T && p.c0 + kCT <= g.C;
+}
+
+// values of the lower and the upper half wave, in every lane
+__device__ __forceinline__ void halves(float v, float& lo, float& hi) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  lo = __builtin_bit_cast(float, (unsigned)r[0]);
+  hi = __builtin_bit_cast(float, (unsigned)r[1]);
 }
 
 // ---- segment maps: (P, E) of each segment, agg [B][segs][2][C] --------------------------------
 // Each time lane walks one contiguous span of the segment, so the lanes join once, at its end.
 // BWD: the map of Q from the segment's end to its start (E from dy, z); else that of h (E from x).
-template <typename T, bool BWD, int LT>
-__global__ __launch_bounds__(kLC* LT) void recur_segment_kernel(Strided<T> e, Strided<T> d, Strided<T> z, Geo g, float* agg) {
-  __shared__ float sP[LT][kCT], sE[LT][kCT];
-  const Place pl = place(g);
-  const int cl = threadIdx.x % kLC, lt = threadIdx.x / kLC, c = pl.c0 + cl * kVC, n = g.C - c;
-  const int64_t first = pl.k0 * kChunk, end = pl.k1 * kChunk < g.T ? pl.k1 * kChunk : g.T;
-  const int64_t span = (end - first + LT - 1) / LT;
-  const int64_t t0 = first + lt * span, t1 = t0 + span < end ? t0 + span : end;
+template <typename T, bool BWD>
+__global__ __launch_bounds__(kThreads) void recur_segment_kernel(Strided<T> e, Strided<T> d, Strided<T> z, Geo g, float* agg) {
+  __shared__ float sP[kLT][kCT], sE[kLT][kCT];
+  const Place p = place(g);
+  const int64_t first = p.k0 * kChunk, end = p.k1 * kChunk < g.T ? p.k1 * kChunk : g.T;
+  const int64_t span = (end - first + kLT - 1) / kLT;
+  const int64_t t0 = first + p.lt * span, t1 = t0 + span < end ? t0 + span : end;
   float P[kVC], E[kVC];
 #pragma unroll
   for (int v = 0; v < kVC; v++) P[v] = 1.f, E[v] = 0.f;
-  if (n > 0) {
-    const T *ep = e.p + pl.b * e.sb + c, *dp = d.p + pl.b * d.sb + c, *zp = z.p ? z.p + pl.b * z.sb + c : nullptr;
+  if (p.n > 0) {
+    const T *ep = e.p + p.b * e.sb + p.c, *dp = d.p + p.b * d.sb + p.c, *zp = z.p ? z.p + p.b * z.sb + p.c : nullptr;
     constexpr int U = 8;
     for (int64_t t = t0; t < t1; t += U) {
-      Quad<T> qe[U], qd[U], qz[U];
+      Words<T, kVC> qe[U], qd[U], qz[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        int64_t k = t + u < t1 ? t + u : t1 - 1;
+      for (int w = 0; w < U; w++) {
+        int64_t k = t + w < t1 ? t + w : t1 - 1;
         if constexpr (BWD) k = t0 + t1 - 1 - k;                       // from the span's end to its start
         k = g.at(k);
-        qe[u] = quad_load(ep + k * e.st, n);
-        qd[u] = quad_load(dp + k * d.st, n);
-        if (BWD && zp) qz[u] = quad_load(zp + k * z.st, n);
+        qe[w] = group_load<kVC>(ep + k * e.st, p.n);
+        qd[w] = group_load<kVC>(dp + k * d.st, p.n);
+        if (BWD && zp) qz[w] = group_load<kVC>(zp + k * z.st, p.n);
       }
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        if (t + u < t1) {
+      for (int w = 0; w < U; w++)
+        if (t + w < t1) {
 #pragma unroll
           for (int v = 0; v < kVC; v++) {
             float a, i;
-            sigmoid_pair((float)qd[u].v[v], a, i);
-            const float in = (float)qe[u].v[v];
-            if constexpr (BWD) E[v] = a * (E[v] + (zp ? in * silu((float)qz[u].v[v]) : in));
+            sigmoid_pair(qd[w].get(v), a, i);
+            const float in = qe[w].get(v);
+            if constexpr (BWD) E[v] = a * (E[v] + (zp ? in * silu(qz[w].get(v)) : in));
             else E[v] = a * E[v] + i * in;
             P[v] *= a;
           }
@@ -140,276 +194,309 @@ __global__ __launch_bounds__(kLC* LT) void recur_segment_kernel(Strided<T> e, St
     }
   }
 #pragma unroll
-  for (int v = 0; v < kVC; v++) sP[lt][cl * kVC + v] = P[v], sE[lt][cl * kVC + v] = E[v];
+  for (int v = 0; v < kVC; v++) sP[p.lt][p.cl + v] = P[v], sE[p.lt][p.cl + v] = E[v];
   __syncthreads();
-  for (int ch = threadIdx.x; ch < kCT; ch += kLC * LT) {
-    if (pl.c0 + ch >= g.C) continue;
-    float p = 1.f, s = 0.f;
+  if (threadIdx.x < kCT && p.c0 + (int)threadIdx.x < g.C) {
+    const int ch = threadIdx.x;
+    float m = 1.f, s = 0.f;
 #pragma unroll
-    for (int j = 0; j < LT; j++) {
-      const int l = BWD ? LT - 1 - j : j;
+    for (int j = 0; j < kLT; j++) {
+      const int l = BWD ? kLT - 1 - j : j;
       s = sP[l][ch] * s + sE[l][ch];
-      p *= sP[l][ch];
+      m *= sP[l][ch];
     }
-    float* out = agg + ((pl.b * g.segs + pl.seg) * 2) * g.C + pl.c0 + ch;
-    out[0] = p;
+    float* out = agg + ((p.b * g.segs + p.seg) * 2) * g.C + p.c0 + ch;
+    out[0] = m;
     out[g.C] = s;
   }
 }
 
-// the state entering this block's segment: `s` run through the maps before it
+// The state entering this block's segment in each lane's channels: `s0` [B][C] (or null: 0) run
+// through the maps of the segments before it (BWD: behind it).  Eight threads a channel take a
+// contiguous part of those maps each.  Ends with a barrier.
 template <bool BWD>
-__device__ __forceinline__ float enter_segment(const float* agg, const Geo& g, const Place& pl, int ch, float s) {
-  const float* q = agg + pl.b * g.segs * 2 * (int64_t)g.C + pl.c0 + ch;
-  if constexpr (BWD) {
-    for (int k = g.segs - 1; k > pl.seg; k--) s = q[2 * (int64_t)k * g.C] * s + q[(2 * (int64_t)k + 1) * g.C];
-  } else {
-    for (int k = 0; k < pl.seg; k++) s = q[2 * (int64_t)k * g.C] * s + q[(2 * (int64_t)k + 1) * g.C];
+__device__ __forceinline__ void enter(const float* s0, const float* agg, const Geo& g, const Place& p, float (&state)[kVC]) {
+  __shared__ float fP[kWaves][kCT], fE[kWaves][kCT];
+  if (!agg) {
+#pragma unroll
+    for (int v = 0; v < kVC; v++) state[v] = s0 && v < p.n ? s0[p.b * g.C + p.c + v] : 0.f;
+    return;
   }
-  return s;
+  const int ch = threadIdx.x & 63, lo = BWD ? p.seg + 1 : 0, cnt = BWD ? g.segs - 1 - p.seg : p.seg;
+  const int part = (cnt + kWaves - 1) / kWaves, j0 = p.wave * part, j1 = j0 + part < cnt ? j0 + part : cnt;
+  float m = 1.f, s = 0.f;
+  if (p.c0 + ch < g.C) {
+    const float* q = agg + (p.b * g.segs + lo) * 2 * (int64_t)g.C + p.c0 + ch;
+#pragma unroll 4
+    for (int j = j0; j < j1; j++) {
+      const int64_t o = 2 * (int64_t)(BWD ? cnt - 1 - j : j) * g.C;
+      const float pj = q[o], ej = q[o + g.C];
+      s = pj * s + ej;
+      m *= pj;
+    }
+  }
+  fP[p.wave][ch] = m;
+  fE[p.wave][ch] = s;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < kVC; v++) {
+    float h = s0 && v < p.n ? s0[p.b * g.C + p.c + v] : 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) h = fP[w][p.cl + v] * h + fE[w][p.cl + v];
+    state[v] = h;
+  }
 }
 
 // ---- forward ----------------------------------------------------------------------------------
-template <typename T, int LT>
-__global__ __launch_bounds__(kLC* LT) void recur_fwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, const float* h0, Geo g,
-                                                            const float* agg, T* y, float* last, float* carry) {
-  constexpr int S = kChunk / LT;
+template <typename T, bool GATE>
+__global__ __launch_bounds__(kThreads) void recur_fwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, const float* h0, Geo g,
+                                                             const float* agg, T* y, float* last, float* carry) {
   // two sets: a chunk's maps are written while slower waves still read those of the chunk before
-  __shared__ __attribute__((aligned(16))) float sP[2][LT][kCT], sE[2][LT][kCT], sH[2][kCT];
-  const Place pl = place(g);
-  const int cl = threadIdx.x % kLC, lt = threadIdx.x / kLC, c = pl.c0 + cl * kVC, n = g.C - c;
-  if (threadIdx.x < kCT) {
-    const int ch = pl.c0 + threadIdx.x;
-    float s = 0.f;
-    if (ch < g.C) {
-      if (h0) s = h0[pl.b * g.C + ch];
-      if (agg) s = enter_segment<false>(agg, g, pl, threadIdx.x, s);
-    }
-    sH[pl.k0 & 1][threadIdx.x] = s;
-  }
-  const T *xp = x.p + pl.b * x.sb + c, *dp = d.p + pl.b * d.sb + c, *zp = z.p ? z.p + pl.b * z.sb + c : nullptr;
-  T* yp = y + pl.b * g.T * g.C + c;
-  for (int64_t k = pl.k0; k < pl.k1; k++) {
+  __shared__ float sP[2][kWaves][kCT], sE[2][kWaves][kCT];
+  const Place p = place(g);
+  float state[kVC];                                                   // entering the chunk
+  enter<false>(h0, agg, g, p, state);
+  Words<T, kVC> nx[kS], nd[kS], nz[kS];
+  auto fetch = [&](int64_t k) {
+    const bool whole = whole_chunk(g, p, k);
+    load_steps(x, g, p, k, whole, 0.f, nx);
+    load_steps(d, g, p, k, whole, __builtin_inff(), nd);
+    if constexpr (GATE) load_steps(z, g, p, k, whole, 0.f, nz);
+  };
+  if (p.k0 < p.k1) fetch(p.k0);
+  for (int64_t k = p.k0; k < p.k1; k++) {
     const int par = k & 1;
-    const int64_t t0 = k * kChunk + lt * S;
-    Quad<T> qx[S], qd[S], qz[S];
-    if (n > 0) {
-#pragma unroll
-      for (int s = 0; s < S; s++)
-        if (t0 + s < g.T) {
-          const int64_t t = g.at(t0 + s);
-          qx[s] = quad_load(xp + t * x.st, n);
-          qd[s] = quad_load(dp + t * d.st, n);
-          if (zp) qz[s] = quad_load(zp + t * z.st, n);
-        }
-    }
-    float A[S][kVC], Bx[S][kVC], P[kVC], E[kVC];
+    float A[kS][kVC], I[kS][kVC], F[kS][kVC], P[kVC], E[kVC];
 #pragma unroll
     for (int v = 0; v < kVC; v++) P[v] = 1.f, E[v] = 0.f;
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-      const bool in = n > 0 && t0 + s < g.T;                          // past the end: the identity
+    for (int s = 0; s < kS; s++)
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        float a, i;
-        sigmoid_pair((float)qd[s].v[v], a, i);
-        A[s][v] = in ? a : 1.f;
-        Bx[s][v] = in ? i * (float)qx[s].v[v] : 0.f;
-        E[v] = A[s][v] * E[v] + Bx[s][v];
+        sigmoid_pair(nd[s].get(v), A[s][v], I[s][v]);
+        I[s][v] *= nx[s].get(v);
+        E[v] = A[s][v] * E[v] + I[s][v];
         P[v] *= A[s][v];
+        if constexpr (GATE) F[s][v] = nz[s].get(v);
+      }
+    if (k + 1 < p.k1) fetch(k + 1);
+    float Pl[kVC], El[kVC];                                           // of the lower half: what enters the upper one
+#pragma unroll
+    for (int v = 0; v < kVC; v++) {
+      float Ph, Eh;
+      halves(P[v], Pl[v], Ph);
+      halves(E[v], El[v], Eh);
+      if (p.half == 0) {
+        sP[par][p.wave][p.cl + v] = Pl[v] * Ph;
+        sE[par][p.wave][p.cl + v] = Ph * El[v] + Eh;
       }
     }
-#pragma unroll
-    for (int v = 0; v < kVC; v++) sP[par][lt][cl * kVC + v] = P[v], sE[par][lt][cl * kVC + v] = E[v];
     __syncthreads();
-    float h[kVC];
-#pragma unroll
-    for (int v = 0; v < kVC; v++) h[v] = sH[par][cl * kVC + v];
-    if (carry && lt == 0) {
+    if (carry && p.wave == 0 && p.half == 0) {
 #pragma unroll
       for (int v = 0; v < kVC; v++)
-        if (v < n) carry[(pl.b * g.chunks + k) * g.C + c + v] = h[v];
+        if (v < p.n) carry[(p.b * g.chunks + k) * g.C + p.c + v] = state[v];
     }
-    for (int j = 0; j < lt; j++)
+    float h[kVC];
 #pragma unroll
-      for (int v = 0; v < kVC; v++) h[v] = sP[par][j][cl * kVC + v] * h[v] + sE[par][j][cl * kVC + v];
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-      Quad<T> o;
+    for (int w = 0; w < kWaves; w++) {
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        h[v] = A[s][v] * h[v] + Bx[s][v];
-        o.v[v] = (T)(zp ? h[v] * silu((float)qz[s].v[v]) : h[v]);
+        if (w == p.wave) h[v] = state[v];
+        state[v] = sP[par][w][p.cl + v] * state[v] + sE[par][w][p.cl + v];
       }
-      if (n > 0 && t0 + s < g.T) quad_store(yp + g.at(t0 + s) * g.C, n, o);
     }
-    if (lt == LT - 1) {
+#pragma unroll
+    for (int v = 0; v < kVC; v++) h[v] = p.half ? Pl[v] * h[v] + El[v] : h[v];
+    const bool whole = whole_chunk(g, p, k);
+    const Steps<T> at(y, g.T * g.C, g.C, g, p, k);
+#pragma unroll
+    for (int s = 0; s < kS; s++) {
+      Words<T, kVC> o;
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        sH[par ^ 1][cl * kVC + v] = h[v];
-        if (k == g.chunks - 1 && v < n) last[pl.b * g.C + c + v] = h[v];
+        h[v] = A[s][v] * h[v] + I[s][v];
+        o.set(v, GATE ? h[v] * silu(F[s][v]) : h[v]);
       }
+      store_step(at, g, p, k, whole, s, o);
     }
+  }
+  if (p.k1 == g.chunks && threadIdx.x < kLC) {
+#pragma unroll
+    for (int v = 0; v < kVC; v++)
+      if (v < p.n) last[p.b * g.C + p.c + v] = state[v];
   }
 }
 
 // ---- backward ---------------------------------------------------------------------------------
-template <typename T, int LT>
-__global__ __launch_bounds__(kLC* LT) void recur_bwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, Strided<T> dy,
-                                                            const float* carry, const float* dlast, Geo g, const float* agg,
-                                                            T* dx, T* dd, T* dz, float* dh0) {
-  constexpr int S = kChunk / LT;
-  __shared__ __attribute__((aligned(16))) float sP[2][LT][kCT], sE[2][LT][kCT], sQ[2][LT][kCT], sG[2][kCT];
-  const Place pl = place(g);
-  const int cl = threadIdx.x % kLC, lt = threadIdx.x / kLC, c = pl.c0 + cl * kVC, n = g.C - c;
-  if (threadIdx.x < kCT) {
-    const int ch = pl.c0 + threadIdx.x;
-    float s = 0.f;
-    if (ch < g.C) {
-      if (dlast) s = dlast[pl.b * g.C + ch];
-      if (agg) s = enter_segment<true>(agg, g, pl, threadIdx.x, s);
-    }
-    sG[(pl.k1 - 1) & 1][threadIdx.x] = s;
-  }
-  const T *xp = x.p + pl.b * x.sb + c, *dp = d.p + pl.b * d.sb + c, *yp = dy.p + pl.b * dy.sb + c;
-  const T* zp = z.p ? z.p + pl.b * z.sb + c : nullptr;
-  const int64_t ob = pl.b * g.T * g.C + c;
-  for (int64_t k = pl.k1 - 1; k >= pl.k0; k--) {
+template <typename T, bool GATE>
+__global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, Strided<T> dy,
+                                                             const float* carry, const float* dlast, Geo g, const float* agg,
+                                                             T* dx, T* dd, T* dz, float* dh0) {
+  // a and i of a step stay in registers, or (fp32 tensors, whose operands take twice the registers)
+  // are computed again from d where they are used
+  constexpr bool kHold = sizeof(T) == 2;
+  __shared__ float sP[2][kWaves][kCT], sE[2][kWaves][kCT], sQ[2][kWaves][kCT];
+  const Place p = place(g);
+  float state[kVC];                                                   // Q entering the chunk from its end
+  enter<true>(dlast, agg, g, p, state);
+  Words<T, kVC> nx[kS], nd[kS], nz[kS], ny[kS];
+  float nh[kVC];
+  auto fetch = [&](int64_t k) {
+    const bool whole = whole_chunk(g, p, k);
+    load_steps(x, g, p, k, whole, 0.f, nx);
+    load_steps(d, g, p, k, whole, __builtin_inff(), nd);
+    load_steps(dy, g, p, k, whole, 0.f, ny);
+    if constexpr (GATE) load_steps(z, g, p, k, whole, 0.f, nz);
+#pragma unroll
+    for (int v = 0; v < kVC; v++) nh[v] = v < p.n ? carry[(p.b * g.chunks + k) * g.C + p.c + v] : 0.f;
+  };
+  if (p.k0 < p.k1) fetch(p.k1 - 1);
+  for (int64_t k = p.k1 - 1; k >= p.k0; k--) {
     const int par = k & 1;
-    const int64_t t0 = k * kChunk + lt * S;
-    Quad<T> qx[S], qd[S], qz[S], qy[S];
-    float hin[kVC];
+    Words<T, kVC> cx[kS], cd[kHold ? 1 : kS];
+    float A[kHold ? kS : 1][kVC], I[kHold ? kS : 1][kVC], top[kS][kVC], yf[kS][kVC], P[kVC], E[kVC], Q[kVC], h[kVC];
+    auto pair = [&](int s, int v, float& a, float& i) {
+      if constexpr (kHold) a = A[s][v], i = I[s][v];
+      else {
+        float t = cd[s].get(v);
+        asm volatile("" : "+v"(t));                                    // else the first pair is kept after all
+        sigmoid_pair(t, a, i);
+      }
+    };
 #pragma unroll
-    for (int v = 0; v < kVC; v++) hin[v] = 0.f;
-    if (n > 0) {
+    for (int v = 0; v < kVC; v++) P[v] = 1.f, E[v] = Q[v] = 0.f, h[v] = nh[v];
 #pragma unroll
-      for (int s = 0; s < S; s++)
-        if (t0 + s < g.T) {
-          const int64_t t = g.at(t0 + s);
-          qx[s] = quad_load(xp + t * x.st, n);
-          qd[s] = quad_load(dp + t * d.st, n);
-          qy[s] = quad_load(yp + t * dy.st, n);
-          if (zp) qz[s] = quad_load(zp + t * z.st, n);
-        }
-#pragma unroll
-      for (int v = 0; v < kVC; v++)
-        if (v < n) hin[v] = carry[(pl.b * g.chunks + k) * g.C + c + v];
-    }
-    float A[S][kVC], P[kVC], E[kVC], Q[kVC];
-#pragma unroll
-    for (int v = 0; v < kVC; v++) P[v] = 1.f, E[v] = 0.f, Q[v] = 0.f;
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-      const bool in = n > 0 && t0 + s < g.T;
+    for (int s = 0; s < kS; s++) {
+      cx[s] = nx[s];
+      if constexpr (!kHold) cd[s] = nd[s];
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
         float a, i;
-        sigmoid_pair((float)qd[s].v[v], a, i);
-        A[s][v] = in ? a : 1.f;
-        E[v] = A[s][v] * E[v] + (in ? i * (float)qx[s].v[v] : 0.f);
-        P[v] *= A[s][v];
+        sigmoid_pair(nd[s].get(v), a, i);
+        if constexpr (kHold) A[s][v] = a, I[s][v] = i;
+        E[v] = a * E[v] + i * nx[s].get(v);
+        P[v] *= a;
+        const float g_out = ny[s].get(v);
+        if constexpr (GATE) {
+          float f, df;
+          silu_pair(nz[s].get(v), f, df);
+          top[s][v] = g_out * f;
+          yf[s][v] = g_out * df;
+        } else {
+          top[s][v] = g_out;
+        }
       }
     }
+    if (k > p.k0) fetch(k - 1);
 #pragma unroll
-    for (int s = S - 1; s >= 0; s--) {
-      const bool in = n > 0 && t0 + s < g.T;
+    for (int s = kS - 1; s >= 0; s--)
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        float top = (float)qy[s].v[v];
-        if (zp) top *= silu((float)qz[s].v[v]);
-        Q[v] = A[s][v] * (Q[v] + (in ? top : 0.f));
+        float a, i;
+        pair(s, v, a, i);
+        Q[v] = a * (Q[v] + top[s][v]);
       }
-    }
+    float Pl[kVC], El[kVC], Ph[kVC], Qh[kVC];
 #pragma unroll
     for (int v = 0; v < kVC; v++) {
-      sP[par][lt][cl * kVC + v] = P[v];
-      sE[par][lt][cl * kVC + v] = E[v];
-      sQ[par][lt][cl * kVC + v] = Q[v];
+      float Eh, Ql;
+      halves(P[v], Pl[v], Ph[v]);
+      halves(E[v], El[v], Eh);
+      halves(Q[v], Ql, Qh[v]);
+      if (p.half == 0) {
+        sP[par][p.wave][p.cl + v] = Pl[v] * Ph[v];
+        sE[par][p.wave][p.cl + v] = Ph[v] * El[v] + Eh;
+        sQ[par][p.wave][p.cl + v] = Pl[v] * Qh[v] + Ql;
+      }
     }
     __syncthreads();
     float q[kVC];
 #pragma unroll
-    for (int v = 0; v < kVC; v++) q[v] = sG[par][cl * kVC + v];
-    for (int j = 0; j < lt; j++)
+    for (int w = 0; w < kWaves; w++) {
 #pragma unroll
-      for (int v = 0; v < kVC; v++) hin[v] = sP[par][j][cl * kVC + v] * hin[v] + sE[par][j][cl * kVC + v];
-    for (int j = LT - 1; j > lt; j--)
+      for (int v = 0; v < kVC; v++) {
+        if (w < p.wave) h[v] = sP[par][w][p.cl + v] * h[v] + sE[par][w][p.cl + v];
+        const int r = kWaves - 1 - w;
+        if (r == p.wave) q[v] = state[v];
+        state[v] = sP[par][r][p.cl + v] * state[v] + sQ[par][r][p.cl + v];
+      }
+    }
 #pragma unroll
-      for (int v = 0; v < kVC; v++) q[v] = sP[par][j][cl * kVC + v] * q[v] + sQ[par][j][cl * kVC + v];
-    float H[S][kVC];                                                   // the state before each step
+    for (int v = 0; v < kVC; v++) {
+      h[v] = p.half ? Pl[v] * h[v] + El[v] : h[v];
+      q[v] = p.half ? q[v] : Ph[v] * q[v] + Qh[v];
+    }
+    float H[kS][kVC];                                                  // the state before each step
 #pragma unroll
-    for (int s = 0; s < S; s++)
+    for (int s = 0; s < kS; s++)
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
         float a, i;
-        sigmoid_pair((float)qd[s].v[v], a, i);
-        H[s][v] = hin[v];
-        hin[v] = A[s][v] * hin[v] + i * (float)qx[s].v[v];
+        pair(s, v, a, i);
+        H[s][v] = h[v];
+        h[v] = a * h[v] + i * cx[s].get(v);
       }
+    const bool whole = whole_chunk(g, p, k);
+    const int64_t sb = g.T * g.C;
+    const Steps<T> ax(dx, sb, g.C, g, p, k), ad(dd, sb, g.C, g, p, k), az(dz, sb, g.C, g, p, k);
 #pragma unroll
-    for (int s = S - 1; s >= 0; s--) {
-      const bool in = n > 0 && t0 + s < g.T;
-      Quad<T> ox, od, oz;
-#pragma unroll
-      for (int v = 0; v < kVC; v++) {
-        float a, i, f = 1.f, df = 0.f;
-        sigmoid_pair((float)qd[s].v[v], a, i);
-        const float xv = (float)qx[s].v[v], yv = (float)qy[s].v[v];
-        if (zp) silu_pair((float)qz[s].v[v], f, df);
-        const float G = q[v] + yv * f;
-        ox.v[v] = (T)(G * i);
-        od.v[v] = (T)(G * (H[s][v] - xv) * a * i);
-        oz.v[v] = (T)(yv * (a * H[s][v] + i * xv) * df);
-        if (in) q[v] = a * G;
-      }
-      if (in) {
-        const int64_t o = ob + g.at(t0 + s) * g.C;
-        if (dx) quad_store(dx + o, n, ox);
-        if (dd) quad_store(dd + o, n, od);
-        if (dz) quad_store(dz + o, n, oz);
-      }
-    }
-    if (lt == 0) {
+    for (int s = kS - 1; s >= 0; s--) {
+      Words<T, kVC> ox, od, oz;
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        sG[par ^ 1][cl * kVC + v] = q[v];
-        if (k == 0 && dh0 && v < n) dh0[pl.b * g.C + c + v] = q[v];
+        float a, i;
+        pair(s, v, a, i);
+        const float xv = cx[s].get(v), G = q[v] + top[s][v], Gi = G * i;
+        ox.set(v, Gi);
+        od.set(v, Gi * (H[s][v] - xv) * a);
+        if constexpr (GATE) oz.set(v, yf[s][v] * (a * H[s][v] + i * xv));
+        q[v] = a * G;
       }
+      if (dx) store_step(ax, g, p, k, whole, s, ox);
+      if (dd) store_step(ad, g, p, k, whole, s, od);
+      if constexpr (GATE)
+        if (dz) store_step(az, g, p, k, whole, s, oz);
     }
+  }
+  if (p.k0 == 0 && dh0 && threadIdx.x < kLC) {
+#pragma unroll
+    for (int v = 0; v < kVC; v++)
+      if (v < p.n) dh0[p.b * g.C + p.c + v] = state[v];
   }
 }
 
 // ---- short sequences --------------------------------------------------------------------------
-// A thread walks kVC channels of a whole sequence (T ≤ kShort, one position of a stream above all):
-// no joins, B·C/kVC threads.
+// A thread walks kShortVC channels of a whole sequence (T ≤ kShort, one position of a stream above all):
+// no joins, B·C/kShortVC threads.
 template <typename T>
 __global__ __launch_bounds__(128) void recur_fwd_short_kernel(Strided<T> x, Strided<T> d, Strided<T> z, const float* h0, Geo g,
                                                               T* y, float* last, float* carry) {
   const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x, b = id / g.tiles;
   if (b >= g.B) return;
-  const int c = (int)(id % g.tiles) * kVC, n = g.C - c;
-  float h[kVC];
+  const int c = (int)(id % g.tiles) * kShortVC, n = g.C - c;
+  float h[kShortVC];
 #pragma unroll
-  for (int v = 0; v < kVC; v++) {
+  for (int v = 0; v < kShortVC; v++) {
     h[v] = h0 && v < n ? h0[b * g.C + c + v] : 0.f;
     if (carry && v < n) carry[b * g.C + c + v] = h[v];
   }
   for (int64_t k = 0; k < g.T; k++) {
     const int64_t t = g.at(k);
-    const Quad<T> qx = quad_load(x.p + b * x.sb + t * x.st + c, n), qd = quad_load(d.p + b * d.sb + t * d.st + c, n);
-    Quad<T> qz, o;
-    if (z.p) qz = quad_load(z.p + b * z.sb + t * z.st + c, n);
+    const Words<T, kShortVC> qx = group_load<kShortVC>(x.p + b * x.sb + t * x.st + c, n), qd = group_load<kShortVC>(d.p + b * d.sb + t * d.st + c, n);
+    Words<T, kShortVC> qz, o;
+    if (z.p) qz = group_load<kShortVC>(z.p + b * z.sb + t * z.st + c, n);
 #pragma unroll
-    for (int v = 0; v < kVC; v++) {
+    for (int v = 0; v < kShortVC; v++) {
       float a, i;
-      sigmoid_pair((float)qd.v[v], a, i);
-      h[v] = a * h[v] + i * (float)qx.v[v];
-      o.v[v] = (T)(z.p ? h[v] * silu((float)qz.v[v]) : h[v]);
+      sigmoid_pair(qd.get(v), a, i);
+      h[v] = a * h[v] + i * qx.get(v);
+      o.set(v, z.p ? h[v] * silu(qz.get(v)) : h[v]);
     }
-    quad_store(y + (b * g.T + t) * g.C + c, n, o);
+    group_store<kShortVC>(y + (b * g.T + t) * g.C + c, n, o);
   }
 #pragma unroll
-  for (int v = 0; v < kVC; v++)
+  for (int v = 0; v < kShortVC; v++)
     if (v < n) last[b * g.C + c + v] = h[v];
 }
 
@@ -419,10 +506,10 @@ __global__ __launch_bounds__(128) void recur_bwd_short_kernel(Strided<T> x, Stri
                                                               T* dz, float* dh0) {
   const int64_t id = (int64_t)blockIdx.x * 128 + threadIdx.x, b = id / g.tiles;
   if (b >= g.B) return;
-  const int c = (int)(id % g.tiles) * kVC, n = g.C - c;
-  float H[kShort][kVC], h[kVC], q[kVC];
+  const int c = (int)(id % g.tiles) * kShortVC, n = g.C - c;
+  float H[kShort][kShortVC], h[kShortVC], q[kShortVC];
 #pragma unroll
-  for (int v = 0; v < kVC; v++) {
+  for (int v = 0; v < kShortVC; v++) {
     h[v] = v < n ? carry[b * g.C + c + v] : 0.f;
     q[v] = dlast && v < n ? dlast[b * g.C + c + v] : 0.f;
   }
@@ -430,56 +517,56 @@ __global__ __launch_bounds__(128) void recur_bwd_short_kernel(Strided<T> x, Stri
   for (int k = 0; k < kShort; k++)
     if (k < g.T) {
       const int64_t t = g.at(k);
-      const Quad<T> qx = quad_load(x.p + b * x.sb + t * x.st + c, n), qd = quad_load(d.p + b * d.sb + t * d.st + c, n);
+      const Words<T, kShortVC> qx = group_load<kShortVC>(x.p + b * x.sb + t * x.st + c, n), qd = group_load<kShortVC>(d.p + b * d.sb + t * d.st + c, n);
 #pragma unroll
-      for (int v = 0; v < kVC; v++) {
+      for (int v = 0; v < kShortVC; v++) {
         float a, i;
-        sigmoid_pair((float)qd.v[v], a, i);
+        sigmoid_pair(qd.get(v), a, i);
         H[k][v] = h[v];
-        h[v] = a * h[v] + i * (float)qx.v[v];
+        h[v] = a * h[v] + i * qx.get(v);
       }
     }
 #pragma unroll
   for (int k = kShort - 1; k >= 0; k--)
     if (k < g.T) {
       const int64_t t = g.at(k);
-      const Quad<T> qx = quad_load(x.p + b * x.sb + t * x.st + c, n), qd = quad_load(d.p + b * d.sb + t * d.st + c, n),
-                    qy = quad_load(dy.p + b * dy.sb + t * dy.st + c, n);
-      Quad<T> qz, ox, od, oz;
-      if (z.p) qz = quad_load(z.p + b * z.sb + t * z.st + c, n);
+      const Words<T, kShortVC> qx = group_load<kShortVC>(x.p + b * x.sb + t * x.st + c, n), qd = group_load<kShortVC>(d.p + b * d.sb + t * d.st + c, n),
+                    qy = group_load<kShortVC>(dy.p + b * dy.sb + t * dy.st + c, n);
+      Words<T, kShortVC> qz, ox, od, oz;
+      if (z.p) qz = group_load<kShortVC>(z.p + b * z.sb + t * z.st + c, n);
 #pragma unroll
-      for (int v = 0; v < kVC; v++) {
+      for (int v = 0; v < kShortVC; v++) {
         float a, i, f = 1.f, df = 0.f;
-        sigmoid_pair((float)qd.v[v], a, i);
-        const float xv = (float)qx.v[v], yv = (float)qy.v[v];
-        if (z.p) silu_pair((float)qz.v[v], f, df);
+        sigmoid_pair(qd.get(v), a, i);
+        const float xv = qx.get(v), yv = qy.get(v);
+        if (z.p) silu_pair(qz.get(v), f, df);
         const float G = q[v] + yv * f;
-        ox.v[v] = (T)(G * i);
-        od.v[v] = (T)(G * (H[k][v] - xv) * a * i);
-        oz.v[v] = (T)(yv * (a * H[k][v] + i * xv) * df);
+        ox.set(v, G * i);
+        od.set(v, G * (H[k][v] - xv) * a * i);
+        oz.set(v, yv * (a * H[k][v] + i * xv) * df);
         q[v] = a * G;
       }
       const int64_t o = (b * g.T + t) * g.C + c;
-      if (dx) quad_store(dx + o, n, ox);
-      if (dd) quad_store(dd + o, n, od);
-      if (dz) quad_store(dz + o, n, oz);
+      if (dx) group_store<kShortVC>(dx + o, n, ox);
+      if (dd) group_store<kShortVC>(dd + o, n, od);
+      if (dz) group_store<kShortVC>(dz + o, n, oz);
     }
   if (dh0) {
 #pragma unroll
-    for (int v = 0; v < kVC; v++)
+    for (int v = 0; v < kShortVC; v++)
       if (v < n) dh0[b * g.C + c + v] = q[v];
   }
 }
 
 // Segments: none once sequences × channel tiles give each of the 256 CUs a block; else as many as
-// bring the launch to about four blocks a CU, each at least four chunks long.
+// bring the launch to about two blocks a CU, each at least four chunks long.
 Geo geometry(int64_t B, int64_t T, int C, int reverse) {
   Geo g{};
   g.B = B, g.T = T, g.C = C, g.reverse = reverse;
   g.chunks = (T + kChunk - 1) / kChunk;
-  g.tiles = T <= kShort ? ceil_div(C, kVC) : ceil_div(C, kCT);
+  g.tiles = T <= kShort ? ceil_div(C, kShortVC) : ceil_div(C, kCT);
   const int64_t base = B * g.tiles;
-  int64_t segs = base >= 256 ? 1 : (1024 + base - 1) / base;
+  int64_t segs = base >= 256 ? 1 : (512 + base - 1) / base;
   if (segs > g.chunks / 4) segs = g.chunks / 4 > 0 ? g.chunks / 4 : 1;
   g.per_seg = (g.chunks + segs - 1) / segs;
   g.segs = (int)((g.chunks + g.per_seg - 1) / g.per_seg);
@@ -516,10 +603,12 @@ int recurrence_fwd(const RecurArgs& r, const float* h0, void* y, float* last, fl
       return check_launch("recurrence_fwd_short");
     }
     if (g.segs > 1) {
-      recur_segment_kernel<T, false, 16><<<grid, kLC * 16, 0, st>>>(x, d, z, g, ws);
+      recur_segment_kernel<T, false><<<grid, kThreads, 0, st>>>(x, d, z, g, ws);
       if (int rc = check_launch("recurrence_segment")) return rc;
     }
-    recur_fwd_kernel<T, 16><<<grid, kLC * 16, 0, st>>>(x, d, z, h0, g, g.segs > 1 ? ws : nullptr, yt, last, carry);
+    const float* agg = g.segs > 1 ? ws : nullptr;
+    if (r.gate) recur_fwd_kernel<T, true><<<grid, kThreads, 0, st>>>(x, d, z, h0, g, agg, yt, last, carry);
+    else recur_fwd_kernel<T, false><<<grid, kThreads, 0, st>>>(x, d, z, h0, g, agg, yt, last, carry);
     return check_launch("recurrence_fwd");
   })
   return kOk;
@@ -538,10 +627,12 @@ int recurrence_bwd(const RecurArgs& r, const float* carry, const void* dy, int64
       return check_launch("recurrence_bwd_short");
     }
     if (g.segs > 1) {
-      recur_segment_kernel<T, true, 16><<<grid, kLC * 16, 0, st>>>(gy, d, z, g, ws);
+      recur_segment_kernel<T, true><<<grid, kThreads, 0, st>>>(gy, d, z, g, ws);
       if (int rc = check_launch("recurrence_segment")) return rc;
     }
-    recur_bwd_kernel<T, 32><<<grid, kLC * 32, 0, st>>>(x, d, z, gy, carry, dlast, g, g.segs > 1 ? ws : nullptr, dxt, ddt, dzt, dh0);
+    const float* agg = g.segs > 1 ? ws : nullptr;
+    if (r.gate) recur_bwd_kernel<T, true><<<grid, kThreads, 0, st>>>(x, d, z, gy, carry, dlast, g, agg, dxt, ddt, dzt, dh0);
+    else recur_bwd_kernel<T, false><<<grid, kThreads, 0, st>>>(x, d, z, gy, carry, dlast, g, agg, dxt, ddt, dzt, dh0);
     return check_launch("recurrence_bwd");
   })
   return kOk;

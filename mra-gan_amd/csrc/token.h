@@ -30,6 +30,31 @@ __device__ __forceinline__ void store_vec(T* p, const float (&in)[N]) {
   *reinterpret_cast<Pack<T, N>*>(p) = r;
 }
 
+// N elements of T held as the 32-bit words they were loaded as (16-bit elements kept apart would take a
+// register each while they wait), read element by element
+template <typename T, int N>
+struct Words {
+  static_assert(sizeof(T) * N % 4 == 0, "");
+  uint32_t w[sizeof(T) * N / 4];
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(float, w[i]);
+    } else if constexpr (__is_same(T, __bf16)) {
+      return __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    } else {
+      return (float)__builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (i & 1) * 16));
+    }
+  }
+  __device__ __forceinline__ void set(int i, float v) {           // rounds to T; elements in order from 0
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __builtin_bit_cast(uint32_t, v);
+    } else {
+      const uint32_t b = __builtin_bit_cast(uint16_t, (T)v);
+      w[i / 2] = i & 1 ? w[i / 2] | b << 16 : b;
+    }
+  }
+};
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
