@@ -5,10 +5,9 @@
 //   dx_t = G_t·i_t,  dd_t = G_t·(h_{t−1} − x_t)·a_t·i_t,  dz_t = dy_t·h_t·silu'(z_t)
 //
 // Both recursions are products of affine maps s ↦ P·s + E, which compose associatively, so time is
-// split: a lane takes S = 8 steps of two channels in order, the two time lanes of a wave join their
-// maps in registers and the eight waves of a block through LDS (a chunk of 128 steps), and a block
-// walks over the chunks with the fp32 state of 64 channels in registers, the next chunk's loads in
-// flight.  HBM is the bound: each tensor is read or written once.  Where B and C give too few blocks
+// split: a lane takes S = 8 steps of two channels in order, the time lanes of a wave join their maps
+// in registers and the waves of a block through LDS (a chunk of 128 steps), and a block walks over
+// the chunks with the fp32 state of its channels in registers, the next chunk's loads in flight.  HBM is the bound: each tensor is read or written once.  Where B and C give too few blocks
 // to fill the chip, the chunks are also split into segments over blocks: a first launch reduces each
 // segment to its (P, E), the second starts each segment from the fold of the ones before it (its
 // inputs then come a second time, as a rule from the 256 MB cache).
@@ -21,12 +20,14 @@ namespace mragan {
 namespace {
 
 constexpr int kVC = 2;                    // channels a lane
-constexpr int kLC = 32;                   // channel lanes: 64 channels, 128 bytes of a 16-bit row
-constexpr int kCT = kLC * kVC;
-constexpr int kWaves = 8, kThreads = 64 * kWaves;
-constexpr int kLT = kWaves * 2;           // time lanes
 constexpr int kS = 8;                     // steps of a time lane
+constexpr int kLT = 16;                   // time lanes of a block
 constexpr int kChunk = kLT * kS;          // 128 steps between two carried states
+// A block's LC channel lanes: 32 (64 channels, 8 waves of 2 time lanes) or 16 (32 channels, 4 waves of 4)
+template <int LC>
+struct Shape {
+  static constexpr int kCT = LC * kVC, kThreads = LC * kLT, kWaves = kThreads / 64;
+};
 constexpr int kShort = 16;                // sequences up to this long: a thread walks the whole sequence
 constexpr int kShortVC = 4;               // of this many channels
 
@@ -67,10 +68,15 @@ __device__ __forceinline__ void silu_pair(float z, float& f, float& df) {
   df = s * (1.f + z * (1.f - s));
 }
 
+template <bool V>
+struct Bool {
+  static constexpr bool value = V;
+};
+
 struct Geo {
   int64_t B, T;
   int C, reverse;
-  int tiles;                    // channel tiles
+  int lc, tiles;                // channel lanes of a block, channel tiles
   int64_t chunks, per_seg;      // chunks of a sequence, chunks of a segment
   int segs;
   __device__ __forceinline__ int64_t at(int64_t t) const { return reverse ? T - 1 - t : t; }
@@ -79,12 +85,13 @@ struct Geo {
 // this block's (sequence, segment, first channel) and this thread's channels and time lane
 struct Place {
   int64_t b, k0, k1;
-  int seg, c0, wave, half, lt, cl, c, n;
+  int seg, c0, wave, half, odd, lt, cl, c, n;                       // half, odd: bits of the time lane in its wave
 };
+template <int LC>
 __device__ __forceinline__ Place place(const Geo& g) {
   Place p;
   int64_t id = blockIdx.x;
-  p.c0 = (int)(id % g.tiles) * kCT;
+  p.c0 = (int)(id % g.tiles) * Shape<LC>::kCT;
   id /= g.tiles;
   p.seg = (int)(id % g.segs);
   p.b = id / g.segs;
@@ -92,8 +99,9 @@ __device__ __forceinline__ Place place(const Geo& g) {
   p.k1 = p.k0 + g.per_seg < g.chunks ? p.k0 + g.per_seg : g.chunks;
   p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   p.half = (threadIdx.x >> 5) & 1;
-  p.lt = p.wave * 2 + p.half;
-  p.cl = (threadIdx.x % kLC) * kVC;
+  p.odd = (threadIdx.x >> 4) & 1;
+  p.lt = threadIdx.x / LC;
+  p.cl = (threadIdx.x % LC) * kVC;
   p.c = p.c0 + p.cl;
   p.n = g.C - p.c;
   return p;
@@ -105,46 +113,52 @@ __device__ __forceinline__ Place place(const Geo& g) {
 // registers.  Steps behind the end and channels behind C read as `fill` and are not written.
 template <typename T>
 struct Steps {
-  T* base;
+  T* base;                                                           // step 0 of time lane 0 (reverse: of the last)
   unsigned off;
-  int64_t st;
-  __device__ __forceinline__ Steps(T* q, int64_t sb, int64_t st_, const Geo& g, const Place& p, int64_t k) : st(st_) {
-    const int64_t low = g.reverse ? g.T - (k + 1) * kChunk : k * kChunk;
+  int64_t step;
+  __device__ __forceinline__ Steps(T* q, int64_t sb, int64_t st, const Geo& g, const Place& p, int64_t k) {
+    const int64_t low = g.reverse ? g.T - (k + 1) * kChunk + kS - 1 : k * kChunk;
     base = q + (p.b * sb + low * st + p.c0);
-    off = (unsigned)(g.reverse ? kChunk - (p.lt + 1) * kS : p.lt * kS) * (unsigned)st + p.cl;
+    off = (unsigned)(g.reverse ? kLT - 1 - p.lt : p.lt) * (unsigned)(kS * st) + p.cl;
+    step = g.reverse ? -st : st;
   }
-  __device__ __forceinline__ T* at(const Geo& g, int s) const { return base + (g.reverse ? kS - 1 - s : s) * st + off; }
+  __device__ __forceinline__ T* at(int s) const { return base + s * step + off; }
 };
-template <typename T>
-__device__ __forceinline__ void load_steps(const Strided<T>& q, const Geo& g, const Place& p, int64_t k, bool whole, float fill,
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void load_steps(const Strided<T>& q, const Geo& g, const Place& p, int64_t k, float fill,
                                            Words<T, kVC> (&r)[kS]) {
   const Steps<const T> a(q.p, q.sb, q.st, g, p, k);
-  if (whole) {
+  const int64_t left = g.T - (k * kChunk + p.lt * kS);
 #pragma unroll
-    for (int s = 0; s < kS; s++) __builtin_memcpy(&r[s], a.at(g, s), sizeof(r[s]));
-  } else {
-    const int64_t left = g.T - (k * kChunk + p.lt * kS);
+  for (int s = 0; s < kS; s++) {
+    if (WHOLE || (s < left && p.n >= kVC)) {
+      __builtin_memcpy(&r[s], a.at(s), sizeof(r[s]));
+    } else {
 #pragma unroll
-    for (int s = 0; s < kS; s++)
-      if (s < left && p.n > 0) {
-        r[s] = group_load<kVC>(a.at(g, s), p.n, fill);
-      } else {
-#pragma unroll
-        for (int v = 0; v < kVC; v++) r[s].set(v, fill);
-      }
+      for (int v = 0; v < kVC; v++) r[s].set(v, s < left && v < p.n ? (float)a.at(s)[v] : fill);
+    }
   }
 }
-template <typename T>
-__device__ __forceinline__ void store_step(const Steps<T>& a, const Geo& g, const Place& p, int64_t k, bool whole, int s,
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store_step(const Steps<T>& a, const Geo& g, const Place& p, int64_t k, int s,
                                            const Words<T, kVC>& r) {
-  if (whole) __builtin_memcpy(a.at(g, s), &r, sizeof(r));
-  else if (k * kChunk + p.lt * kS + s < g.T && p.n > 0) group_store<kVC>(a.at(g, s), p.n, r);
+  if (WHOLE) __builtin_memcpy(a.at(s), &r, sizeof(r));
+  else if (k * kChunk + p.lt * kS + s < g.T && p.n > 0) group_store<kVC>(a.at(s), p.n, r);
 }
-__device__ __forceinline__ bool whole_chunk(const Geo& g, const Place& p, int64_t k) {
-  return (k + 1) * kChunk <= g.T && p.c0 + kCT <= g.C;
+// chunks from k0 on that lie inside the sequence with all channels of the tile: the loop over them
+// has no other path, whose merges would wait for the loads in flight
+template <int LC>
+__device__ __forceinline__ int64_t whole_chunks_end(const Geo& g, const Place& p) {
+  const int64_t e = p.c0 + Shape<LC>::kCT <= g.C ? g.T / kChunk : p.k0;
+  return e < p.k0 ? p.k0 : e < p.k1 ? e : p.k1;
 }
 
-// values of the lower and the upper half wave, in every lane
+// of each two neighbouring rows of 16 lanes, or of the two half waves: the lower's and the upper's value
+__device__ __forceinline__ void rows16(float v, float& lo, float& hi) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  lo = __builtin_bit_cast(float, (unsigned)r[0]);
+  hi = __builtin_bit_cast(float, (unsigned)r[1]);
+}
 __device__ __forceinline__ void halves(float v, float& lo, float& hi) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
   lo = __builtin_bit_cast(float, (unsigned)r[0]);
@@ -154,10 +168,12 @@ __device__ __forceinline__ void halves(float v, float& lo, float& hi) {
 // ---- segment maps: (P, E) of each segment, agg [B][segs][2][C] --------------------------------
 // Each time lane walks one contiguous span of the segment, so the lanes join once, at its end.
 // BWD: the map of Q from the segment's end to its start (E from dy, z); else that of h (E from x).
-template <typename T, bool BWD>
-__global__ __launch_bounds__(kThreads) void recur_segment_kernel(Strided<T> e, Strided<T> d, Strided<T> z, Geo g, float* agg) {
+template <typename T, bool BWD, int LC>
+__global__ __launch_bounds__(Shape<LC>::kThreads) void recur_segment_kernel(Strided<T> e, Strided<T> d, Strided<T> z, Geo g,
+                                                                            float* agg) {
+  constexpr int kCT = Shape<LC>::kCT;
   __shared__ float sP[kLT][kCT], sE[kLT][kCT];
-  const Place p = place(g);
+  const Place p = place<LC>(g);
   const int64_t first = p.k0 * kChunk, end = p.k1 * kChunk < g.T ? p.k1 * kChunk : g.T;
   const int64_t span = (end - first + kLT - 1) / kLT;
   const int64_t t0 = first + p.lt * span, t1 = t0 + span < end ? t0 + span : end;
@@ -213,17 +229,17 @@ __global__ __launch_bounds__(kThreads) void recur_segment_kernel(Strided<T> e, S
 
 // The state entering this block's segment in each lane's channels: `s0` [B][C] (or null: 0) run
 // through the maps of the segments before it (BWD: behind it).  Eight threads a channel take a
-// contiguous part of those maps each.  Ends with a barrier.
-template <bool BWD>
+// contiguous part of those maps each.
+template <bool BWD, int LC>
 __device__ __forceinline__ void enter(const float* s0, const float* agg, const Geo& g, const Place& p, float (&state)[kVC]) {
-  __shared__ float fP[kWaves][kCT], fE[kWaves][kCT];
-  if (!agg) {
+  constexpr int kCT = Shape<LC>::kCT, kParts = Shape<LC>::kThreads / kCT;
+  __shared__ float fP[kParts][kCT], fE[kParts][kCT];
 #pragma unroll
-    for (int v = 0; v < kVC; v++) state[v] = s0 && v < p.n ? s0[p.b * g.C + p.c + v] : 0.f;
-    return;
-  }
-  const int ch = threadIdx.x & 63, lo = BWD ? p.seg + 1 : 0, cnt = BWD ? g.segs - 1 - p.seg : p.seg;
-  const int part = (cnt + kWaves - 1) / kWaves, j0 = p.wave * part, j1 = j0 + part < cnt ? j0 + part : cnt;
+  for (int v = 0; v < kVC; v++) state[v] = s0 && v < p.n ? s0[p.b * g.C + p.c + v] : 0.f;
+  if (!agg) return;
+  const int ch = threadIdx.x % kCT, at = threadIdx.x / kCT;
+  const int lo = BWD ? p.seg + 1 : 0, cnt = BWD ? g.segs - 1 - p.seg : p.seg;
+  const int part = (cnt + kParts - 1) / kParts, j0 = at * part, j1 = j0 + part < cnt ? j0 + part : cnt;
   float m = 1.f, s = 0.f;
   if (p.c0 + ch < g.C) {
     const float* q = agg + (p.b * g.segs + lo) * 2 * (int64_t)g.C + p.c0 + ch;
@@ -235,36 +251,38 @@ __device__ __forceinline__ void enter(const float* s0, const float* agg, const G
       m *= pj;
     }
   }
-  fP[p.wave][ch] = m;
-  fE[p.wave][ch] = s;
+  fP[at][ch] = m;
+  fE[at][ch] = s;
   __syncthreads();
 #pragma unroll
-  for (int v = 0; v < kVC; v++) {
-    float h = s0 && v < p.n ? s0[p.b * g.C + p.c + v] : 0.f;
+  for (int w = 0; w < kParts; w++)
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) h = fP[w][p.cl + v] * h + fE[w][p.cl + v];
-    state[v] = h;
-  }
+    for (int v = 0; v < kVC; v++) state[v] = fP[w][p.cl + v] * state[v] + fE[w][p.cl + v];
 }
 
 // ---- forward ----------------------------------------------------------------------------------
-template <typename T, bool GATE>
-__global__ __launch_bounds__(kThreads) void recur_fwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, const float* h0, Geo g,
-                                                             const float* agg, T* y, float* last, float* carry) {
+template <typename T, bool GATE, int LC>
+__global__ __launch_bounds__(Shape<LC>::kThreads) void recur_fwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, const float* h0,
+                                                                        Geo g, const float* agg, T* y, float* last,
+                                                                        float* carry) {
+  constexpr int kCT = Shape<LC>::kCT, kWaves = Shape<LC>::kWaves;
   // two sets: a chunk's maps are written while slower waves still read those of the chunk before
   __shared__ float sP[2][kWaves][kCT], sE[2][kWaves][kCT];
-  const Place p = place(g);
+  const Place p = place<LC>(g);
   float state[kVC];                                                   // entering the chunk
-  enter<false>(h0, agg, g, p, state);
-  Words<T, kVC> nx[kS], nd[kS], nz[kS];
-  auto fetch = [&](int64_t k) {
-    const bool whole = whole_chunk(g, p, k);
-    load_steps(x, g, p, k, whole, 0.f, nx);
-    load_steps(d, g, p, k, whole, __builtin_inff(), nd);
-    if constexpr (GATE) load_steps(z, g, p, k, whole, 0.f, nz);
+  enter<false, LC>(h0, agg, g, p, state);
+  struct Raw {                                                        // a chunk's operands as loaded
+    Words<T, kVC> x[kS], d[kS], z[GATE ? kS : 1];
   };
-  if (p.k0 < p.k1) fetch(p.k0);
-  for (int64_t k = p.k0; k < p.k1; k++) {
+  auto fetch = [&](auto whole, int64_t k, Raw& n) {
+    constexpr bool W = decltype(whole)::value;
+    load_steps<W>(x, g, p, k, 0.f, n.x);
+    load_steps<W>(d, g, p, k, __builtin_inff(), n.d);
+    if constexpr (GATE) load_steps<W>(z, g, p, k, 0.f, n.z);
+  };
+  const int64_t whole_end = whole_chunks_end<LC>(g, p);
+  auto chunk = [&](auto whole, int64_t k, Raw& n) {
+    constexpr bool W = decltype(whole)::value;
     const int par = k & 1;
     float A[kS][kVC], I[kS][kVC], F[kS][kVC], P[kVC], E[kVC];
 #pragma unroll
@@ -273,26 +291,33 @@ __global__ __launch_bounds__(kThreads) void recur_fwd_kernel(Strided<T> x, Strid
     for (int s = 0; s < kS; s++)
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        sigmoid_pair(nd[s].get(v), A[s][v], I[s][v]);
-        I[s][v] *= nx[s].get(v);
+        sigmoid_pair(n.d[s].get(v), A[s][v], I[s][v]);
+        I[s][v] *= n.x[s].get(v);
         E[v] = A[s][v] * E[v] + I[s][v];
         P[v] *= A[s][v];
-        if constexpr (GATE) F[s][v] = nz[s].get(v);
+        if constexpr (GATE) F[s][v] = n.z[s].get(v);
       }
-    if (k + 1 < p.k1) fetch(k + 1);
-    float Pl[kVC], El[kVC];                                           // of the lower half: what enters the upper one
+    if (W && k + 1 < whole_end) fetch(whole, k + 1, n);
+    // maps of the lower row of 16 and of the lower half: what enters the rows and the half above them
+    float Pa[kVC], Ea[kVC], Pl[kVC], El[kVC];
 #pragma unroll
     for (int v = 0; v < kVC; v++) {
       float Ph, Eh;
+      if constexpr (LC == 16) {
+        rows16(P[v], Pa[v], Ph);
+        rows16(E[v], Ea[v], Eh);
+        P[v] = Pa[v] * Ph;
+        E[v] = Ph * Ea[v] + Eh;
+      }
       halves(P[v], Pl[v], Ph);
       halves(E[v], El[v], Eh);
-      if (p.half == 0) {
+      if (threadIdx.x % 64 < LC) {
         sP[par][p.wave][p.cl + v] = Pl[v] * Ph;
         sE[par][p.wave][p.cl + v] = Ph * El[v] + Eh;
       }
     }
     __syncthreads();
-    if (carry && p.wave == 0 && p.half == 0) {
+    if (carry && threadIdx.x < LC) {
 #pragma unroll
       for (int v = 0; v < kVC; v++)
         if (v < p.n) carry[(p.b * g.chunks + k) * g.C + p.c + v] = state[v];
@@ -307,8 +332,10 @@ __global__ __launch_bounds__(kThreads) void recur_fwd_kernel(Strided<T> x, Strid
       }
     }
 #pragma unroll
-    for (int v = 0; v < kVC; v++) h[v] = p.half ? Pl[v] * h[v] + El[v] : h[v];
-    const bool whole = whole_chunk(g, p, k);
+    for (int v = 0; v < kVC; v++) {
+      h[v] = p.half ? Pl[v] * h[v] + El[v] : h[v];
+      if constexpr (LC == 16) h[v] = p.odd ? Pa[v] * h[v] + Ea[v] : h[v];
+    }
     const Steps<T> at(y, g.T * g.C, g.C, g, p, k);
 #pragma unroll
     for (int s = 0; s < kS; s++) {
@@ -318,10 +345,17 @@ __global__ __launch_bounds__(kThreads) void recur_fwd_kernel(Strided<T> x, Strid
         h[v] = A[s][v] * h[v] + I[s][v];
         o.set(v, GATE ? h[v] * silu(F[s][v]) : h[v]);
       }
-      store_step(at, g, p, k, whole, s, o);
+      store_step<W>(at, g, p, k, s, o);
     }
+  };
+  Raw n;
+  if (p.k0 < whole_end) fetch(Bool<true>{}, p.k0, n);
+  for (int64_t k = p.k0; k < whole_end; k++) chunk(Bool<true>{}, k, n);
+  for (int64_t k = whole_end; k < p.k1; k++) {
+    fetch(Bool<false>{}, k, n);
+    chunk(Bool<false>{}, k, n);
   }
-  if (p.k1 == g.chunks && threadIdx.x < kLC) {
+  if (p.k1 == g.chunks && threadIdx.x < LC) {
 #pragma unroll
     for (int v = 0; v < kVC; v++)
       if (v < p.n) last[p.b * g.C + p.c + v] = state[v];
@@ -329,30 +363,33 @@ __global__ __launch_bounds__(kThreads) void recur_fwd_kernel(Strided<T> x, Strid
 }
 
 // ---- backward ---------------------------------------------------------------------------------
-template <typename T, bool GATE>
-__global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, Strided<T> dy,
-                                                             const float* carry, const float* dlast, Geo g, const float* agg,
-                                                             T* dx, T* dd, T* dz, float* dh0) {
-  // a and i of a step stay in registers, or (fp32 tensors, whose operands take twice the registers)
-  // are computed again from d where they are used
+template <typename T, bool GATE, int LC>
+__global__ __launch_bounds__(Shape<LC>::kThreads) void recur_bwd_kernel(Strided<T> x, Strided<T> d, Strided<T> z, Strided<T> dy,
+                                                                        const float* carry, const float* dlast, Geo g,
+                                                                        const float* agg, T* dx, T* dd, T* dz, float* dh0) {
+  constexpr int kCT = Shape<LC>::kCT, kWaves = Shape<LC>::kWaves;
+  // a and i of a step stay in registers where those suffice, else are computed again from d
   constexpr bool kHold = sizeof(T) == 2;
   __shared__ float sP[2][kWaves][kCT], sE[2][kWaves][kCT], sQ[2][kWaves][kCT];
-  const Place p = place(g);
+  const Place p = place<LC>(g);
   float state[kVC];                                                   // Q entering the chunk from its end
-  enter<true>(dlast, agg, g, p, state);
-  Words<T, kVC> nx[kS], nd[kS], nz[kS], ny[kS];
-  float nh[kVC];
-  auto fetch = [&](int64_t k) {
-    const bool whole = whole_chunk(g, p, k);
-    load_steps(x, g, p, k, whole, 0.f, nx);
-    load_steps(d, g, p, k, whole, __builtin_inff(), nd);
-    load_steps(dy, g, p, k, whole, 0.f, ny);
-    if constexpr (GATE) load_steps(z, g, p, k, whole, 0.f, nz);
-#pragma unroll
-    for (int v = 0; v < kVC; v++) nh[v] = v < p.n ? carry[(p.b * g.chunks + k) * g.C + p.c + v] : 0.f;
+  enter<true, LC>(dlast, agg, g, p, state);
+  struct Raw {
+    Words<T, kVC> x[kS], d[kS], y[kS], z[GATE ? kS : 1];
+    float h[kVC];
   };
-  if (p.k0 < p.k1) fetch(p.k1 - 1);
-  for (int64_t k = p.k1 - 1; k >= p.k0; k--) {
+  auto fetch = [&](auto whole, int64_t k, Raw& n) {
+    constexpr bool W = decltype(whole)::value;
+    load_steps<W>(x, g, p, k, 0.f, n.x);
+    load_steps<W>(d, g, p, k, __builtin_inff(), n.d);
+    load_steps<W>(dy, g, p, k, 0.f, n.y);
+    if constexpr (GATE) load_steps<W>(z, g, p, k, 0.f, n.z);
+#pragma unroll
+    for (int v = 0; v < kVC; v++) n.h[v] = W || v < p.n ? carry[(p.b * g.chunks + k) * g.C + p.c + v] : 0.f;
+  };
+  const int64_t whole_end = whole_chunks_end<LC>(g, p);
+  auto chunk = [&](auto whole, int64_t k, Raw& n) {
+    constexpr bool W = decltype(whole)::value;
     const int par = k & 1;
     Words<T, kVC> cx[kS], cd[kHold ? 1 : kS];
     float A[kHold ? kS : 1][kVC], I[kHold ? kS : 1][kVC], top[kS][kVC], yf[kS][kVC], P[kVC], E[kVC], Q[kVC], h[kVC];
@@ -365,22 +402,22 @@ __global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strid
       }
     };
 #pragma unroll
-    for (int v = 0; v < kVC; v++) P[v] = 1.f, E[v] = Q[v] = 0.f, h[v] = nh[v];
+    for (int v = 0; v < kVC; v++) P[v] = 1.f, E[v] = Q[v] = 0.f, h[v] = n.h[v];
 #pragma unroll
     for (int s = 0; s < kS; s++) {
-      cx[s] = nx[s];
-      if constexpr (!kHold) cd[s] = nd[s];
+      cx[s] = n.x[s];
+      if constexpr (!kHold) cd[s] = n.d[s];
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
         float a, i;
-        sigmoid_pair(nd[s].get(v), a, i);
+        sigmoid_pair(n.d[s].get(v), a, i);
         if constexpr (kHold) A[s][v] = a, I[s][v] = i;
-        E[v] = a * E[v] + i * nx[s].get(v);
+        E[v] = a * E[v] + i * n.x[s].get(v);
         P[v] *= a;
-        const float g_out = ny[s].get(v);
+        const float g_out = n.y[s].get(v);
         if constexpr (GATE) {
           float f, df;
-          silu_pair(nz[s].get(v), f, df);
+          silu_pair(n.z[s].get(v), f, df);
           top[s][v] = g_out * f;
           yf[s][v] = g_out * df;
         } else {
@@ -388,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strid
         }
       }
     }
-    if (k > p.k0) fetch(k - 1);
+    if (W && k > p.k0) fetch(whole, k - 1, n);
 #pragma unroll
     for (int s = kS - 1; s >= 0; s--)
 #pragma unroll
@@ -397,14 +434,22 @@ __global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strid
         pair(s, v, a, i);
         Q[v] = a * (Q[v] + top[s][v]);
       }
-    float Pl[kVC], El[kVC], Ph[kVC], Qh[kVC];
+    float Pa[kVC], Ea[kVC], Pb[kVC], Qb[kVC], Pl[kVC], El[kVC], Ph[kVC], Qh[kVC];
 #pragma unroll
     for (int v = 0; v < kVC; v++) {
       float Eh, Ql;
+      if constexpr (LC == 16) {
+        rows16(P[v], Pa[v], Pb[v]);
+        rows16(E[v], Ea[v], Eh);
+        rows16(Q[v], Ql, Qb[v]);
+        P[v] = Pa[v] * Pb[v];
+        E[v] = Pb[v] * Ea[v] + Eh;
+        Q[v] = Pa[v] * Qb[v] + Ql;
+      }
       halves(P[v], Pl[v], Ph[v]);
       halves(E[v], El[v], Eh);
       halves(Q[v], Ql, Qh[v]);
-      if (p.half == 0) {
+      if (threadIdx.x % 64 < LC) {
         sP[par][p.wave][p.cl + v] = Pl[v] * Ph[v];
         sE[par][p.wave][p.cl + v] = Ph[v] * El[v] + Eh;
         sQ[par][p.wave][p.cl + v] = Pl[v] * Qh[v] + Ql;
@@ -426,6 +471,10 @@ __global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strid
     for (int v = 0; v < kVC; v++) {
       h[v] = p.half ? Pl[v] * h[v] + El[v] : h[v];
       q[v] = p.half ? q[v] : Ph[v] * q[v] + Qh[v];
+      if constexpr (LC == 16) {
+        h[v] = p.odd ? Pa[v] * h[v] + Ea[v] : h[v];
+        q[v] = p.odd ? q[v] : Pb[v] * q[v] + Qb[v];
+      }
     }
     float H[kS][kVC];                                                  // the state before each step
 #pragma unroll
@@ -437,7 +486,6 @@ __global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strid
         H[s][v] = h[v];
         h[v] = a * h[v] + i * cx[s].get(v);
       }
-    const bool whole = whole_chunk(g, p, k);
     const int64_t sb = g.T * g.C;
     const Steps<T> ax(dx, sb, g.C, g, p, k), ad(dd, sb, g.C, g, p, k), az(dz, sb, g.C, g, p, k);
 #pragma unroll
@@ -453,13 +501,20 @@ __global__ __launch_bounds__(kThreads) void recur_bwd_kernel(Strided<T> x, Strid
         if constexpr (GATE) oz.set(v, yf[s][v] * (a * H[s][v] + i * xv));
         q[v] = a * G;
       }
-      if (dx) store_step(ax, g, p, k, whole, s, ox);
-      if (dd) store_step(ad, g, p, k, whole, s, od);
+      if (dx) store_step<W>(ax, g, p, k, s, ox);
+      if (dd) store_step<W>(ad, g, p, k, s, od);
       if constexpr (GATE)
-        if (dz) store_step(az, g, p, k, whole, s, oz);
+        if (dz) store_step<W>(az, g, p, k, s, oz);
     }
+  };
+  Raw n;
+  for (int64_t k = p.k1 - 1; k >= whole_end; k--) {
+    fetch(Bool<false>{}, k, n);
+    chunk(Bool<false>{}, k, n);
   }
-  if (p.k0 == 0 && dh0 && threadIdx.x < kLC) {
+  if (p.k0 < whole_end) fetch(Bool<true>{}, whole_end - 1, n);
+  for (int64_t k = whole_end - 1; k >= p.k0; k--) chunk(Bool<true>{}, k, n);
+  if (p.k0 == 0 && dh0 && threadIdx.x < LC) {
 #pragma unroll
     for (int v = 0; v < kVC; v++)
       if (v < p.n) dh0[p.b * g.C + p.c + v] = state[v];
@@ -558,13 +613,15 @@ __global__ __launch_bounds__(128) void recur_bwd_short_kernel(Strided<T> x, Stri
   }
 }
 
+// Tiles of 64 channels where they give each CU two blocks, else of 32 (64-byte rows of 16-bit tensors).
 // Segments: none once sequences × channel tiles give each of the 256 CUs a block; else as many as
 // bring the launch to about two blocks a CU, each at least four chunks long.
 Geo geometry(int64_t B, int64_t T, int C, int reverse) {
   Geo g{};
   g.B = B, g.T = T, g.C = C, g.reverse = reverse;
   g.chunks = (T + kChunk - 1) / kChunk;
-  g.tiles = T <= kShort ? ceil_div(C, kShortVC) : ceil_div(C, kCT);
+  g.lc = 32;
+  g.tiles = T <= kShort ? ceil_div(C, kShortVC) : ceil_div(C, g.lc * kVC);
   const int64_t base = B * g.tiles;
   int64_t segs = base >= 256 ? 1 : (512 + base - 1) / base;
   if (segs > g.chunks / 4) segs = g.chunks / 4 > 0 ? g.chunks / 4 : 1;
@@ -572,6 +629,16 @@ Geo geometry(int64_t B, int64_t T, int C, int reverse) {
   g.segs = (int)((g.chunks + g.per_seg - 1) / g.per_seg);
   return g;
 }
+
+// run the statement block with the channel lanes as LC
+#define MRAGAN_RECUR_LC(lc, ...) \
+  if (lc == 32) {                \
+    constexpr int LC = 32;       \
+    __VA_ARGS__;                 \
+  } else {                       \
+    constexpr int LC = 16;       \
+    __VA_ARGS__;                 \
+  }
 
 template <typename T>
 Strided<T> strided(const void* p, int64_t sb, int64_t st) {
@@ -602,13 +669,16 @@ int recurrence_fwd(const RecurArgs& r, const float* h0, void* y, float* last, fl
       recur_fwd_short_kernel<T><<<grid, 128, 0, st>>>(x, d, z, h0, g, yt, last, carry);
       return check_launch("recurrence_fwd_short");
     }
-    if (g.segs > 1) {
-      recur_segment_kernel<T, false><<<grid, kThreads, 0, st>>>(x, d, z, g, ws);
-      if (int rc = check_launch("recurrence_segment")) return rc;
-    }
     const float* agg = g.segs > 1 ? ws : nullptr;
-    if (r.gate) recur_fwd_kernel<T, true><<<grid, kThreads, 0, st>>>(x, d, z, h0, g, agg, yt, last, carry);
-    else recur_fwd_kernel<T, false><<<grid, kThreads, 0, st>>>(x, d, z, h0, g, agg, yt, last, carry);
+    MRAGAN_RECUR_LC(g.lc, {
+      constexpr int N = Shape<LC>::kThreads;
+      if (agg) {
+        recur_segment_kernel<T, false, LC><<<grid, N, 0, st>>>(x, d, z, g, ws);
+        if (int rc = check_launch("recurrence_segment")) return rc;
+      }
+      if (r.gate) recur_fwd_kernel<T, true, LC><<<grid, N, 0, st>>>(x, d, z, h0, g, agg, yt, last, carry);
+      else recur_fwd_kernel<T, false, LC><<<grid, N, 0, st>>>(x, d, z, h0, g, agg, yt, last, carry);
+    })
     return check_launch("recurrence_fwd");
   })
   return kOk;
@@ -626,13 +696,16 @@ int recurrence_bwd(const RecurArgs& r, const float* carry, const void* dy, int64
       recur_bwd_short_kernel<T><<<grid, 128, 0, st>>>(x, d, z, gy, carry, dlast, g, dxt, ddt, dzt, dh0);
       return check_launch("recurrence_bwd_short");
     }
-    if (g.segs > 1) {
-      recur_segment_kernel<T, true><<<grid, kThreads, 0, st>>>(gy, d, z, g, ws);
-      if (int rc = check_launch("recurrence_segment")) return rc;
-    }
     const float* agg = g.segs > 1 ? ws : nullptr;
-    if (r.gate) recur_bwd_kernel<T, true><<<grid, kThreads, 0, st>>>(x, d, z, gy, carry, dlast, g, agg, dxt, ddt, dzt, dh0);
-    else recur_bwd_kernel<T, false><<<grid, kThreads, 0, st>>>(x, d, z, gy, carry, dlast, g, agg, dxt, ddt, dzt, dh0);
+    MRAGAN_RECUR_LC(g.lc, {
+      constexpr int N = Shape<LC>::kThreads;
+      if (agg) {
+        recur_segment_kernel<T, true, LC><<<grid, N, 0, st>>>(gy, d, z, g, ws);
+        if (int rc = check_launch("recurrence_segment")) return rc;
+      }
+      if (r.gate) recur_bwd_kernel<T, true, LC><<<grid, N, 0, st>>>(x, d, z, gy, carry, dlast, g, agg, dxt, ddt, dzt, dh0);
+      else recur_bwd_kernel<T, false, LC><<<grid, N, 0, st>>>(x, d, z, gy, carry, dlast, g, agg, dxt, ddt, dzt, dh0);
+    })
     return check_launch("recurrence_bwd");
   })
   return kOk;
