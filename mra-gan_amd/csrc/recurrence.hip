@@ -613,14 +613,14 @@ __global__ __launch_bounds__(128) void recur_bwd_short_kernel(Strided<T> x, Stri
   }
 }
 
-// Tiles of 64 channels where they give each CU two blocks, else of 32 (64-byte rows of 16-bit tensors).
+// Tiles of 64 channels, of 32 where C has no more (XXX).
 // Segments: none once sequences × channel tiles give each of the 256 CUs a block; else as many as
 // bring the launch to about two blocks a CU, each at least four chunks long.
 Geo geometry(int64_t B, int64_t T, int C, int reverse) {
   Geo g{};
   g.B = B, g.T = T, g.C = C, g.reverse = reverse;
   g.chunks = (T + kChunk - 1) / kChunk;
-  g.lc = 32;
+  g.lc = C <= 32 ? 16 : 32;
   g.tiles = T <= kShort ? ceil_div(C, kShortVC) : ceil_div(C, g.lc * kVC);
   const int64_t base = B * g.tiles;
   int64_t segs = base >= 256 ? 1 : (512 + base - 1) / base;
