@@ -427,9 +427,9 @@ int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, c
  * throughout; 16-byte aligned contiguous tensors.  fp32 tensors are multiplied in the process
  * mode of mragan_set_conv_precision (f32 here: three bf16 planes per operand, six products, fp32
  * accumulation, ≤ 2⁻²² relative error per product); 16-bit tensors as they are, and what the
- * products take from each other (h, dg, du, `kept`) is rounded to that type.  kept [3][M][F]
- * (dtype) holds h, act'(g)·u and act(g): fwd writes it when given, bwd reads it, or recomputes it
- * from x when NULL.  bwd: any gradient may be NULL to skip it. */
+ * products take from each other (h, dg, du) is rounded to that type.  kept (fp32: [3][M][F], 16-bit
+ * types: [4][M][F], the last two factors with 24 bits) holds h, act'(g)·u and act(g): fwd writes it
+ * when given, bwd reads it, or recomputes it from x when NULL.  bwd: any gradient may be NULL to skip it. */
 enum mragan_gate_act { MRAGAN_ACT_SILU = 5, MRAGAN_ACT_GELU = 6 };
 size_t mragan_gated_ffn_workspace(int64_t M, int C, int F, int O, int dtype, int backward, int recompute);
 int mragan_gated_ffn_fwd(const void* x, int64_t M, int C, int F, int O, int dtype, const void* w_gate, const void* w_up,

@@ -66,66 +66,115 @@ __device__ __forceinline__ void split_planes(float v, int planes, H (&out)[3]) {
   out[2] = planes > 2 ? (H)(r - (float)out[1]) : (H)0.f;
 }
 
-// src [R][K] (any type) → 16-bit planes dst [planes][R][ld], zeros from K to ld
+// src [R][K] (any type) → 16-bit planes dst [planes][R][ld], zeros from K to ld; several tensors a launch,
+// kPackQuads groups of four elements a block
+constexpr int kPackQuads = 1024, kMaxPacks = 8;
+struct PackJob {
+  const void* src;
+  void* dst;
+  int64_t R, K, ld;
+  int64_t first;                  // its first block
+};
+struct PackArgs {
+  PackJob job[kMaxPacks];
+  int jobs, planes;
+};
 template <typename T, typename H>
-__global__ __launch_bounds__(256) void ffn_pack_kernel(const T* src, int64_t R, int64_t K, int planes, H* dst, int64_t ld) {
-  const int64_t quads = ld / 4, total = R * quads, step = (int64_t)gridDim.x * 256, plane = R * ld;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+__global__ __launch_bounds__(256) void ffn_pack_kernel(const PackArgs a) {
+  int j = 0;
+  while (j + 1 < a.jobs && blockIdx.x >= a.job[j + 1].first) j++;
+  const PackJob& q = a.job[j];
+  const T* src = static_cast<const T*>(q.src);
+  const int64_t quads = q.ld / 4, total = q.R * quads, plane = q.R * q.ld, i0 = (blockIdx.x - q.first) * kPackQuads;
+#pragma unroll
+  for (int n = 0; n < kPackQuads / 256; n++) {
+    const int64_t i = i0 + n * 256 + threadIdx.x;
+    if (i >= total) break;
     const int64_t r = i / quads, k = (i - r * quads) * 4;
+    float v[4];
+    if ((q.K & 3) == 0 && k < q.K) {
+      load_vec<T, 4>(src + r * q.K + k, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = k + e < q.K ? (float)src[r * q.K + k + e] : 0.f;
+    }
     H w[4][3];
 #pragma unroll
-    for (int q = 0; q < 4; q++) split_planes<H>(k + q < K ? (float)src[r * K + k + q] : 0.f, planes, w[q]);
+    for (int e = 0; e < 4; e++) split_planes<H>(v[e], a.planes, w[e]);
 #pragma unroll
     for (int p = 0; p < 3; p++)
-      if (p < planes) {
+      if (p < a.planes) {
         Pack<H, 4> o;
 #pragma unroll
-        for (int q = 0; q < 4; q++) o.v[q] = w[q][p];
-        *reinterpret_cast<Pack<H, 4>*>(dst + p * plane + r * ld + k) = o;
+        for (int e = 0; e < 4; e++) o.v[e] = w[e][p];
+        *reinterpret_cast<Pack<H, 4>*>(static_cast<H*>(q.dst) + p * plane + r * q.ld + k) = o;
       }
   }
 }
 
-// Σ over a chunk of rows of the columns of planes [planes][rows][ld] → part [chunks][cols]; a thread
-// takes four columns, the waves of a block every fourth row
-template <typename H>
-__global__ __launch_bounds__(256) void ffn_col_sum_kernel(const H* src, int64_t rows, int cols, int64_t ld, int planes,
-                                                          int64_t per_chunk, float* part) {
-  __shared__ float s[4][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 256 + lane * 4;
+// Σ over chunk blockIdx.y of the rows of src [rows][cols] → part [chunks][cols]: a thread per column and
+// every fourth row of the chunk
+template <typename T>
+__global__ __launch_bounds__(256) void ffn_col_sum_kernel(const T* src, int64_t rows, int cols, int64_t per_chunk, float* part) {
+  __shared__ float s[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
   const int64_t r0 = blockIdx.y * per_chunk, r1 = r0 + per_chunk < rows ? r0 + per_chunk : rows;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < ld)
-    for (int p = 0; p < planes; p++)
-#pragma unroll 4
-      for (int64_t r = r0 + wave; r < r1; r += 4) {
-        float t[4];
-        load_vec<H, 4>(src + (p * rows + r) * ld + c, t);
-#pragma unroll
-        for (int q = 0; q < 4; q++) v[q] += t[q];
-      }
-#pragma unroll
-  for (int q = 0; q < 4; q++) s[wave][lane * 4 + q] = v[q];
-  __syncthreads();
-  const int col = blockIdx.x * 256 + threadIdx.x;
-  if (col < cols) {
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) t += s[w][threadIdx.x];
-    part[(int64_t)blockIdx.y * cols + col] = t;
+  float v = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = r0 + wave; r < r1; r += 4) v += (float)src[r * cols + c];
   }
+  s[wave][lane] = v;
+  __syncthreads();
+  if (wave == 0 && c < cols) part[(int64_t)blockIdx.y * cols + c] = s[0][lane] + s[1][lane] + s[2][lane] + s[3][lane];
 }
 
-// out[i] = Σ_s part[s][i] in order (+ bias[i mod N])
-template <typename TO>
-__global__ __launch_bounds__(256) void ffn_reduce_kernel(const float* part, int parts, int64_t total, int N, const TO* bias,
-                                                         TO* out) {
-  const int64_t step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    float v = 0.f;
-    for (int s = 0; s < parts; s++) v += part[s * total + i];
+// out[i] = Σ_s part[s][i] (+ bias[i mod N]): 64 elements a block, SLOTS threads each that take every
+// SLOTS-th part and join in order
+template <typename TO, int SLOTS>
+__global__ __launch_bounds__(64 * SLOTS) void ffn_reduce_kernel(const float* part, int parts, int64_t total, int N, const TO* bias,
+                                                                TO* out) {
+  __shared__ float s[SLOTS][64];
+  const int lane = threadIdx.x & 63, slot = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+  float v = 0.f;
+  if (i < total) {
+#pragma unroll 8
+    for (int p = slot; p < parts; p += SLOTS) v += part[p * total + i];
+  }
+  s[slot][lane] = v;
+  __syncthreads();
+  if (slot == 0 && i < total) {
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < SLOTS; k++) v += s[k][lane];
     if (bias) v += (float)bias[i % N];
     out[i] = (TO)v;
+  }
+}
+
+// db of both projections from the column sums [rows][2][F] of the dg / du launch
+template <typename TO>
+__global__ __launch_bounds__(1024) void ffn_bias_reduce_kernel(const float* part, int rows, int F, TO* dbg, TO* dbu) {
+  __shared__ float s[16][64];
+  const int lane = threadIdx.x & 63, slot = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane, total = 2 * (int64_t)F;
+  float v = 0.f;
+  if (i < total) {
+#pragma unroll 8
+    for (int p = slot; p < rows; p += 16) v += part[p * total + i];
+  }
+  s[slot][lane] = v;
+  __syncthreads();
+  if (slot == 0 && i < total) {
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; k++) v += s[k][lane];
+    if (i < F) {
+      if (dbg) dbg[i] = (TO)v;
+    } else if (dbu) {
+      dbu[i - F] = (TO)v;
+    }
   }
 }
 
@@ -146,7 +195,8 @@ struct GemmArgs {
   // kEpiGate / kEpiGateBwd: 16-bit planes of [M][ldf]
   const void *bias_g, *bias_u;
   int act, planes;
-  void* kept;                     // [3][M][N] (h, act'·u, act): written by kEpiGate if given, read by kEpiGateBwd
+  void* kept;                     // [M][N] layers (see store_kept): written by kEpiGate if given, read by kEpiGateBwd
+  float* col_part;                // kEpiGateBwd, or null: [tiles_m·WM][2][N] column sums of dg and du
   void *h, *dg, *du;
   int64_t ldf;
 };
@@ -211,6 +261,67 @@ __device__ __forceinline__ void load8(const TO* row, int n, int N, bool vec, flo
       if (n + i < N) v[i] = (float)row[n + i];
   }
 }
+// What the forward keeps for the backward, as layers [M][N] of TO: h, then P = act'(g)·u and f = act(g).
+// fp32 tensors: a layer each.  16-bit tensors: P and f with 24 bits of their fp32 form (rounding them to
+// the type would cost dg and du as much again as their own rounding): a layer of the upper halves
+// each, and one with the next byte of both.
+constexpr int kept_layers(size_t element) { return element == 4 ? 3 : 4; }
+template <typename TO>
+__device__ __forceinline__ void store_kept(TO* k, int64_t layer, int n, int N, bool vec, const float (&h)[8], const float (&P)[8],
+                                           const float (&f)[8]) {
+  store8<TO>(k, n, N, vec, h);
+  if constexpr (sizeof(TO) == 4) {
+    store8<TO>(k + layer, n, N, vec, P);
+    store8<TO>(k + 2 * layer, n, N, vec, f);
+  } else {
+    Pack<uint16_t, 8> hp, hf, lo;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t bp = __builtin_bit_cast(uint32_t, P[i]) + 0x80u, bf = __builtin_bit_cast(uint32_t, f[i]) + 0x80u;
+      hp.v[i] = bp >> 16;
+      hf.v[i] = bf >> 16;
+      lo.v[i] = (bp >> 8 & 0xffu) | (bf & 0xff00u);
+    }
+    uint16_t* q = reinterpret_cast<uint16_t*>(k) + layer + n;
+    if (vec) {
+      if (n < N) {
+        *reinterpret_cast<Pack<uint16_t, 8>*>(q) = hp;
+        *reinterpret_cast<Pack<uint16_t, 8>*>(q + layer) = hf;
+        *reinterpret_cast<Pack<uint16_t, 8>*>(q + 2 * layer) = lo;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (n + i < N) q[i] = hp.v[i], q[layer + i] = hf.v[i], q[2 * layer + i] = lo.v[i];
+    }
+  }
+}
+template <typename TO>
+__device__ __forceinline__ void load_kept(const TO* k, int64_t layer, int n, int N, bool vec, float (&P)[8], float (&f)[8]) {
+  if constexpr (sizeof(TO) == 4) {
+    load8<TO>(k + layer, n, N, vec, P);
+    load8<TO>(k + 2 * layer, n, N, vec, f);
+  } else {
+    Pack<uint16_t, 8> hp{}, hf{}, lo{};
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(k) + layer + n;
+    if (vec) {
+      if (n < N) {
+        hp = *reinterpret_cast<const Pack<uint16_t, 8>*>(q);
+        hf = *reinterpret_cast<const Pack<uint16_t, 8>*>(q + layer);
+        lo = *reinterpret_cast<const Pack<uint16_t, 8>*>(q + 2 * layer);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (n + i < N) hp.v[i] = q[i], hf.v[i] = q[layer + i], lo.v[i] = q[2 * layer + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      P[i] = __builtin_bit_cast(float, (uint32_t)hp.v[i] << 16 | (uint32_t)(lo.v[i] & 0xff) << 8);
+      f[i] = __builtin_bit_cast(float, (uint32_t)hf.v[i] << 16 | (uint32_t)(lo.v[i] & 0xff00));
+    }
+  }
+}
 // planes of eight values at element `off` of each plane (rows of whole groups of eight)
 template <typename H>
 __device__ __forceinline__ void store_planes8(void* base, int64_t off, int64_t plane, int planes, const float (&v)[8]) {
@@ -238,13 +349,17 @@ struct IntConst {
 //                    rows.  B: fragment rows are 4·NF apart in fours (see `nrow`), so row & 3 and the
 //                    lowest bit of that distance.
 //   rows contiguous: [64 k][ROWS / 8 chunks], chunk ^ (k & 3 | (k >> 3 & 3) << 2): the 16 k rows that
-//                    a wave's transposed reads touch land on 16 different chunks.
+//                    a wave's transposed reads touch land on 16 different chunks (64 rows, 8 chunks
+//                    an LDS row, two LDS rows over all banks: bits 1, 3 and 4 of k).
 template <int ROWS, bool T>
 struct TileMap {
   static constexpr int kChunks = T ? ROWS / 8 : 8;               // per LDS row
   static constexpr int kRowsPerLoad = 64 / kChunks;
 };
-__device__ __forceinline__ int swz_t(int k) { return (k & 3) | ((k >> 3 & 3) << 2); }
+template <int ROWS>
+__device__ __forceinline__ int swz_t(int k) {
+  return ROWS == 64 ? (k >> 1 & 1) | (k >> 2 & 6) : (k & 3) | ((k >> 3 & 3) << 2);
+}
 
 // One block: a BM×BN tile of D (kEpiGate: BM×BN/2 of g and of u), WM×WN waves of 16×16×32 MFMAs, k in
 // stages of kBK that travel from HBM straight into LDS through a ring of NS stages, NS − 1 of them in
@@ -285,14 +400,14 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
 #pragma unroll
   for (int i = 0; i < LA; i++) {
     constexpr int C = TileMap<BM, TA>::kChunks;
-    const int r = (wave * LA + i) * TileMap<BM, TA>::kRowsPerLoad + lane / C, ch = (lane % C) ^ (TA ? swz_t(r) : r & 7);
+    const int r = (wave * LA + i) * TileMap<BM, TA>::kRowsPerLoad + lane / C, ch = (lane % C) ^ (TA ? swz_t<BM>(r) : r & 7);
     offA[i] = (unsigned)r * (unsigned)a.lda * 2 + ch * 16;
   }
 #pragma unroll
   for (int i = 0; i < LB; i++) {
     constexpr int C = TileMap<BN, TB>::kChunks;
     int r = (wave * LB + i) * TileMap<BN, TB>::kRowsPerLoad + lane / C;
-    const int ch = (lane % C) ^ (TB ? swz_t(r) : (r & 3) | ((r >> kNBit & 1) << 2));
+    const int ch = (lane % C) ^ (TB ? swz_t<BN>(r) : (r & 3) | ((r >> kNBit & 1) << 2));
     if (EPI == kEpiGate) r %= BN / 2;
     offB[i] = (unsigned)r * (unsigned)a.ldb * 2 + ch * 16;
   }
@@ -336,12 +451,13 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
     const int up = EPI == kEpiGate && j >= NF ? BN / 2 : 0;
     return up + wn * (16 * NF) + (r >> 2) * (4 * NF) + (j % NF) * 4 + (r & 3);
   };
-  auto frag_t = [&](const char* base, int rows, int ks, int col) {
+  auto frag_t = [&](auto tile_rows, const char* base, int ks, int col) {
+    constexpr int rows = decltype(tile_rows)::value;
     s16x4 half[2];
 #pragma unroll
     for (int hb = 0; hb < 2; hb++) {
       const int k = ks * 32 + fk * 8 + hb * 4 + (fr >> 2);
-      half[hb] = read_transposed(base + k * rows * 2 + (((col >> 3) ^ swz_t(k)) << 4) + (col & 4) * 2);
+      half[hb] = read_transposed(base + k * rows * 2 + (((col >> 3) ^ swz_t<rows>(k)) << 4) + (col & 4) * 2);
     }
     return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
@@ -354,13 +470,13 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
 #pragma unroll
       for (int i = 0; i < FM; i++) {
         const int r0 = wm * (BM / WM) + i * 16;
-        if constexpr (TA) fa[i] = frag_t(reinterpret_cast<const char*>(la), BM, ks, r0 + (fr & 3) * 4);
+        if constexpr (TA) fa[i] = frag_t(IntConst<BM>{}, reinterpret_cast<const char*>(la), ks, r0 + (fr & 3) * 4);
         else fa[i] = __builtin_bit_cast(bf16x8, la[(r0 + fr) * 8 + ((ks * 4 + fk) ^ (fr & 7))]);
       }
 #pragma unroll
       for (int j = 0; j < FN; j++) {
         if constexpr (TB) {
-          fb[j] = frag_t(reinterpret_cast<const char*>(lb), BN, ks, nrow(j, (fr & 3) * 4));
+          fb[j] = frag_t(IntConst<BN>{}, reinterpret_cast<const char*>(lb), ks, nrow(j, (fr & 3) * 4));
         } else {
           const int r = nrow(j, fr);
           fb[j] = __builtin_bit_cast(bf16x8, lb[r * 8 + ((ks * 4 + fk) ^ ((r & 3) | ((r >> kNBit & 1) << 2)))]);
@@ -444,12 +560,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
             du[q] = df * u;
           }
           if (m < a.M) {
-            if (a.kept) {
-              TO* k = static_cast<TO*>(a.kept) + (int64_t)m * a.N;
-              store8<TO>(k, n, a.N, vec, h);
-              store8<TO>(k + arr, n, a.N, vec, du);
-              store8<TO>(k + 2 * arr, n, a.N, vec, f);
-            }
+            if (a.kept) store_kept<TO>(static_cast<TO*>(a.kept) + (int64_t)m * a.N, arr, n, a.N, vec, h, du, f);
             if (a.h && n < a.ldf) store_planes8<H>(a.h, (int64_t)m * a.ldf + n, (int64_t)a.M * a.ldf, a.planes, h);
           }
         }
@@ -465,26 +576,43 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
       default: finish(IntConst<kActSilu>{}); break;
     }
   } else {
-    const TO* k = static_cast<const TO*>(a.kept) + (int64_t)a.M * a.N;
+    const TO* k = static_cast<const TO*>(a.kept);
     const int64_t arr = (int64_t)a.M * a.N, plane = (int64_t)a.M * a.ldf;
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const int m = mb + i * 16;
+    for (int j = 0; j < NF; j += 2) {
+      const int n = nb + j * 4;
+      float sg[8], su[8];
 #pragma unroll
-      for (int j = 0; j < NF; j += 2) {
-        const int n = nb + j * 4;
+      for (int q = 0; q < 8; q++) sg[q] = su[q] = 0.f;
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+        const int m = mb + i * 16;
         if (m < a.M && n < a.ldf) {
           float du[8], f[8];
-          load8<TO>(k + (int64_t)m * a.N, n, a.N, vec, du);      // zeros past N: so are dg and du there
-          load8<TO>(k + arr + (int64_t)m * a.N, n, a.N, vec, f);
+          load_kept<TO>(k + (int64_t)m * a.N, arr, n, a.N, vec, du, f);   // zeros past N: so are dg and du there
 #pragma unroll
           for (int q = 0; q < 8; q++) {
             const float dh = n + q < a.N ? acc[i][j + q / 4][q % 4] : 0.f;
             du[q] *= dh;
             f[q] *= dh;
+            sg[q] += du[q];
+            su[q] += f[q];
           }
           store_planes8<H>(a.dg, (int64_t)m * a.ldf + n, plane, a.planes, du);
           store_planes8<H>(a.du, (int64_t)m * a.ldf + n, plane, a.planes, f);
+        }
+      }
+      if (a.col_part) {
+        // over the 16 rows of a fragment: lanes of a row of 16 (a whole wave takes part in the sums)
+        float* part = a.col_part + (int64_t)(m0 / BM * WM + wm) * 2 * a.N;
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+          sg[q] = group_sum<16>(sg[q]);
+          su[q] = group_sum<16>(su[q]);
+          if (fr == 0 && n + q < a.N) {
+            part[n + q] = sg[q];
+            part[a.N + n + q] = su[q];
+          }
         }
       }
     }
@@ -529,19 +657,22 @@ constexpr size_t kPartialCap = (size_t)256 << 20;   // bytes of split-K partials
 constexpr int kColChunks = 64;                      // row chunks of a column sum at most
 
 struct Tiling {
-  int bm, tiles_m, tiles_n, splits, per_split;
+  int bm, bn, tiles_m, tiles_n, splits, per_split;   // bn: columns of the output
 };
-// 256×256 tiles where they give each of the 256 CUs one, else 128×128 (two blocks a CU); a product
-// of fewer tiles than CUs splits k into runs of at least 4 stages, up to about two blocks a CU.
+// The largest of three tiles that still gives the 256 CUs a block each: 256×256, 128×128 (two blocks a
+// CU), 64×64 (kEpiGate: half as many columns of g and of u each, 64×64 with 64).  Where even the smallest gives
+// fewer blocks, a product whose partial sums may be stored splits k into runs of at least 4 stages, up
+// to about two blocks a CU.
 Tiling tile(int64_t M, int64_t N, int batches, int stages, bool gate, bool may_split) {
   Tiling t{};
-  const int64_t big = ((M + 255) / 256) * ((N * (gate ? 2 : 1) + 255) / 256) * batches;
-  t.bm = big >= 224 ? 256 : 128;
-  t.tiles_m = (int)((M + t.bm - 1) / t.bm);
-  t.tiles_n = (int)((N + (gate ? t.bm / 2 : t.bm) - 1) / (gate ? t.bm / 2 : t.bm));
+  for (int b : {256, 128, 64}) {
+    t.bm = b, t.bn = gate && b > 64 ? b / 2 : b;
+    t.tiles_m = (int)((M + t.bm - 1) / t.bm), t.tiles_n = (int)((N + t.bn - 1) / t.bn);
+    if ((int64_t)t.tiles_m * t.tiles_n * batches >= 224) break;
+  }
   t.splits = 1;
   const int64_t tiles = (int64_t)t.tiles_m * t.tiles_n * batches;
-  if (may_split && tiles < 256) {
+  if (may_split && tiles < 224) {
     int64_t s = 512 / tiles;
     if (s > stages / 4) s = stages / 4;
     const int64_t cap = (int64_t)(kPartialCap / ((size_t)M * N * batches * 4));
@@ -555,11 +686,6 @@ Tiling tile(int64_t M, int64_t N, int batches, int stages, bool gate, bool may_s
 size_t partial_bytes(const Tiling& t, int64_t M, int64_t N, int batches) {
   return t.splits > 1 ? (size_t)t.splits * M * N * batches * sizeof(float) : 0;
 }
-unsigned grid_of(int64_t items) {
-  const int64_t b = (items + 255) / 256;
-  return (unsigned)(b < 8192 ? b : 8192);
-}
-
 // One call: the same walk over the steps sizes the workspace (dry: no base pointer) and launches.
 template <typename H, typename TO>
 struct Ffn {
@@ -573,6 +699,16 @@ struct Ffn {
   Ffn(const FfnArgs& fa, Mode m, void* w, hipStream_t s)
       : f(fa), mode(m), planes(m.planes), ws{static_cast<char*>(w)}, dry(!w), st(s) {}
 
+  struct Packed {
+    const void* src;
+    int64_t K;
+    Operand o;
+  };
+  PackArgs packs{};
+  int64_t pack_blocks = 0;
+  Packed packed[kMaxPacks];
+  int done = 0;
+
   int npairs() const { return planes * (planes + 1) / 2; }
   Operand planes_of(int64_t rows, int64_t cols) {
     Operand o;
@@ -583,16 +719,30 @@ struct Ffn {
   }
 
   // `src` [R][K] in product form: itself where its rows are whole stages (k contiguous) or whole
-  // 16-byte chunks (k the slow axis), else packed into the workspace
-  int operand(const void* src, int64_t R, int64_t K, bool k_slow, Operand& o) {
+  // 16-byte chunks (k the slow axis), else packed into the workspace, once a call, by the next flush()
+  Operand operand(const void* src, int64_t R, int64_t K, bool k_slow) {
+    Operand o;
     if (!mode.pack && K % (k_slow ? 8 : kBK) == 0) {
       o.p = static_cast<const char*>(src), o.rows = R, o.ld = K;
-      return kOk;
+      return o;
     }
+    for (int i = 0; i < done; i++)
+      if (packed[i].src == src && packed[i].o.rows == R && packed[i].K == K) return packed[i].o;
     o = planes_of(R, K);
-    if (dry) return kOk;
-    ffn_pack_kernel<TO, H><<<grid_of(R * o.ld / 4), 256, 0, st>>>(static_cast<const TO*>(src), R, K, planes,
-                                                                  reinterpret_cast<H*>(const_cast<char*>(o.p)), o.ld);
+    packed[done++] = {src, K, o};
+    PackJob& j = packs.job[packs.jobs++];
+    j = {src, const_cast<char*>(o.p), R, K, o.ld, pack_blocks};
+    pack_blocks += (R * o.ld / 4 + kPackQuads - 1) / kPackQuads;
+    return o;
+  }
+  int flush() {
+    packs.planes = planes;
+    const int n = packs.jobs;
+    const int64_t blocks = pack_blocks;
+    packs.jobs = 0, pack_blocks = 0;
+    if (!n || dry) return kOk;
+    const PackArgs a = [&] { PackArgs c = packs; c.jobs = n; return c; }();
+    ffn_pack_kernel<TO, H><<<(unsigned)blocks, 256, 0, st>>>(a);
     return check_launch("ffn_pack");
   }
 
@@ -616,31 +766,43 @@ struct Ffn {
     a.tiles_m = t.tiles_m, a.tiles_n = t.tiles_n, a.splits = t.splits, a.per_split = t.per_split;
     a.partial = t.splits > 1 ? static_cast<float*>(partial) : nullptr;
     const unsigned grid = (unsigned)t.tiles_m * t.tiles_n * t.splits * a.batches;
+    constexpr int SN = EPI == kEpiGate ? 128 : 64;           // LDS columns of the smallest tile
     if (t.bm == 256) ffn_gemm_kernel<H, TO, EPI, TA, TB, 256, 256, 2, 4, 2><<<grid, 512, 0, st>>>(a);
-    else if (grid >= 512) ffn_gemm_kernel<H, TO, EPI, TA, TB, 128, 128, 2, 2, 2><<<grid, 256, 0, st>>>(a);
-    else ffn_gemm_kernel<H, TO, EPI, TA, TB, 128, 128, 2, 2, 4><<<grid, 256, 0, st>>>(a);
+    else if (t.bm == 128) ffn_gemm_kernel<H, TO, EPI, TA, TB, 128, 128, 2, 2, 2><<<grid, 256, 0, st>>>(a);
+    else ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 3><<<grid, 256, 0, st>>>(a);
     if (int rc = check_launch(EPI == kEpiStore ? "ffn_gemm" : EPI == kEpiGate ? "ffn_gemm_gate" : "ffn_gemm_gate_bwd")) return rc;
     if (t.splits > 1) {
       const int64_t total = (int64_t)a.M * a.N;
-      for (int b = 0; b < a.batches; b++) {
-        ffn_reduce_kernel<TO><<<grid_of(total), 256, 0, st>>>(a.partial + b * t.splits * total, t.splits, total, a.N,
-                                                              static_cast<const TO*>(a.bias),
-                                                              static_cast<TO*>(b ? a.out2 : a.out));
-        if (int rc = check_launch("ffn_reduce")) return rc;
-      }
+      for (int b = 0; b < a.batches; b++)
+        if (int rc = reduce(a.partial + b * t.splits * total, t.splits, total, a.N, a.bias, b ? a.out2 : a.out)) return rc;
     }
     return kOk;
   }
 
-  // h (planes) and / or kept of all rows
-  int gate(const Operand& h, void* kept) {
+  // many parts of few elements: more threads an element
+  int reduce(const float* part, int parts, int64_t total, int N, const void* bias, void* out) {
+    const unsigned grid = (unsigned)((total + 63) / 64);
+    const TO* b = static_cast<const TO*>(bias);
+    if (parts > 8) ffn_reduce_kernel<TO, 16><<<grid, 1024, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
+    else ffn_reduce_kernel<TO, 4><<<grid, 256, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
+    return check_launch("ffn_reduce");
+  }
+
+  struct GateIn {
     Operand x, wg, wu;
-    if (int rc = operand(f.x, f.M, f.C, false, x)) return rc;
-    if (int rc = operand(f.wg, f.F, f.C, false, wg)) return rc;
-    if (int rc = operand(f.wu, f.F, f.C, false, wu)) return rc;
+  };
+  GateIn gate_operands() {
+    GateIn g;
+    g.x = operand(f.x, f.M, f.C, false);
+    g.wg = operand(f.wg, f.F, f.C, false);
+    g.wu = operand(f.wu, f.F, f.C, false);
+    return g;
+  }
+  // h (planes) and / or kept of all rows
+  int gate(const GateIn& in, const Operand& h, void* kept) {
     if (dry) return kOk;
     GemmArgs a{};
-    pairs(a, x, nullptr, wg, &wu, f.C);
+    pairs(a, in.x, nullptr, in.wg, &in.wu, f.C);
     a.M = (int)f.M, a.N = f.F;
     a.bias_g = f.bg, a.bias_u = f.bu, a.act = f.act, a.planes = planes;
     a.kept = kept;
@@ -649,9 +811,11 @@ struct Ffn {
   }
 
   int forward(void* y, void* kept) {
-    Operand h = planes_of(f.M, f.F), wd;
-    if (int rc = gate(h, kept)) return rc;
-    if (int rc = operand(f.wd, f.O, f.F, false, wd)) return rc;
+    const Operand h = planes_of(f.M, f.F);
+    const GateIn in = gate_operands();
+    const Operand wd = operand(f.wd, f.O, f.F, false);
+    if (int rc = flush()) return rc;
+    if (int rc = gate(in, h, kept)) return rc;
     const Tiling t = tile(f.M, f.O, 1, npairs() * (int)(h.ld / kBK), false, true);
     void* partial = ws.take(partial_bytes(t, f.M, f.O, 1));
     if (dry) return kOk;
@@ -662,44 +826,59 @@ struct Ffn {
     return gemm<kEpiStore, false, false>(a, t, partial);
   }
 
-  int column_sums(const Operand& o, int cols, void* out) {
-    const int64_t per = (o.rows + kColChunks - 1) / kColChunks, chunks = (o.rows + per - 1) / per;
+  int column_sums(const void* src, int64_t rows, int cols, void* out) {
+    const int64_t per = rows > 64 * kColChunks ? (rows + kColChunks - 1) / kColChunks : 64, chunks = (rows + per - 1) / per;
     float* part = static_cast<float*>(ws.take((size_t)chunks * cols * sizeof(float)));
     if (dry) return kOk;
-    ffn_col_sum_kernel<H><<<dim3(ceil_div(cols, 256), (unsigned)chunks), 256, 0, st>>>(reinterpret_cast<const H*>(o.p), o.rows, cols,
-                                                                                       o.ld, planes, per, part);
+    ffn_col_sum_kernel<TO><<<dim3(ceil_div(cols, 64), (unsigned)chunks), 256, 0, st>>>(static_cast<const TO*>(src), rows, cols, per,
+                                                                                       part);
     if (int rc = check_launch("ffn_col_sum")) return rc;
-    ffn_reduce_kernel<TO><<<grid_of(cols), 256, 0, st>>>(part, (int)chunks, cols, cols, static_cast<const TO*>(nullptr),
-                                                         static_cast<TO*>(out));
-    return check_launch("ffn_reduce");
+    return reduce(part, (int)chunks, cols, cols, nullptr, out);
   }
 
   int backward(const void* dy, const void* kept, const FfnGrads& o) {
-    if (!kept) {                                             // recomputed
-      void* k = ws.take((size_t)3 * f.M * f.F * sizeof(TO));
-      if (int rc = gate(Operand{}, k)) return rc;
-      kept = k;
+    const bool inner = o.dx || o.dwg || o.dwu || o.dbg || o.dbu, weights = o.dwg || o.dwu;
+    const bool again = !kept;                                // h, act'·u and act are computed again
+    GateIn in;
+    if (again) {
+      in = gate_operands();
+      kept = ws.take((size_t)kept_layers(sizeof(TO)) * f.M * f.F * sizeof(TO));
     }
-    const bool inner = o.dx || o.dwg || o.dwu || o.dbg || o.dbu;
-    Operand dg, du;
+    Operand dyr, dyk, wd, wg, wu, x, h, dg, du;
+    if (inner) dyr = operand(dy, f.M, f.O, false), wd = operand(f.wd, f.O, f.F, true);
+    if (o.dx) wg = operand(f.wg, f.F, f.C, true), wu = operand(f.wu, f.F, f.C, true);
+    if (weights) x = operand(f.x, f.M, f.C, true);
+    if (o.dwd) dyk = operand(dy, f.M, f.O, true);
+    if (o.dwd && !again) h = operand(kept, f.M, f.F, true);  // the first layer of kept
+    if (int rc = flush()) return rc;
+    if (again) {
+      if (int rc = gate(in, Operand{}, const_cast<void*>(kept))) return rc;
+      if (o.dwd) {
+        h = operand(kept, f.M, f.F, true);
+        if (int rc = flush()) return rc;
+      }
+    }
     if (inner) {
-      Operand dyo, wd;
       dg = planes_of(f.M, f.F), du = planes_of(f.M, f.F);
-      if (int rc = operand(dy, f.M, f.O, false, dyo)) return rc;
-      if (int rc = operand(f.wd, f.O, f.F, true, wd)) return rc;
+      const Tiling t = tile(f.M, f.F, 1, npairs() * (int)(round_k(f.O) / kBK), false, false);
+      const int rows = t.tiles_m * 2;                        // two waves along m in every tile
+      float* part = o.dbg || o.dbu ? static_cast<float*>(ws.take((size_t)rows * 2 * f.F * sizeof(float))) : nullptr;
       if (!dry) {
         GemmArgs a{};
-        pairs(a, dyo, nullptr, wd, nullptr, f.O);
+        pairs(a, dyr, nullptr, wd, nullptr, f.O);
         a.M = (int)f.M, a.N = f.F;
         a.planes = planes, a.kept = const_cast<void*>(kept);
         a.dg = const_cast<char*>(dg.p), a.du = const_cast<char*>(du.p), a.ldf = dg.ld;
-        if (int rc = gemm<kEpiGateBwd, false, true>(a, tile(f.M, f.F, 1, a.pairs * a.ktiles, false, false), nullptr)) return rc;
+        a.col_part = part;
+        if (int rc = gemm<kEpiGateBwd, false, true>(a, t, nullptr)) return rc;
+        if (part) {
+          ffn_bias_reduce_kernel<TO><<<(unsigned)ceil_div(2 * (int64_t)f.F, 64), 1024, 0, st>>>(
+              part, rows, f.F, static_cast<TO*>(o.dbg), static_cast<TO*>(o.dbu));
+          if (int rc = check_launch("ffn_bias_reduce")) return rc;
+        }
       }
     }
     if (o.dx) {
-      Operand wg, wu;
-      if (int rc = operand(f.wg, f.F, f.C, true, wg)) return rc;
-      if (int rc = operand(f.wu, f.F, f.C, true, wu)) return rc;
       const Tiling t = tile(f.M, f.C, 1, 2 * npairs() * (int)(dg.ld / kBK), false, true);
       void* partial = ws.take(partial_bytes(t, f.M, f.C, 1));
       if (!dry) {
@@ -711,9 +890,7 @@ struct Ffn {
         if (int rc = gemm<kEpiStore, false, true>(a, t, partial)) return rc;
       }
     }
-    if (o.dwg || o.dwu) {
-      Operand x;
-      if (int rc = operand(f.x, f.M, f.C, true, x)) return rc;
+    if (weights) {
       const int both = o.dwg && o.dwu ? 2 : 1;
       const Tiling t = tile(f.F, f.C, both, npairs() * (int)(round_k(f.M) / kBK), false, true);
       void* partial = ws.take(partial_bytes(t, f.F, f.C, both));
@@ -725,39 +902,31 @@ struct Ffn {
         if (int rc = gemm<kEpiStore, true, true>(a, t, partial)) return rc;
       }
     }
-    if (o.dbg)
-      if (int rc = column_sums(dg, f.F, o.dbg)) return rc;
-    if (o.dbu)
-      if (int rc = column_sums(du, f.F, o.dbu)) return rc;
-    if (o.dwd || o.dbd) {
-      Operand dyo;
-      if (int rc = operand(dy, f.M, f.O, true, dyo)) return rc;
-      if (o.dwd) {
-        Operand h;
-        if (int rc = operand(kept, f.M, f.F, true, h)) return rc;
-        const Tiling t = tile(f.O, f.F, 1, npairs() * (int)(round_k(f.M) / kBK), false, true);
-        void* partial = ws.take(partial_bytes(t, f.O, f.F, 1));
-        if (!dry) {
-          GemmArgs a{};
-          pairs(a, dyo, nullptr, h, nullptr, f.M);
-          a.M = f.O, a.N = f.F;
-          a.out = o.dwd;
-          if (int rc = gemm<kEpiStore, true, true>(a, t, partial)) return rc;
-        }
+    if (o.dwd) {
+      const Tiling t = tile(f.O, f.F, 1, npairs() * (int)(round_k(f.M) / kBK), false, true);
+      void* partial = ws.take(partial_bytes(t, f.O, f.F, 1));
+      if (!dry) {
+        GemmArgs a{};
+        pairs(a, dyk, nullptr, h, nullptr, f.M);
+        a.M = f.O, a.N = f.F;
+        a.out = o.dwd;
+        if (int rc = gemm<kEpiStore, true, true>(a, t, partial)) return rc;
       }
-      if (o.dbd)
-        if (int rc = column_sums(dyo, f.O, o.dbd)) return rc;
     }
+    if (o.dbd)
+      if (int rc = column_sums(dy, f.M, f.O, o.dbd)) return rc;
     return kOk;
   }
 };
 
 template <typename H, typename TO>
-size_t ffn_ws(const FfnArgs& f, Mode mode, int backward, int recompute) {
-  static char any;
+size_t ffn_ws(const FfnArgs& shape, Mode mode, int backward, int recompute) {
+  static char t[8];              // distinct tensors, none of them packed once for two
+  FfnArgs f = shape;
+  f.x = t, f.wg = t + 1, f.wu = t + 2, f.wd = t + 3;
   Ffn<H, TO> r(f, mode, nullptr, nullptr);
-  if (backward) r.backward(&any, recompute ? nullptr : &any, FfnGrads{&any, &any, &any, &any, &any, &any, &any});
-  else r.forward(&any, nullptr);
+  if (backward) r.backward(t + 4, recompute ? nullptr : t + 5, FfnGrads{t, t, t, t, t, t, t});
+  else r.forward(t, nullptr);
   return r.ws.used;
 }
 

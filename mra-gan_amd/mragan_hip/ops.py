@@ -1209,6 +1209,10 @@ def layer_norm_bwd(x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, dy: 
     return dx, dw, db
 
 
+def _kept_shape(x, M, F):
+    return (3 if x.dtype == torch.float32 else 4, M, F)
+
+
 def _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
     dt = _token_dtype(x, "gated_ffn.x")
     if act not in GATE_ACT:
@@ -1230,13 +1234,13 @@ def gated_ffn_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_d
                   b_down: Optional[torch.Tensor] = None, act: str = "silu", keep: bool = False):
     """y = (act(x·w_gateᵀ + b_gate) · (x·w_upᵀ + b_up))·w_downᵀ + b_down for x [..., C], w_gate, w_up [F, C],
     w_down [O, F], one type throughout; act: silu, gelu or one of ACT.  float32 tensors are multiplied in
-    set_conv_precision's mode.  Returns (y [..., O], kept): kept [3, rows, F] spares the backward the first
-    two products (keep=True), else None."""
+    set_conv_precision's mode.  Returns (y [..., O], kept): kept ([3, rows, F], 16-bit types [4, rows, F]) spares
+    the backward the first two products (keep=True), else None."""
     dt, C, F, O = _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
     x, w_gate, w_up, w_down, b_gate, b_up, b_down = map(_dense, (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
     M = x.numel() // C
     y = torch.empty(x.shape[:-1] + (O,), device=x.device, dtype=x.dtype)
-    kept = torch.empty((3, M, F), device=x.device, dtype=x.dtype) if keep else None
+    kept = torch.empty(_kept_shape(x, M, F), device=x.device, dtype=x.dtype) if keep else None
     nbytes = query("mragan_gated_ffn_workspace", M, C, F, O, dt, 0, 0)
     ws = _scratch(nbytes, x)
     fn = lambda: _call_on(x, "mragan_gated_ffn_fwd", _ptr(x), M, C, F, O, dt, _ptr(w_gate), _ptr(w_up), _ptr(w_down),
@@ -1255,7 +1259,7 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_d
     dt, C, F, O = _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
     _like(dy, "gated_ffn_bwd.dy", x, x.shape[:-1] + (O,))
     M = x.numel() // C
-    _like(kept, "gated_ffn_bwd.kept", x, (3, M, F))
+    _like(kept, "gated_ffn_bwd.kept", x, _kept_shape(x, M, F))
     like = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
     grads = [torch.empty(t.shape, device=x.device, dtype=x.dtype) if n and t is not None else None for t, n in zip(like, need)]
     if M == 0:                                             # no rows: empty sums

@@ -309,7 +309,7 @@ layer_norm.register_autograd(_ln_backward, setup_context=_ln_setup)
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
               b_gate: Optional[torch.Tensor], b_up: Optional[torch.Tensor], b_down: Optional[torch.Tensor], act: str,
               keep: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(y, kept).  keep: hold the inner products for the backward ([3, rows, F]); else kept is empty and a backward
+    """(y, kept).  keep: hold the inner products for the backward; else kept is empty and a backward
     computes them again (inference, or less memory for a third more work)."""
     y, kept = ops.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep)
     return y, x.new_empty(0) if kept is None else kept
@@ -319,7 +319,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act, keep):
     rows = x.numel() // x.shape[-1]
     return (x.new_empty(x.shape[:-1] + (w_down.shape[0],)),
-            x.new_empty((3, rows, w_gate.shape[0])) if keep else x.new_empty(0))
+            x.new_empty(ops._kept_shape(x, rows, w_gate.shape[0])) if keep else x.new_empty(0))
 
 
 def _ffn_setup(ctx, inputs, output):

@@ -17,7 +17,7 @@ def test_fake_shapes():
         assert y.shape == x.shape and y.dtype == x.dtype and mean.shape == rstd.shape == (2, 4, 4, 4) and mean.dtype == torch.float32
         w = [torch.empty(s, dtype=torch.bfloat16) for s in ((200, 96), (200, 96), (48, 200))]
         y, kept = m.gated_ffn(x, *w, None, None, None, "silu", True)
-        assert y.shape == (2, 4, 4, 4, 48) and kept.shape == (3, 128, 200) and kept.dtype == torch.bfloat16
+        assert y.shape == (2, 4, 4, 4, 48) and kept.shape == (4, 128, 200) and kept.dtype == torch.bfloat16
         assert m.gated_ffn(x, *w, None, None, None, "silu", False)[1].numel() == 0
         s = torch.empty(3, 300, 96)
         y, last, carry = m.linear_recurrence(s, s, None, None, False)

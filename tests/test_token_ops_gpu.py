@@ -197,12 +197,12 @@ def check_ffn(ops, a, b, dy, act, mode="f32", keep=True, need=(True,) * 7):
     grads = ops.gated_ffn_bwd(*a, dy, kept, *b, act=act, need=need)
     dh = mm(g_out, wd)
     edh = k(O) * mm(g_out.abs(), wd.abs())
-    kr = u(T)                                                  # P and f are kept in the tensors' type
+    kr = E if T == torch.float32 else 2.0 ** -16               # P and f are kept with 24 bits
     dg, du = dh * P, dh * f
-    edg = edh * P.abs() + (dh.abs() + edh) * (eP + kr * P.abs() + tiny(T)) + (h_v + 2 * E) * dg.abs() + t16
-    edu = edh * f.abs() + (dh.abs() + edh) * (ef + kr * f.abs() + tiny(T)) + (h_v + 2 * E) * du.abs() + t16
+    edg = edh * P.abs() + (dh.abs() + edh) * (eP + kr * P.abs() + 1e-38) + (h_v + 2 * E) * dg.abs() + t16
+    edu = edh * f.abs() + (dh.abs() + edh) * (ef + kr * f.abs() + 1e-38) + (h_v + 2 * E) * du.abs() + t16
     wants = [mm(dg, wg) + mm(du, wu), mm(dg.t(), x), mm(du.t(), x), mm(g_out.t(), h), dg.sum(0), du.sum(0), g_out.sum(0)]
-    ek = eh + (kr + h_v) * h.abs() + t16 + tiny(T)             # h as kept, then as an operand
+    ek = eh + (u(T) + h_v) * h.abs() + t16 + tiny(T)             # h as kept, then as an operand
     bounds = [mm(edg, wg.abs()) + mm(edu, wu.abs()) + k(2 * F) * (mm(dg.abs(), wg.abs()) + mm(du.abs(), wu.abs())),
               mm(edg.t(), x.abs()) + k(M) * mm(dg.abs().t(), x.abs()), mm(edu.t(), x.abs()) + k(M) * mm(du.abs().t(), x.abs()),
               mm(g_out.abs().t(), ek) + k(M) * mm(g_out.abs().t(), h.abs()), edg.sum(0) + k(M) * dg.abs().sum(0),
@@ -257,7 +257,7 @@ def test_gated_ffn_views_and_empty(ops):
     y2, _ = ops.gated_ffn_fwd(x.contiguous(), wg, wu, wd, *b)
     assert y.shape == (2, 3, 4, 33) and torch.equal(y.reshape(24, 33), y2)
     y, kept = ops.gated_ffn_fwd(x[:0], wg, wu, wd, *b, keep=True)
-    assert y.shape == (0, 33) and kept.shape == (3, 0, 40)
+    assert y.shape == (0, 33) and kept.shape == (4, 0, 40)
     grads = ops.gated_ffn_bwd(x[:0], wg, wu, wd, dy[:0], kept, *b)
     assert all(not g.any() for g in grads) and grads[1].shape == wg.shape
 
