@@ -362,8 +362,7 @@ __device__ __forceinline__ int swz_t(int k) {
 }
 
 // One block: a BM×BN tile of D (kEpiGate: BM×BN/2 of g and of u), WM×WN waves of 16×16×32 MFMAs, k in
-// stages of kBK that travel from HBM straight into LDS through a ring of NS stages, NS − 1 of them in
-// flight while one is multiplied; one barrier a stage.  Rows past an operand's
+// stages of kBK that travel from HBM straight into LDS through a ring of NS stages; one barrier a stage.  Rows past an operand's
 // edge and k past its end are outside the buffer descriptor and arrive as zeros.  The right
 // operand's fragment is the first MFMA operand, and its fragment rows are chosen so that a lane ends
 // with 4·NF consecutive n of one row m (nrow), which the epilogue moves 16 bytes at a time.
@@ -411,31 +410,54 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
     if (EPI == kEpiGate) r %= BN / 2;
     offB[i] = (unsigned)r * (unsigned)a.ldb * 2 + ch * 16;
   }
-  // descriptor of an operand from its row r0 and the k of stage t on, to its end
-  auto window = [&](const void* p, bool trans, int64_t ld, int64_t rows, int r0, int64_t k) {
-    const int64_t first = trans ? k * ld + r0 : r0 * ld + k, all = (trans ? a.K : rows) * ld;
-    int64_t left = (all - first) * 2;
-    if (left < 0) left = 0;
-    if (left > 0x7ffffff0) left = 0x7ffffff0;
-    return descriptor(static_cast<const char*>(p) + first * 2, (uint32_t)left);
+  // An operand from the next stage's first row and k to its end: the base and size of its descriptor.
+  // They move on by a constant inside a pair and are set anew at the next one.
+  struct Window {
+    const char* p;
+    int64_t left;                                                  // bytes
+    __device__ __forceinline__ i32x4 rsrc() const {
+      return descriptor(p, left <= 0 ? 0u : left > 0x7ffffff0 ? 0x7ffffff0u : (uint32_t)left);
+    }
+  };
+  auto window = [&](const void* q, bool trans, int64_t ld, int64_t rows, int r0, int64_t k) {
+    const int64_t first = trans ? k * ld + r0 : r0 * ld + k;
+    return Window{static_cast<const char*>(q) + first * 2, ((trans ? a.K : rows) * ld - first) * 2};
+  };
+  const int64_t stepA = kBK * 2 * (TA ? a.lda : 1), stepB = kBK * 2 * (TB ? a.ldb : 1);
+  Window wa, wb, wb2;
+  // The row tiles of a group start their (circular) walk over the stages two apart: rows of whole
+  // multiples of 4 KB have the same k in the same channel of the L2, and in step all blocks would ask
+  // that one channel.  Blocks of one row tile stay in step and share its rows.
+  const int kfirst = kt;
+  int cur = kt + (kt < kend ? in_group % rows_in * 2 % (kend - kt) : 0), pair = cur / a.ktiles, in_pair = cur - pair * a.ktiles;
+  auto open = [&] {
+    const int64_t k = (int64_t)in_pair * kBK;
+    wa = window(batch ? a.A2[pair] : a.A[pair], TA, a.lda, a.M, m0, k);
+    wb = window(a.B[pair], TB, a.ldb, a.N, n0, k);
+    if constexpr (EPI == kEpiGate) wb2 = window(a.B2[pair], TB, a.ldb, a.N, n0, k);
+  };
+  auto advance = [&] {
+    in_pair++;
+    if (++cur == kend || in_pair == a.ktiles) {
+      if (cur == kend) cur = kfirst;
+      pair = cur / a.ktiles, in_pair = cur - pair * a.ktiles;
+      open();
+    } else {
+      wa.p += stepA, wa.left -= stepA;
+      wb.p += stepB, wb.left -= stepB;
+      if constexpr (EPI == kEpiGate) wb2.p += stepB, wb2.left -= stepB;
+    }
   };
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)&lds[0][0];
-  auto stage = [&](int t, int buf) {
-    const int p = t / a.ktiles;
-    const int64_t k = (int64_t)(t - p * a.ktiles) * kBK;
-    const i32x4 ra = window(batch ? a.A2[p] : a.A[p], TA, a.lda, a.M, m0, k);
-    const i32x4 rb = window(a.B[p], TB, a.ldb, a.N, n0, k);
-    const unsigned la = lds0 + buf * ((BM + BN) * 128) + wave * (LA * 1024);
-    const unsigned lb = lds0 + buf * ((BM + BN) * 128) + BM * 128 + wave * (LB * 1024);
-#pragma unroll
-    for (int i = 0; i < LA; i++) load_to_lds(ra, la + i * 1024, offA[i]);
-    if constexpr (EPI == kEpiGate) {
-      const i32x4 rb2 = window(a.B2[p], TB, a.ldb, a.N, n0, k);
-#pragma unroll
-      for (int i = 0; i < LB; i++) load_to_lds((wave * LB + i) * 8 >= BN / 2 ? rb2 : rb, lb + i * 1024, offB[i]);
+  // load `i` of this wave's LA + LB of a stage, into the ring's slot
+  auto issue = [&](int i, int slot) {
+    const unsigned l = lds0 + slot * ((BM + BN) * 128);
+    if (i < LA) {
+      load_to_lds(wa.rsrc(), l + (wave * LA + i) * 1024, offA[i < LA ? i : 0]);
     } else {
-#pragma unroll
-      for (int i = 0; i < LB; i++) load_to_lds(rb, lb + i * 1024, offB[i]);
+      const int j = i - LA;
+      const bool up = EPI == kEpiGate && (wave * LB + j) * 8 >= BN / 2;
+      load_to_lds(up ? wb2.rsrc() : wb.rsrc(), l + BM * 128 + (wave * LB + j) * 1024, offB[j < 0 ? 0 : j]);
     }
   };
 
@@ -461,49 +483,84 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
     }
     return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto compute = [&](int buf) {
-    const uint4* la = lds[buf];
-    const uint4* lb = lds[buf] + BM * 8;
-#pragma unroll
-    for (int ks = 0; ks < kBK / 32; ks++) {
-      bf16x8 fa[FM], fb[FN];
-#pragma unroll
-      for (int i = 0; i < FM; i++) {
-        const int r0 = wm * (BM / WM) + i * 16;
-        if constexpr (TA) fa[i] = frag_t(IntConst<BM>{}, reinterpret_cast<const char*>(la), ks, r0 + (fr & 3) * 4);
-        else fa[i] = __builtin_bit_cast(bf16x8, la[(r0 + fr) * 8 + ((ks * 4 + fk) ^ (fr & 7))]);
+  struct Frags {
+    bf16x8 a[FM], b[FN];
+  };
+  // fragment `i` of FN + FM of k step ks in a slot
+  auto read = [&](int slot, int ks, int i, Frags& f) {
+    const uint4* la = lds[slot];
+    const uint4* lb = lds[slot] + BM * 8;
+    if (i < FN) {
+      if constexpr (TB) {
+        f.b[i] = frag_t(IntConst<BN>{}, reinterpret_cast<const char*>(lb), ks, nrow(i, (fr & 3) * 4));
+      } else {
+        const int r = nrow(i, fr);
+        f.b[i] = __builtin_bit_cast(bf16x8, lb[r * 8 + ((ks * 4 + fk) ^ ((r & 3) | ((r >> kNBit & 1) << 2)))]);
       }
-#pragma unroll
-      for (int j = 0; j < FN; j++) {
-        if constexpr (TB) {
-          fb[j] = frag_t(IntConst<BN>{}, reinterpret_cast<const char*>(lb), ks, nrow(j, (fr & 3) * 4));
-        } else {
-          const int r = nrow(j, fr);
-          fb[j] = __builtin_bit_cast(bf16x8, lb[r * 8 + ((ks * 4 + fk) ^ ((r & 3) | ((r >> kNBit & 1) << 2)))]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mfma16<H>(fb[j], fa[i], acc[i][j]);
+    } else {
+      const int r0 = wm * (BM / WM) + (i - FN) * 16;
+      if constexpr (TA) f.a[i - FN] = frag_t(IntConst<BM>{}, reinterpret_cast<const char*>(la), ks, r0 + (fr & 3) * 4);
+      else f.a[i - FN] = __builtin_bit_cast(bf16x8, la[(r0 + fr) * 8 + ((ks * 4 + fk) ^ (fr & 7))]);
     }
   };
 
-  // iteration kt: stage kt has landed for every wave, and every wave is done with stage kt − 1, whose
-  // slot takes stage kt + NS − 1
-  int put = 0, get = 0;
+  // A stage is two k steps of 32.  A k step's products go row by row of fragments, and between the rows
+  // go the reads of the next step's fragments and, in the second step, the loads of stage kt + NS (the
+  // matrix unit runs on while the wave issues them; sched_barrier keeps the order).  Between the two
+  // steps all waves meet: the next stage has landed for each, and the slot of this one, read by all,
+  // is free for the loads.
+  constexpr int L = LA + LB, NR = FM + FN;
+  static_assert(kBK == 64, "");
+  int get = 0;
+  if (kt < kend) {
+    open();
 #pragma unroll
-  for (int i = 0; i < NS - 1; i++)
-    if (kt + i < kend) stage(kt + i, put++);
-  for (; kt < kend; kt++) {
-    if (kt + NS - 2 < kend) wait_and_barrier<(NS - 2) * (LA + LB)>();
+    for (int s = 0; s < NS; s++)
+      if (kt + s < kend) {
+#pragma unroll
+        for (int i = 0; i < L; i++) issue(i, s);
+        advance();
+      }
+    Frags f0, f1;
+    if (kt + NS - 1 < kend) wait_and_barrier<(NS - 1) * L>();
     else wait_and_barrier<0>();
-    if (kt + NS - 1 < kend) {
-      stage(kt + NS - 1, put);
-      put = put + 1 == NS ? 0 : put + 1;
-    }
-    compute(get);
-    get = get + 1 == NS ? 0 : get + 1;
+#pragma unroll
+    for (int i = 0; i < NR; i++) read(0, 0, i, f0);
+    auto both_steps = [&](auto more_c, auto load_c) {                // stages kt + 1, kt + NS follow
+      constexpr bool more = decltype(more_c)::value, load = decltype(load_c)::value;
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mfma16<H>(f0.b[j], f0.a[i], acc[i][j]);
+#pragma unroll
+        for (int r = i * NR / FM; r < (i + 1) * NR / FM; r++) read(get, 1, r, f1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const int slot = get;
+      if constexpr (more) {
+        if (load || kt + NS - 1 < kend) wait_and_barrier<(NS - 2) * L>();
+        else wait_and_barrier<0>();
+        get = get + 1 == NS ? 0 : get + 1;
+      }
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mfma16<H>(f1.b[j], f1.a[i], acc[i][j]);
+        if constexpr (more) {
+#pragma unroll
+          for (int r = i * NR / FM; r < (i + 1) * NR / FM; r++) read(get, 0, r, f0);
+        }
+        if constexpr (load) {
+#pragma unroll
+          for (int r = i * L / FM; r < (i + 1) * L / FM; r++) issue(r, slot);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (load) advance();
+    };
+    for (; kt + NS < kend; kt++) both_steps(IntConst<1>{}, IntConst<1>{});
+    for (; kt + 1 < kend; kt++) both_steps(IntConst<1>{}, IntConst<0>{});
+    both_steps(IntConst<0>{}, IntConst<0>{});
   }
 
   // ---- epilogue: lane holds n = nb … nb + 4·NF − 1 of the rows m = … + i·16 + fr ----------------
@@ -811,11 +868,14 @@ struct Ffn {
   }
 
   int forward(void* y, void* kept) {
-    const Operand h = planes_of(f.M, f.F);
+    // kept's first layer is h as the next product takes it, unless that needs planes or padding
+    const bool direct = !mode.pack && f.F % kBK == 0;
+    Operand h = planes_of(f.M, f.F);
+    if (direct && kept) h.p = static_cast<const char*>(kept);
     const GateIn in = gate_operands();
     const Operand wd = operand(f.wd, f.O, f.F, false);
     if (int rc = flush()) return rc;
-    if (int rc = gate(in, h, kept)) return rc;
+    if (int rc = gate(in, direct && kept ? Operand{} : h, kept)) return rc;
     const Tiling t = tile(f.M, f.O, 1, npairs() * (int)(h.ld / kBK), false, true);
     void* partial = ws.take(partial_bytes(t, f.M, f.O, 1));
     if (dry) return kOk;
