@@ -18,6 +18,8 @@
 // The forward keeps h, act'(g)·u and act(g) for the backward, whose epilogue is then two products
 // with dh; h is the operand of dWd as it stands.
 #pragma once
+#include <type_traits>
+
 #include "prec.h"
 #include "token_ops.h"
 
@@ -238,93 +240,121 @@ __device__ __forceinline__ f32x4 mfma16(const bf16x8& a, const bf16x8& b, f32x4 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// eight consecutive values of a row from column n; `vec`: rows of whole, aligned groups of eight
+// Addresses of the epilogue: a wave-uniform pointer and the lane's offset in elements (below 2³² bytes), so
+// that the rows and layers a lane visits cost no address registers.
 template <typename TO>
-__device__ __forceinline__ void store8(TO* row, int n, int N, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ TO* lane_ptr(TO* uniform, unsigned lane) {
+  return reinterpret_cast<TO*>(reinterpret_cast<char*>(const_cast<std::remove_const_t<TO>*>(uniform)) + (size_t)(lane * (unsigned)sizeof(TO)));
+}
+// eight consecutive values of a row, `left` of them before its end; `vec`: rows of whole, aligned groups of eight
+template <typename TO>
+__device__ __forceinline__ void store8(TO* p, unsigned lane, int left, bool vec, const float (&v)[8]) {
+  TO* q = lane_ptr(p, lane);
   if (vec) {
-    if (n < N) store_vec<TO, 8>(row + n, v);
+    if (left > 0) store_vec<TO, 8>(q, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++)
-      if (n + i < N) row[n + i] = (TO)v[i];
+      if (i < left) q[i] = (TO)v[i];
   }
 }
 template <typename TO>
-__device__ __forceinline__ void load8(const TO* row, int n, int N, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void load8(const TO* row, int left, float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = 0.f;
-  if (vec) {
-    if (n < N) load_vec<TO, 8>(row + n, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (n + i < N) v[i] = (float)row[n + i];
-  }
+  for (int i = 0; i < 8; i++) v[i] = i < left ? (float)row[i] : 0.f;
 }
+template <int V>
+struct IntConst {
+  static constexpr int value = V;
+};
+
 // What the forward keeps for the backward, as layers [M][N] of TO: h, then P = act'(g)·u and f = act(g).
 // fp32 tensors: a layer each.  16-bit tensors: P and f with 24 bits of their fp32 form (rounding them to
 // the type would cost dg and du as much again as their own rounding): a layer of the upper halves
 // each, and one with the next byte of both.
 constexpr int kept_layers(size_t element) { return element == 4 ? 3 : 4; }
 template <typename TO>
-__device__ __forceinline__ void store_kept(TO* k, int64_t layer, int n, int N, bool vec, const float (&h)[8], const float (&P)[8],
-                                           const float (&f)[8]) {
-  store8<TO>(k, n, N, vec, h);
+__device__ __forceinline__ void store_kept(TO* k, unsigned lane, int64_t layer, int left, bool vec, const float (&h)[8],
+                                           const float (&P)[8], const float (&f)[8]) {
+  store8<TO>(k, lane, left, vec, h);
   if constexpr (sizeof(TO) == 4) {
-    store8<TO>(k + layer, n, N, vec, P);
-    store8<TO>(k + 2 * layer, n, N, vec, f);
+    store8<TO>(k + layer, lane, left, vec, P);
+    store8<TO>(k + 2 * layer, lane, left, vec, f);
   } else {
-    Pack<uint16_t, 8> hp, hf, lo;
+    Pack<uint16_t, 8> w[3];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const uint32_t bp = __builtin_bit_cast(uint32_t, P[i]) + 0x80u, bf = __builtin_bit_cast(uint32_t, f[i]) + 0x80u;
-      hp.v[i] = bp >> 16;
-      hf.v[i] = bf >> 16;
-      lo.v[i] = (bp >> 8 & 0xffu) | (bf & 0xff00u);
+      w[0].v[i] = bp >> 16;
+      w[1].v[i] = bf >> 16;
+      w[2].v[i] = (bp >> 8 & 0xffu) | (bf & 0xff00u);
     }
-    uint16_t* q = reinterpret_cast<uint16_t*>(k) + layer + n;
-    if (vec) {
-      if (n < N) {
-        *reinterpret_cast<Pack<uint16_t, 8>*>(q) = hp;
-        *reinterpret_cast<Pack<uint16_t, 8>*>(q + layer) = hf;
-        *reinterpret_cast<Pack<uint16_t, 8>*>(q + 2 * layer) = lo;
-      }
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (n + i < N) q[i] = hp.v[i], q[layer + i] = hf.v[i], q[2 * layer + i] = lo.v[i];
+    for (int l = 0; l < 3; l++) {
+      uint16_t* q = lane_ptr(reinterpret_cast<uint16_t*>(k) + (l + 1) * layer, lane);
+      if (vec) {
+        if (left > 0) *reinterpret_cast<Pack<uint16_t, 8>*>(q) = w[l];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (i < left) q[i] = w[l].v[i];
+      }
     }
   }
 }
+// eight values of P and f as they lie in memory (aligned rows), and as fp32
 template <typename TO>
-__device__ __forceinline__ void load_kept(const TO* k, int64_t layer, int n, int N, bool vec, float (&P)[8], float (&f)[8]) {
-  if constexpr (sizeof(TO) == 4) {
-    load8<TO>(k + layer, n, N, vec, P);
-    load8<TO>(k + 2 * layer, n, N, vec, f);
-  } else {
-    Pack<uint16_t, 8> hp{}, hf{}, lo{};
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(k) + layer + n;
-    if (vec) {
-      if (n < N) {
-        hp = *reinterpret_cast<const Pack<uint16_t, 8>*>(q);
-        hf = *reinterpret_cast<const Pack<uint16_t, 8>*>(q + layer);
-        lo = *reinterpret_cast<const Pack<uint16_t, 8>*>(q + 2 * layer);
-      }
+struct KeptRaw {
+  uint4 v[sizeof(TO) == 4 ? 4 : 3];
+  __device__ __forceinline__ void load(const TO* k, unsigned lane, int64_t layer) {
+    if constexpr (sizeof(TO) == 4) {
+      const uint4 *p = reinterpret_cast<const uint4*>(lane_ptr(k + layer, lane)),
+                  *q = reinterpret_cast<const uint4*>(lane_ptr(k + 2 * layer, lane));
+      v[0] = p[0], v[1] = p[1], v[2] = q[0], v[3] = q[1];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (n + i < N) hp.v[i] = q[i], hf.v[i] = q[layer + i], lo.v[i] = q[2 * layer + i];
+      for (int i = 0; i < 3; i++) v[i] = *reinterpret_cast<const uint4*>(lane_ptr(k + (i + 1) * layer, lane));
     }
+  }
+  __device__ __forceinline__ void get(float (&P)[8], float (&f)[8]) const {
+    if constexpr (sizeof(TO) == 4) {
+      const float4 a = __builtin_bit_cast(float4, v[0]), b = __builtin_bit_cast(float4, v[1]), c = __builtin_bit_cast(float4, v[2]),
+                   d = __builtin_bit_cast(float4, v[3]);
+      P[0] = a.x, P[1] = a.y, P[2] = a.z, P[3] = a.w, P[4] = b.x, P[5] = b.y, P[6] = b.z, P[7] = b.w;
+      f[0] = c.x, f[1] = c.y, f[2] = c.z, f[3] = c.w, f[4] = d.x, f[5] = d.y, f[6] = d.z, f[7] = d.w;
+    } else {
+      const uint32_t hp[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, hf[4] = {v[1].x, v[1].y, v[1].z, v[1].w},
+                     lo[4] = {v[2].x, v[2].y, v[2].z, v[2].w};
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      P[i] = __builtin_bit_cast(float, (uint32_t)hp.v[i] << 16 | (uint32_t)(lo.v[i] & 0xff) << 8);
-      f[i] = __builtin_bit_cast(float, (uint32_t)hf.v[i] << 16 | (uint32_t)(lo.v[i] & 0xff00));
+      for (int i = 0; i < 4; i++) {
+        P[2 * i] = __builtin_bit_cast(float, hp[i] << 16 | (lo[i] & 0xffu) << 8);
+        P[2 * i + 1] = __builtin_bit_cast(float, (hp[i] & 0xffff0000u) | (lo[i] >> 8 & 0xff00u));
+        f[2 * i] = __builtin_bit_cast(float, hf[i] << 16 | (lo[i] & 0xff00u));
+        f[2 * i + 1] = __builtin_bit_cast(float, (hf[i] & 0xffff0000u) | (lo[i] >> 16 & 0xff00u));
+      }
+    }
+  }
+};
+template <typename TO>
+__device__ __forceinline__ void load_kept(const TO* k, int64_t layer, int left, float (&P)[8], float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    P[i] = f[i] = 0.f;
+    if (i < left) {
+      if constexpr (sizeof(TO) == 4) {
+        P[i] = k[layer + i], f[i] = k[2 * layer + i];
+      } else {
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(k) + layer + i;
+        const uint32_t lo = q[2 * layer];
+        P[i] = __builtin_bit_cast(float, (uint32_t)q[0] << 16 | (lo & 0xffu) << 8);
+        f[i] = __builtin_bit_cast(float, (uint32_t)q[layer] << 16 | (lo & 0xff00u));
+      }
     }
   }
 }
-// planes of eight values at element `off` of each plane (rows of whole groups of eight)
+// planes of eight values (rows of whole groups of eight)
 template <typename H>
-__device__ __forceinline__ void store_planes8(void* base, int64_t off, int64_t plane, int planes, const float (&v)[8]) {
+__device__ __forceinline__ void store_planes8(H* base, unsigned lane, int64_t plane, int planes, const float (&v)[8]) {
   H w[8][3];
 #pragma unroll
   for (int i = 0; i < 8; i++) split_planes<H>(v[i], planes, w[i]);
@@ -334,20 +364,14 @@ __device__ __forceinline__ void store_planes8(void* base, int64_t off, int64_t p
       Pack<H, 8> q;
 #pragma unroll
       for (int i = 0; i < 8; i++) q.v[i] = w[i][p];
-      *reinterpret_cast<Pack<H, 8>*>(static_cast<H*>(base) + p * plane + off) = q;
+      *reinterpret_cast<Pack<H, 8>*>(lane_ptr(base + p * plane, lane)) = q;
     }
 }
-
-template <int V>
-struct IntConst {
-  static constexpr int value = V;
-};
 
 // Tile images in LDS.  Loads write LDS linearly (16 bytes a lane), so a permutation of the 16-byte
 // chunks of a row, which spreads the fragment reads over the banks, is made on the global address.
 //   k contiguous:    [rows][8 chunks], chunk ^ swz(row).  A: row & 7, fragments read 16 successive
-//                    rows.  B: fragment rows are 4·NF apart in fours (see `nrow`), so row & 3 and the
-//                    lowest bit of that distance.
+//                    rows.  B: fragment rows are fours 8 apart (see `nrow`), so row & 3 and bit 3.
 //   rows contiguous: [64 k][ROWS / 8 chunks], chunk ^ (k & 3 | (k >> 3 & 3) << 2): the 16 k rows that
 //                    a wave's transposed reads touch land on 16 different chunks (64 rows, 8 chunks
 //                    an LDS row, two LDS rows over all banks: bits 1, 3 and 4 of k).
@@ -365,13 +389,13 @@ __device__ __forceinline__ int swz_t(int k) {
 // stages of kBK that travel from HBM straight into LDS through a ring of NS stages; one barrier a stage.  Rows past an operand's
 // edge and k past its end are outside the buffer descriptor and arrive as zeros.  The right
 // operand's fragment is the first MFMA operand, and its fragment rows are chosen so that a lane ends
-// with 4·NF consecutive n of one row m (nrow), which the epilogue moves 16 bytes at a time.
+// with eight consecutive n of a row m, four lanes with 32 (nrow): the epilogue moves 16 bytes a lane, 64
+// a row, at a time.
 template <typename H, typename TO, int EPI, bool TA, bool TB, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a) {
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2))) void ffn_gemm_kernel(const GemmArgs a) {
   constexpr int kWaves = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int NF = EPI == kEpiGate ? FN / 2 : FN;              // n fragments of one output
   constexpr int LA = BM / 8 / kWaves, LB = BN / 8 / kWaves;      // loads of a wave per stage
-  constexpr int kNBit = NF == 4 ? 4 : 3;                         // log2(4·NF)
   static_assert(NF == 4 || NF == 2, "");
   __shared__ uint4 lds[NS][(BM + BN) * 8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
@@ -406,7 +430,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
   for (int i = 0; i < LB; i++) {
     constexpr int C = TileMap<BN, TB>::kChunks;
     int r = (wave * LB + i) * TileMap<BN, TB>::kRowsPerLoad + lane / C;
-    const int ch = (lane % C) ^ (TB ? swz_t<BN>(r) : (r & 3) | ((r >> kNBit & 1) << 2));
+    const int ch = (lane % C) ^ (TB ? swz_t<BN>(r) : (r & 3) | ((r >> 3 & 1) << 2));
     if (EPI == kEpiGate) r %= BN / 2;
     offB[i] = (unsigned)r * (unsigned)a.ldb * 2 + ch * 16;
   }
@@ -471,18 +495,25 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
   // tile row of row r of n fragment j
   auto nrow = [&](int j, int r) {
     const int up = EPI == kEpiGate && j >= NF ? BN / 2 : 0;
-    return up + wn * (16 * NF) + (r >> 2) * (4 * NF) + (j % NF) * 4 + (r & 3);
+    return up + wn * (16 * NF) + (j % NF) / 2 * 32 + (r >> 2) * 8 + (j & 1) * 4 + (r & 3);
   };
-  auto frag_t = [&](auto tile_rows, const char* base, int ks, int col) {
+  // A fragment of a tile whose rows are contiguous: `at` addresses this lane's quad of the wave's first
+  // fragment in the k rows fk·8 + fr / 4; other fragments differ in bits of the chunk only, which the
+  // permutation leaves a difference by exclusive or, other k rows by a multiple of 4 (no change to it).
+  auto frag_t = [&](auto tile_rows, unsigned at, unsigned other, int slot, int ks) {
     constexpr int rows = decltype(tile_rows)::value;
     s16x4 half[2];
 #pragma unroll
-    for (int hb = 0; hb < 2; hb++) {
-      const int k = ks * 32 + fk * 8 + hb * 4 + (fr >> 2);
-      half[hb] = read_transposed(base + k * rows * 2 + (((col >> 3) ^ swz_t<rows>(k)) << 4) + (col & 4) * 2);
-    }
+    for (int hb = 0; hb < 2; hb++)
+      half[hb] = read_transposed(reinterpret_cast<const char*>(lds) + ((at ^ other) + slot * ((BM + BN) * 128)) + (ks * 32 + hb * 4) * rows * 2);
     return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
+  unsigned atA = 0, atB = 0;
+  {
+    const int k = fk * 8 + (fr >> 2);
+    if constexpr (TA) atA = k * BM * 2 + (((wm * (BM / WM / 8) + ((fr & 3) >> 1)) ^ swz_t<BM>(k)) << 4) + (fr & 1) * 8;
+    if constexpr (TB) atB = BM * 128 + k * BN * 2 + (((wn * (2 * NF) + (fr & 3)) ^ swz_t<BN>(k)) << 4);
+  }
   struct Frags {
     bf16x8 a[FM], b[FN];
   };
@@ -492,15 +523,14 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
     const uint4* lb = lds[slot] + BM * 8;
     if (i < FN) {
       if constexpr (TB) {
-        f.b[i] = frag_t(IntConst<BN>{}, reinterpret_cast<const char*>(lb), ks, nrow(i, (fr & 3) * 4));
+        f.b[i] = frag_t(IntConst<BN>{}, atB, (i >> 1) * 64 + (i & 1) * 8, slot, ks);
       } else {
         const int r = nrow(i, fr);
-        f.b[i] = __builtin_bit_cast(bf16x8, lb[r * 8 + ((ks * 4 + fk) ^ ((r & 3) | ((r >> kNBit & 1) << 2)))]);
+        f.b[i] = __builtin_bit_cast(bf16x8, lb[r * 8 + ((ks * 4 + fk) ^ ((r & 3) | ((r >> 3 & 1) << 2)))]);
       }
     } else {
-      const int r0 = wm * (BM / WM) + (i - FN) * 16;
-      if constexpr (TA) f.a[i - FN] = frag_t(IntConst<BM>{}, reinterpret_cast<const char*>(la), ks, r0 + (fr & 3) * 4);
-      else f.a[i - FN] = __builtin_bit_cast(bf16x8, la[(r0 + fr) * 8 + ((ks * 4 + fk) ^ (fr & 7))]);
+      if constexpr (TA) f.a[i - FN] = frag_t(IntConst<BM>{}, atA, (i - FN) * 32, slot, ks);
+      else f.a[i - FN] = __builtin_bit_cast(bf16x8, la[(wm * (BM / WM) + (i - FN) * 16 + fr) * 8 + ((ks * 4 + fk) ^ (fr & 7))]);
     }
   };
 
@@ -563,62 +593,73 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
     both_steps(IntConst<0>{}, IntConst<0>{});
   }
 
-  // ---- epilogue: lane holds n = nb … nb + 4·NF − 1 of the rows m = … + i·16 + fr ----------------
-  const int nb = n0 + wn * (16 * NF) + fk * (4 * NF), mb = m0 + wm * (BM / WM) + fr;
+  // ---- epilogue: lane holds n = un + j·16 + ln … + 7 (j even) of the rows m = um + i·16 + fr --------
+  const int um = m0 + wm * (BM / WM), un = n0 + wn * (16 * NF), ln = fk * 8;
   const bool vec = (a.N & 7) == 0;
+  const unsigned lane_n = (unsigned)fr * (unsigned)a.N + ln, lane_f = (unsigned)fr * (unsigned)a.ldf + ln;
+  auto at_n = [&](int i, int j) { return (int64_t)(um + i * 16) * a.N + un + j * 16; };
+  auto at_f = [&](int i, int j) { return (um + i * 16) * a.ldf + un + j * 16; };
   if constexpr (EPI == kEpiStore) {
+    TO* out = static_cast<TO*>(batch ? a.out2 : a.out);
+    float* partial = a.partial ? a.partial + ((int64_t)batch * a.splits + split) * a.M * a.N : nullptr;
 #pragma unroll
     for (int j = 0; j < NF; j += 2) {
-      const int n = nb + j * 4;
+      const int left = a.N - (un + j * 16 + ln);
       float b[8];
-      load8<TO>(static_cast<const TO*>(a.bias), n, a.bias && !a.partial ? a.N : 0, false, b);
+#pragma unroll
+      for (int q = 0; q < 8; q++) b[q] = 0.f;
+      if (a.bias && !partial) load8<TO>(static_cast<const TO*>(a.bias) + un + j * 16 + ln, left, b);
 #pragma unroll
       for (int i = 0; i < FM; i++) {
-        const int m = mb + i * 16;
         float v[8];
 #pragma unroll
         for (int q = 0; q < 8; q++) v[q] = acc[i][j + q / 4][q % 4] + b[q];
-        if (m < a.M) {
-          if (a.partial) store8<float>(a.partial + (((int64_t)batch * a.splits + split) * a.M + m) * a.N, n, a.N, vec, v);
-          else store8<TO>(static_cast<TO*>(batch ? a.out2 : a.out) + (int64_t)m * a.N, n, a.N, vec, v);
+        if (um + i * 16 + fr < a.M) {
+          if (partial) store8<float>(partial + at_n(i, j), lane_n, left, vec, v);
+          else store8<TO>(out + at_n(i, j), lane_n, left, vec, v);
         }
       }
     }
   } else if constexpr (EPI == kEpiGate) {
-    const int64_t arr = (int64_t)a.M * a.N;
+    const int64_t layer = (int64_t)a.M * a.N, plane = (int64_t)a.M * a.ldf;
 #pragma unroll
     for (int j = 0; j < NF; j += 2) {
-      const int n = nb + j * 4;
-      float bg[8], bu[8];
-      load8<TO>(static_cast<const TO*>(a.bias_g), n, a.bias_g ? a.N : 0, false, bg);
-      load8<TO>(static_cast<const TO*>(a.bias_u), n, a.bias_u ? a.N : 0, false, bu);
+      const int n = un + j * 16 + ln;
+      if (a.bias_g) {
+        float b[8];
+        load8<TO>(static_cast<const TO*>(a.bias_g) + n, a.N - n, b);
 #pragma unroll
-      for (int i = 0; i < FM; i++)
+        for (int i = 0; i < FM; i++)
 #pragma unroll
-        for (int q = 0; q < 8; q++) {
-          acc[i][j + q / 4][q % 4] += bg[q];
-          acc[i][j + NF + q / 4][q % 4] += bu[q];
-        }
+          for (int q = 0; q < 8; q++) acc[i][j + q / 4][q % 4] += b[q];
+      }
+      if (a.bias_u) {
+        float b[8];
+        load8<TO>(static_cast<const TO*>(a.bias_u) + n, a.N - n, b);
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+          for (int q = 0; q < 8; q++) acc[i][j + NF + q / 4][q % 4] += b[q];
+      }
     }
     auto finish = [&](auto act) {                                // one unrolled body per activation
 #pragma unroll
       for (int i = 0; i < FM; i++) {
-        const int m = mb + i * 16;
 #pragma unroll
         for (int j = 0; j < NF; j += 2) {
-          const int n = nb + j * 4;
+          const int left = a.N - (un + j * 16 + ln);
           float h[8], du[8], f[8];
 #pragma unroll
           for (int q = 0; q < 8; q++) {
             const float g = acc[i][j + q / 4][q % 4], u = acc[i][j + NF + q / 4][q % 4];
             float df;
             gate_act_pair(g, decltype(act)::value, f[q], df);
-            h[q] = n + q < a.N ? f[q] * u : 0.f;
+            h[q] = q < left ? f[q] * u : 0.f;
             du[q] = df * u;
           }
-          if (m < a.M) {
-            if (a.kept) store_kept<TO>(static_cast<TO*>(a.kept) + (int64_t)m * a.N, arr, n, a.N, vec, h, du, f);
-            if (a.h && n < a.ldf) store_planes8<H>(a.h, (int64_t)m * a.ldf + n, (int64_t)a.M * a.ldf, a.planes, h);
+          if (um + i * 16 + fr < a.M) {
+            if (a.kept) store_kept<TO>(static_cast<TO*>(a.kept) + at_n(i, j), lane_n, layer, left, vec, h, du, f);
+            if (a.h && a.N - left < a.ldf) store_planes8<H>(static_cast<H*>(a.h) + at_f(i, j), lane_f, plane, a.planes, h);
           }
         }
       }
@@ -634,41 +675,64 @@ __global__ __launch_bounds__(64 * WM * WN) void ffn_gemm_kernel(const GemmArgs a
     }
   } else {
     const TO* k = static_cast<const TO*>(a.kept);
-    const int64_t arr = (int64_t)a.M * a.N, plane = (int64_t)a.M * a.ldf;
+    H *dg = static_cast<H*>(a.dg), *du = static_cast<H*>(a.du);
+    const int64_t layer = (int64_t)a.M * a.N, plane = (int64_t)a.M * a.ldf;
+    const bool inside = vec && m0 + BM <= a.M && n0 + BN <= a.N;      // no row or column of the tile is cut
 #pragma unroll
     for (int j = 0; j < NF; j += 2) {
-      const int n = nb + j * 4;
+      const int left = a.N - (un + j * 16 + ln);
       float sg[8], su[8];
 #pragma unroll
       for (int q = 0; q < 8; q++) sg[q] = su[q] = 0.f;
+      auto finish = [&](int i, float (&P)[8], float (&f)[8]) {        // dg = dh·P, du = dh·act
 #pragma unroll
-      for (int i = 0; i < FM; i++) {
-        const int m = mb + i * 16;
-        if (m < a.M && n < a.ldf) {
-          float du[8], f[8];
-          load_kept<TO>(k + (int64_t)m * a.N, arr, n, a.N, vec, du, f);   // zeros past N: so are dg and du there
+        for (int q = 0; q < 8; q++) {
+          const float dh = acc[i][j + q / 4][q % 4];
+          P[q] *= dh;
+          f[q] *= dh;
+          sg[q] += P[q];
+          su[q] += f[q];
+        }
+        store_planes8<H>(dg + at_f(i, j), lane_f, plane, a.planes, P);
+        store_planes8<H>(du + at_f(i, j), lane_f, plane, a.planes, f);
+      };
+      if (inside) {
+        constexpr int G = 2;                                          // rows whose loads are in flight together
 #pragma unroll
-          for (int q = 0; q < 8; q++) {
-            const float dh = n + q < a.N ? acc[i][j + q / 4][q % 4] : 0.f;
-            du[q] *= dh;
-            f[q] *= dh;
-            sg[q] += du[q];
-            su[q] += f[q];
+        for (int i0 = 0; i0 < FM; i0 += G) {
+          KeptRaw<TO> raw[G];
+#pragma unroll
+          for (int i = 0; i < G; i++) raw[i].load(k + at_n(i0 + i, j), lane_n, layer);
+#pragma unroll
+          for (int i = 0; i < G; i++) {
+            float P[8], f[8];
+            raw[i].get(P, f);
+            finish(i0 + i, P, f);
           }
-          store_planes8<H>(a.dg, (int64_t)m * a.ldf + n, plane, a.planes, du);
-          store_planes8<H>(a.du, (int64_t)m * a.ldf + n, plane, a.planes, f);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+          if (um + i * 16 + fr < a.M && a.N - left < a.ldf) {
+            float P[8], f[8];
+            load_kept<TO>(lane_ptr(k + at_n(i, j), lane_n), layer, left, P, f);   // zeros past N: so are dg and du there
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+              if (q >= left) acc[i][j + q / 4][q % 4] = 0.f;
+            finish(i, P, f);
+          }
         }
       }
       if (a.col_part) {
         // over the 16 rows of a fragment: lanes of a row of 16 (a whole wave takes part in the sums)
-        float* part = a.col_part + (int64_t)(m0 / BM * WM + wm) * 2 * a.N;
+        float* part = a.col_part + (int64_t)(m0 / BM * WM + wm) * 2 * a.N + un + j * 16 + ln;
 #pragma unroll
         for (int q = 0; q < 8; q++) {
           sg[q] = group_sum<16>(sg[q]);
           su[q] = group_sum<16>(su[q]);
-          if (fr == 0 && n + q < a.N) {
-            part[n + q] = sg[q];
-            part[a.N + n + q] = su[q];
+          if (fr == 0 && q < left) {
+            part[q] = sg[q];
+            part[a.N + q] = su[q];
           }
         }
       }
@@ -824,7 +888,8 @@ struct Ffn {
     a.partial = t.splits > 1 ? static_cast<float*>(partial) : nullptr;
     const unsigned grid = (unsigned)t.tiles_m * t.tiles_n * t.splits * a.batches;
     constexpr int SN = EPI == kEpiGate ? 128 : 64;           // LDS columns of the smallest tile
-    if (t.bm == 256) ffn_gemm_kernel<H, TO, EPI, TA, TB, 256, 256, 2, 4, 2><<<grid, 512, 0, st>>>(a);
+    constexpr int GM = EPI == kEpiGate ? 4 : 2;              // waves along m: 128-byte rows of the gate's outputs a wave
+    if (t.bm == 256) ffn_gemm_kernel<H, TO, EPI, TA, TB, 256, 256, GM, 8 / GM, 2><<<grid, 512, 0, st>>>(a);
     else if (t.bm == 128) ffn_gemm_kernel<H, TO, EPI, TA, TB, 128, 128, 2, 2, 2><<<grid, 256, 0, st>>>(a);
     else ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 3><<<grid, 256, 0, st>>>(a);
     if (int rc = check_launch(EPI == kEpiStore ? "ffn_gemm" : EPI == kEpiGate ? "ffn_gemm_gate" : "ffn_gemm_gate_bwd")) return rc;
