@@ -293,7 +293,7 @@ __device__ __forceinline__ void store_kept(TO* k, unsigned lane, int64_t layer, 
     for (int l = 0; l < 3; l++) {
       uint16_t* q = lane_ptr(reinterpret_cast<uint16_t*>(k) + (l + 1) * layer, lane);
       if (vec) {
-        if (left > 0) *reinterpret_cast<Pack<uint16_t, 8>*>(q) = w[l];
+        if (left > 0) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, w[l]), reinterpret_cast<i32x4*>(q));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -313,7 +313,8 @@ struct KeptRaw {
       v[0] = p[0], v[1] = p[1], v[2] = q[0], v[3] = q[1];
     } else {
 #pragma unroll
-      for (int i = 0; i < 3; i++) v[i] = *reinterpret_cast<const uint4*>(lane_ptr(k + (i + 1) * layer, lane));
+      for (int i = 0; i < 3; i++)
+        v[i] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(lane_ptr(k + (i + 1) * layer, lane))));
     }
   }
   __device__ __forceinline__ void get(float (&P)[8], float (&f)[8]) const {
