@@ -741,6 +741,174 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   }
 }
 
+// ---- few rows ---------------------------------------------------------------------------------
+// Up to kSkinnyRows rows in inference: the time is that of reading the weights once, so nothing is
+// staged.  A block takes 16 rows of a weight, its waves split k; a lane loads 16 bytes of a weight row
+// and of each 16 rows of x straight into MFMA fragments, the waves' sums meet in LDS.  h stays in fp32
+// between the two launches and enters the second as two planes (16-bit tensors).
+constexpr int kSkinnyRows = 64;
+
+// eight elements from k as the fragments of P planes; zeros at and behind K (a multiple of eight)
+template <typename H, typename T, int P>
+__device__ __forceinline__ void load_frags(const T* row, int64_t k, int64_t K, bf16x8 (&out)[P]) {
+  if constexpr (sizeof(T) == 2 && P == 1) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k < K) v = *reinterpret_cast<const uint4*>(row + k);
+    out[0] = __builtin_bit_cast(bf16x8, v);
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = 0.f;
+    if (k < K) load_vec<T, 8>(row + k, v);
+    Pack<H, 8> w[3];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      H e[3];
+      split_planes<H>(v[i], P, e);
+#pragma unroll
+      for (int p = 0; p < 3; p++) w[p].v[i] = e[p];
+    }
+#pragma unroll
+    for (int p = 0; p < P; p++) out[p] = __builtin_bit_cast(bf16x8, w[p]);
+  }
+}
+
+__device__ __forceinline__ float gate_act(float g, int act) {
+  float f, df;
+  gate_act_pair(g, act, f, df);
+  return f;
+}
+
+// Up to kDotRows rows of fewer than kDotCols columns: a wave per column and plain fp32 products, so that
+// every CU takes part in reading the weight (the MFMA form below gives N / 16 blocks).  Lanes walk the
+// column's weight row 16 bytes at a time.  1 row, 4096 → 1024 bf16: 6.6 us against 9.0.
+constexpr int kDotRows = 2, kDotCols = 4096;
+template <typename T>
+__device__ __forceinline__ Words<T, 8> load_words8(const T* row, int64_t k, int64_t K) {   // K a multiple of 8
+  Words<T, 8> r{};
+  if (k < K) r = *reinterpret_cast<const Words<T, 8>*>(row + k);
+  return r;
+}
+// round: the operand rounding of the one-plane modes of fp32 tensors (op_round)
+template <typename TX, typename TO, int NB, int MR>
+__global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_t K, const TO* w0, const TO* w1, const TO* b0,
+                                                      const TO* b1, int N, int act, int round, void* out) {
+  constexpr int U = 8 / NB / MR;                                   // loads of a weight row in flight
+  const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  const TO* w[2] = {w0 + n * K, NB == 2 ? w1 + n * K : nullptr};
+  float acc[NB][MR];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int m = 0; m < MR; m++) acc[b][m] = 0.f;
+  for (int64_t k0 = lane * 8; k0 < K; k0 += 512 * U) {
+    Words<TO, 8> wv[U][NB];
+    Words<TX, 8> xv[U][MR];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+      for (int b = 0; b < NB; b++) wv[u][b] = load_words8(w[b], k0 + u * 512, K);
+#pragma unroll
+      for (int m = 0; m < MR; m++) xv[u][m] = load_words8(x + (int64_t)(m < M ? m : M - 1) * K, k0 + u * 512, K);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int m = 0; m < MR; m++)
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) acc[b][m] += op_round(xv[u][m].get(i), round) * op_round(wv[u][b].get(i), round);
+  }
+#pragma unroll
+  for (int m = 0; m < MR; m++) {
+    float v[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) v[b] = group_sum<64>(acc[b][m]);
+    if (lane == 0 && m < M) {
+      float r = v[0] + (b0 ? (float)b0[n] : 0.f);
+      if constexpr (NB == 2) {
+        r = gate_act(r, act) * (v[1] + (b1 ? (float)b1[n] : 0.f));
+        static_cast<float*>(out)[(int64_t)m * N + n] = r;
+      } else {
+        static_cast<TO*>(out)[(int64_t)m * N + n] = (TO)r;
+      }
+    }
+  }
+}
+
+// NB weights (gate and up, or down alone) times x [M][K] (TX): PX planes of x, PW of the weights.
+// out: h [M][N] in fp32 (NB = 2) or y [M][N]
+template <typename H, typename TX, typename TO, int NB, int MF, int PX, int PW, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TX* x, int M, int64_t K, const TO* w0, const TO* w1,
+                                                                const TO* b0, const TO* b1, int N, int act, void* out) {
+  constexpr int kOrder = PX > PW ? PX : PW, kFrags = MF * PX + NB * PW;
+  constexpr int U = kFrags <= 4 ? 4 : kFrags <= 8 ? 2 : 1;            // k steps whose loads are in flight
+  __shared__ f32x4 part[WAVES][NB * MF][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fk = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int64_t row = n0 + fr < N ? n0 + fr : N - 1;
+  const TO* w[2] = {w0 + row * K, NB == 2 ? w1 + row * K : nullptr};
+  f32x4 acc[NB][MF];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int m = 0; m < MF; m++) acc[b][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t steps = (K + 31) / 32, per = (steps + WAVES - 1) / WAVES, s1 = (wave + 1) * per < steps ? (wave + 1) * per : steps;
+  for (int64_t s = wave * per; s < s1; s += U) {
+    bf16x8 fw[U][NB][PW], fx[U][MF][PX];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int64_t k = (s + u) * 32 + fk * 8, end = s + u < s1 ? K : 0;
+#pragma unroll
+      for (int b = 0; b < NB; b++) load_frags<H, TO, PW>(w[b], k, end, fw[u][b]);
+#pragma unroll
+      for (int m = 0; m < MF; m++) load_frags<H, TX, PX>(x + (int64_t)(m * 16 + fr < M ? m * 16 + fr : M - 1) * K, k, end, fx[u][m]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+#pragma unroll
+          for (int o = kOrder - 1; o >= 0; o--)
+#pragma unroll
+            for (int i = 0; i < PX; i++)
+              if (o - i >= 0 && o - i < PW) acc[b][m] = mfma16<H>(fw[u][b][o - i < 0 || o - i >= PW ? 0 : o - i], fx[u][m][i], acc[b][m]);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int m = 0; m < MF; m++) part[wave][b * MF + m][lane] = acc[b][m];
+  __syncthreads();
+  // wave m joins the rows m·16 …: lane holds columns n0 + 4·fk … + 3 of row m·16 + fr
+  const int m = wave * 16 + fr;
+  if (wave < MF && m < M) {
+    f32x4 v[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      v[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < WAVES; q++) v[b] += part[q][b * MF + wave][lane];
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int n = n0 + fk * 4 + q;
+      if (n < N) {
+        float r = v[0][q] + (b0 ? (float)b0[n] : 0.f);
+        if constexpr (NB == 2) {
+          r = gate_act(r, act) * (v[1][q] + (b1 ? (float)b1[n] : 0.f));
+          static_cast<float*>(out)[(int64_t)m * N + n] = r;
+        } else {
+          static_cast<TO*>(out)[(int64_t)m * N + n] = (TO)r;
+        }
+      }
+    }
+  }
+}
+
 // ---- host -------------------------------------------------------------------------------------
 // How the operands become 16-bit planes
 struct Mode {
@@ -933,7 +1101,39 @@ struct Ffn {
     return gemm<kEpiGate, false, false>(a, tile(f.M, f.F, 1, a.pairs * a.ktiles, true, false), nullptr);
   }
 
+  // One launch for few rows, x [M][K]: NB = 2 gate, up → h in fp32; NB = 1 down → y.  PX, PW: planes of x, w.
+  template <int NB, int PX, int PW, typename TX>
+  int skinny(const TX* x, int64_t K, const void* w0, const void* w1, const void* b0, const void* b1, int N, void* out) {
+    const TO *v0 = static_cast<const TO*>(w0), *v1 = static_cast<const TO*>(w1), *c0 = static_cast<const TO*>(b0),
+             *c1 = static_cast<const TO*>(b1);
+    const int M = (int)f.M;
+    if (M <= kDotRows && N < kDotCols) {
+      const int round = mode.pack && planes == 1 ? (__is_same(H, _Float16) ? kPrecF16 : kPrecBf16) : 0;
+      const unsigned grid = (unsigned)ceil_div(N, 4);
+      if (M == 1) ffn_dot_kernel<TX, TO, NB, 1><<<grid, 256, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, round, out);
+      else ffn_dot_kernel<TX, TO, NB, 2><<<grid, 256, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, round, out);
+      return check_launch("ffn_dot");
+    }
+    constexpr int W = 8;
+    const unsigned grid = (unsigned)ceil_div(N, 16);
+    if (M <= 16) ffn_skinny_kernel<H, TX, TO, NB, 1, PX, PW, W><<<grid, 64 * W, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, out);
+    else if (M <= 32) ffn_skinny_kernel<H, TX, TO, NB, 2, PX, PW, W><<<grid, 64 * W, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, out);
+    else ffn_skinny_kernel<H, TX, TO, NB, 4, PX, PW, W><<<grid, 64 * W, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, out);
+    return check_launch("ffn_skinny");
+  }
+  template <int P>
+  int few_rows(void* y, float* h) {
+    if (int rc = skinny<2, P, P, TO>(static_cast<const TO*>(f.x), f.C, f.wg, f.wu, f.bg, f.bu, f.F, h)) return rc;
+    return skinny<1, sizeof(TO) == 2 ? 2 : P, P, float>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, y);
+  }
+
   int forward(void* y, void* kept) {
+    if (!kept && f.M <= kSkinnyRows && f.C % 8 == 0 && f.F % 8 == 0) {
+      float* h = static_cast<float*>(ws.take((size_t)f.M * f.F * sizeof(float)));
+      if (dry) return kOk;
+      if constexpr (sizeof(TO) == 2) return few_rows<1>(y, h);
+      else return planes == 3 ? few_rows<3>(y, h) : planes == 2 ? few_rows<2>(y, h) : few_rows<1>(y, h);
+    }
     // kept's first layer is h as the next product takes it, unless that needs planes or padding
     const bool direct = !mode.pack && f.F % kBK == 0;
     Operand h = planes_of(f.M, f.F);
@@ -1051,9 +1251,14 @@ size_t ffn_ws(const FfnArgs& shape, Mode mode, int backward, int recompute) {
   FfnArgs f = shape;
   f.x = t, f.wg = t + 1, f.wu = t + 2, f.wd = t + 3;
   Ffn<H, TO> r(f, mode, nullptr, nullptr);
-  if (backward) r.backward(t + 4, recompute ? nullptr : t + 5, FfnGrads{t, t, t, t, t, t, t});
-  else r.forward(t, nullptr);
-  return r.ws.used;
+  if (backward) {
+    r.backward(t + 4, recompute ? nullptr : t + 5, FfnGrads{t, t, t, t, t, t, t});
+    return r.ws.used;
+  }
+  r.forward(t, t + 6);           // with kept, and without: the larger
+  Ffn<H, TO> q(f, mode, nullptr, nullptr);
+  q.forward(t, nullptr);
+  return r.ws.used > q.ws.used ? r.ws.used : q.ws.used;
 }
 
 }  // namespace

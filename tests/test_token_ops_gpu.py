@@ -243,6 +243,16 @@ def test_gated_ffn_recomputed_and_without_bias(ops, size, dtype):
     check_ffn(ops, *ffn_inputs(*size, dtype, bias=False), "silu", keep=False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("size", [(1, 1024, 4096, 1024), (1, 8, 8, 8), (2, 72, 200, 24), (16, 264, 136, 33), (17, 1000, 1000, 1000),
+                                  (33, 128, 520, 96), (64, 320, 640, 64), (65, 320, 640, 64)])
+def test_gated_ffn_few_rows(ops, size, dtype):
+    """Inference on up to 64 rows and one more; in fp32 each precision mode's planes."""
+    for mode in ("f32", "bf16x3", "bf16", "fp16") if dtype == torch.float32 else ("f32",):
+        a, b, dy = ffn_inputs(*size, dtype)
+        check_ffn(ops, a, b, dy, "silu", mode=mode, keep=False, need=(False,) * 7)
+
+
 @pytest.mark.parametrize("need", [(1, 0, 0, 0, 0, 0, 0), (0, 1, 0, 0, 0, 0, 0), (0, 0, 1, 0, 0, 0, 1), (0, 0, 0, 1, 0, 0, 0),
                                   (0, 0, 0, 0, 1, 0, 0), (0, 0, 0, 0, 0, 1, 0), (0,) * 7])
 def test_gated_ffn_some_gradients(ops, need):
