@@ -413,7 +413,7 @@ enum mragan_dtype { MRAGAN_DT_F32 = 0, MRAGAN_DT_BF16 = 1, MRAGAN_DT_F16 = 2 };
  * weight / bias ([C], type wdtype: dtype or fp32) may be NULL (1 / 0); mean and rstd ([rows]) are
  * outputs the backward reads.  bwd: dx, dweight, dbias (types as x and weight) may each be NULL to
  * skip it; dweight and dbias are reduced over the rows in a fixed order.  No tensor may overlap an
- * output, except that bwd's dx may be dy. */
+ * output. */
 int mragan_layer_norm_fwd(const void* x, int64_t rows, int C, int dtype, const void* weight, const void* bias, int wdtype,
                           float eps, void* y, float* mean, float* rstd, void* stream);
 size_t mragan_layer_norm_bwd_workspace(int64_t rows, int C, int dtype);

@@ -18,52 +18,53 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// 16 bytes of T; rows of any channel count start at any element, so the access is typed with the
-// element's alignment (gfx950 takes global accesses of any alignment; aligned ones cost the same)
+// A lane's 16 bytes of a row.  Rows of any channel count start at any element; gfx950 takes global
+// accesses of any alignment.  How a row ends:
+//   kExact    C is a multiple of N: a vector is inside the row or behind it
+//   kOverlap  the last vector of a row is moved back to end with it; what it shares with the one before
+//             is left out of the sums and written twice, with the same value
+//   kTiny     C < N: element by element
+enum RowEnd : int { kExact = 0, kOverlap = 1, kTiny = 2 };
 template <typename T>
-struct RowVec {
-  static constexpr int N = 16 / sizeof(T);
-  T v[N];
-};
+constexpr int vec_len() { return 16 / sizeof(T); }
 
-template <typename T>
-__device__ __forceinline__ RowVec<T> row_load(const T* row, int col, int C) {
-  RowVec<T> r;
-  if (col + RowVec<T>::N <= C) {
-    __builtin_memcpy(&r, row + col, 16);
-  } else {
+// vector of the columns from `col`: where it is loaded, and how many of its elements to skip (N: all)
+struct Slot {
+  int at, skip;
+};
+template <int N, int END>
+__device__ __forceinline__ Slot slot(int col, int C) {
+  if (col >= C) return {0, N};
+  if (END == kOverlap && col + N > C) return {C - N, col + N - C};
+  return {col, 0};
+}
+template <int N, int END, typename T>
+__device__ __forceinline__ Words<T, N> vec_load(const T* row, Slot s, int C) {
+  Words<T, N> r{};
+  if constexpr (END == kTiny) {
 #pragma unroll
-    for (int i = 0; i < RowVec<T>::N; i++) r.v[i] = col + i < C ? row[col + i] : (T)0.f;
+    for (int i = 0; i < N; i++) r.set(i, s.skip == 0 && i < C ? (float)row[i] : 0.f);
+  } else {
+    if (s.skip < N) __builtin_memcpy(&r, row + s.at, sizeof(r));
   }
   return r;
 }
-template <typename T>
-__device__ __forceinline__ void row_store(T* row, int col, int C, const RowVec<T>& r) {
-  if (col + RowVec<T>::N <= C) {
-    __builtin_memcpy(row + col, &r, 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < RowVec<T>::N; i++)
-      if (col + i < C) row[col + i] = r.v[i];
-  }
-}
-
-// N consecutive parameters from p (fp32 or T): `dflt` where p is null or past the row
-template <int N, typename W>
-__device__ __forceinline__ void param_load(const W* p, int col, int C, float dflt, float (&out)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; i++) out[i] = dflt;
-  if (!p) return;
-  if (col + N <= C) {
-    W t[N];
-    __builtin_memcpy(t, p + col, N * sizeof(W));
-#pragma unroll
-    for (int i = 0; i < N; i++) out[i] = (float)t[i];
-  } else {
+template <int N, int END, typename T>
+__device__ __forceinline__ void vec_store(T* row, Slot s, int C, const Words<T, N>& r) {
+  if constexpr (END == kTiny) {
 #pragma unroll
     for (int i = 0; i < N; i++)
-      if (col + i < C) out[i] = (float)p[col + i];
+      if (s.skip == 0 && i < C) row[i] = (T)r.get(i);
+  } else {
+    if (s.skip < N) __builtin_memcpy(row + s.at, &r, sizeof(r));
   }
+}
+// whether element j of a vector counts
+template <int N, int END>
+__device__ __forceinline__ bool counts(Slot s, int j, int C) {
+  if constexpr (END == kTiny) return s.skip == 0 && j < C;
+  else if constexpr (END == kExact) return s.skip == 0;
+  else return j >= s.skip;
 }
 
 // sum over the G lanes of a row; G > 64: over the block's waves through `red` (one slot per wave),
@@ -83,51 +84,57 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   }
 }
 
-template <typename T, typename W, int G, int NV>
-__global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(const T* x, int64_t rows, int C, const W* w,
-                                                                             const W* b, float eps, T* y, float* mean,
-                                                                             float* rstd) {
-  constexpr int N = RowVec<T>::N, BT = G > kThreads ? G : kThreads;
+template <typename T, typename W, int G, int NV, int END>
+__global__ __launch_bounds__(kThreads) void ln_fwd_kernel(const T* x, int64_t rows, int C, const W* w, const W* b, float eps, T* y,
+                                                          float* mean, float* rstd) {
+  constexpr int N = vec_len<T>();
   __shared__ float red[2][16];
   const int lane = threadIdx.x % G;
-  const int64_t step = (int64_t)gridDim.x * (BT / G);
-  int64_t row = (int64_t)blockIdx.x * (BT / G) + threadIdx.x / G;
+  const int64_t step = (int64_t)gridDim.x * (kThreads / G);
+  int64_t row = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
   const float inv = 1.f / (float)C;
-  RowVec<T> cur[NV], nxt[NV];
-  if (row < rows) {
+  Slot at[NV];
+  Words<W, N> wv[NV], bv[NV];                                        // held for all rows of the block
+  Words<T, N> cur[NV], nxt[NV];
 #pragma unroll
-    for (int i = 0; i < NV; i++) cur[i] = row_load(x + row * C, (i * G + lane) * N, C);
+  for (int i = 0; i < NV; i++) {
+    at[i] = slot<N, END>((i * G + lane) * N, C);
+    if (row < rows) cur[i] = vec_load<N, END>(x + row * C, at[i], C);
+    if (w) wv[i] = vec_load<N, END>(w, at[i], C);
+    if (b) bv[i] = vec_load<N, END>(b, at[i], C);
   }
   for (; row < rows; row += step) {
     if (row + step < rows) {
 #pragma unroll
-      for (int i = 0; i < NV; i++) nxt[i] = row_load(x + (row + step) * C, (i * G + lane) * N, C);
+      for (int i = 0; i < NV; i++) nxt[i] = vec_load<N, END>(x + (row + step) * C, at[i], C);
     }
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int j = 0; j < N; j++) s += (float)cur[i].v[j];          // lanes past the row hold zeros
+      for (int j = 0; j < N; j++)                                      // vectors behind the row hold zeros
+        if (END != kOverlap || counts<N, END>(at[i], j, C)) s += cur[i].get(j);
     const float mu = row_sum<G>(s, red[0]) * inv;
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
       for (int j = 0; j < N; j++) {
-        const float d = (float)cur[i].v[j] - mu;
-        if ((i * G + lane) * N + j < C) q += d * d;
+        const float d = cur[i].get(j) - mu;
+        q += counts<N, END>(at[i], j, C) ? d * d : 0.f;
       }
     const float r = rsqrtf(row_sum<G>(q, red[1]) * inv + eps);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int col = (i * G + lane) * N;
-      float wv[N], bv[N];
-      param_load<N>(w, col, C, 1.f, wv);
-      param_load<N>(b, col, C, 0.f, bv);
-      RowVec<T> o;
+      Words<T, N> o;
 #pragma unroll
-      for (int j = 0; j < N; j++) o.v[j] = (T)(((float)cur[i].v[j] - mu) * r * wv[j] + bv[j]);
-      row_store(y + row * C, col, C, o);
+      for (int j = 0; j < N; j++) {
+        float v = (cur[i].get(j) - mu) * r;
+        if (w) v *= wv[i].get(j);
+        if (b) v += bv[i].get(j);
+        o.set(j, v);
+      }
+      vec_store<N, END>(y + row * C, at[i], C, o);
     }
     if (lane == 0) {
       mean[row] = mu;
@@ -140,41 +147,39 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(con
 }
 
 // part: [gridDim.x][2][C] fp32 sums of this block's rows (Σ dy·x̂, Σ dy), or null
-template <typename T, typename W, int G, int NV>
+template <typename T, typename W, int G, int NV, int END>
 __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(const T* x, const float* mean, const float* rstd,
                                                                              const T* dy, int64_t rows, int C, const W* w,
                                                                              T* dx, float* part) {
-  constexpr int N = RowVec<T>::N, BT = G > kThreads ? G : kThreads, E = NV * N;
+  constexpr int N = vec_len<T>(), BT = G > kThreads ? G : kThreads, E = NV * N;
   __shared__ float red[2][16];
   __shared__ float acc_s[G <= 64 ? BT / 64 : 1][G <= 64 ? G * E + 1 : 1];
   const int lane = threadIdx.x % G;
   const int64_t step = (int64_t)gridDim.x * (BT / G);
   int64_t row = (int64_t)blockIdx.x * (BT / G) + threadIdx.x / G;
   const float inv = 1.f / (float)C;
-  float wv[NV][N], aw[NV][N], ab[NV][N];
+  Slot at[NV];
+  Words<W, N> wv[NV];
+  Words<T, N> cx[NV], cd[NV], nx[NV], nd[NV];
+  float aw[NV][N], ab[NV][N], mu = 0.f, r = 0.f, nmu = 0.f, nr = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; i++) {
-    param_load<N>(w, (i * G + lane) * N, C, 1.f, wv[i]);
+    at[i] = slot<N, END>((i * G + lane) * N, C);
+    if (row < rows) {
+      cx[i] = vec_load<N, END>(x + row * C, at[i], C);
+      cd[i] = vec_load<N, END>(dy + row * C, at[i], C);
+    }
+    if (w) wv[i] = vec_load<N, END>(w, at[i], C);
 #pragma unroll
     for (int j = 0; j < N; j++) aw[i][j] = ab[i][j] = 0.f;
   }
-  RowVec<T> cx[NV], cd[NV], nx[NV], nd[NV];
-  float mu = 0.f, r = 0.f, nmu = 0.f, nr = 0.f;
-  if (row < rows) {
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      cx[i] = row_load(x + row * C, (i * G + lane) * N, C);
-      cd[i] = row_load(dy + row * C, (i * G + lane) * N, C);
-    }
-    mu = mean[row];
-    r = rstd[row];
-  }
+  if (row < rows) mu = mean[row], r = rstd[row];
   for (; row < rows; row += step) {
     if (row + step < rows) {
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        nx[i] = row_load(x + (row + step) * C, (i * G + lane) * N, C);
-        nd[i] = row_load(dy + (row + step) * C, (i * G + lane) * N, C);
+        nx[i] = vec_load<N, END>(x + (row + step) * C, at[i], C);
+        nd[i] = vec_load<N, END>(dy + (row + step) * C, at[i], C);
       }
       nmu = mean[row + step];
       nr = rstd[row + step];
@@ -183,10 +188,12 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(con
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int j = 0; j < N; j++) {                                  // dy is zero past the row
-        const float d = (float)cd[i].v[j], xh = ((float)cx[i].v[j] - mu) * r, p = d * wv[i][j];
-        s1 += p;
-        s2 += p * xh;
+      for (int j = 0; j < N; j++) {                                  // dy is zero behind the row
+        const float d = cd[i].get(j), xh = (cx[i].get(j) - mu) * r, p = w ? d * wv[i].get(j) : d;
+        if (END != kOverlap || counts<N, END>(at[i], j, C)) {
+          s1 += p;
+          s2 += p * xh;
+        }
         aw[i][j] += d * xh;
         ab[i][j] += d;
       }
@@ -194,13 +201,13 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(con
       const float m1 = row_sum<G>(s1, red[0]) * inv, m2 = row_sum<G>(s2, red[1]) * inv;
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        RowVec<T> o;
+        Words<T, N> o;
 #pragma unroll
         for (int j = 0; j < N; j++) {
-          const float xh = ((float)cx[i].v[j] - mu) * r, p = (float)cd[i].v[j] * wv[i][j];
-          o.v[j] = (T)(r * (p - m1 - xh * m2));
+          const float d = cd[i].get(j), xh = (cx[i].get(j) - mu) * r, p = w ? d * wv[i].get(j) : d;
+          o.set(j, r * (p - m1 - xh * m2));
         }
-        row_store(dx + row * C, (i * G + lane) * N, C, o);
+        vec_store<N, END>(dx + row * C, at[i], C, o);
       }
       if constexpr (G > 64) __syncthreads();
     }
@@ -218,13 +225,11 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(con
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int j = 0; j < N; j++) {
-        const int col = (i * G + lane) * N + j;
-        if (col < C) {
-          out[col] = aw[i][j];
-          out[C + col] = ab[i][j];
+      for (int j = 0; j < N; j++)
+        if (counts<N, END>(at[i], j, C)) {
+          out[at[i].at + j] = aw[i][j];
+          out[C + at[i].at + j] = ab[i][j];
         }
-      }
   } else {
     const int wave = threadIdx.x >> 6;
 #pragma unroll
@@ -240,7 +245,7 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(con
           if constexpr (G <= 8) v += __shfl_xor(v, 8);
           if constexpr (G <= 16) v += __shfl_xor(v, 16);
           if constexpr (G <= 32) v += __shfl_xor(v, 32);
-          if ((threadIdx.x & 63) < G) acc_s[wave][(i * G + lane) * N + j] = v;
+          if ((threadIdx.x & 63) < G && counts<N, END>(at[i], j, C)) acc_s[wave][at[i].at + j] = v;
         }
       __syncthreads();
       for (int col = threadIdx.x; col < C; col += BT) {
@@ -260,8 +265,10 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* part
   const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + cl, n = 2 * (int64_t)C;
   float v = 0.f;
-  if (col < n)
+  if (col < n) {
+#pragma unroll 8
     for (int k = slot; k < nb; k += 32) v += part[k * n + col];
+  }
   s[slot][cl] = v;
   __syncthreads();
   if (slot == 0 && col < n) {
@@ -359,7 +366,7 @@ Shape pick(int64_t rows, int C, int N, int most) {
 template <typename T, typename W>
 int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, float eps, void* y, float* mean, float* rstd,
            hipStream_t st) {
-  constexpr int N = RowVec<T>::N;
+  constexpr int N = vec_len<T>();
   const T* xt = static_cast<const T*>(x);
   const W *wt = static_cast<const W*>(w), *bt = static_cast<const W*>(b);
   T* yt = static_cast<T*>(y);
@@ -370,16 +377,24 @@ int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, flo
   const Shape s = pick(rows, C, N, 32);
   const int64_t per = kThreads / s.G, blocks = (rows + per - 1) / per, most = 2048;
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-#define LN_RUN(G_, NV_)                                                                                                  \
-  if constexpr (NV_ * N <= 32) {                                                                                         \
-    if (s.G == G_ && s.NV == NV_) {                                                                                      \
-      ln_fwd_kernel<T, W, G_, NV_><<<grid, kThreads, 0, st>>>(xt, rows, C, wt, bt, eps, yt, mean, rstd); \
-      return check_launch("layer_norm_fwd");                                                                             \
-    }                                                                                                                    \
+#define LN_END(G_, NV_, END_)                                                                                            \
+  ln_fwd_kernel<T, W, G_, NV_, END_><<<grid, kThreads, 0, st>>>(xt, rows, C, wt, bt, eps, yt, mean, rstd)
+#define LN_RUN(G_, NV_)                                                   \
+  if constexpr (NV_ * N <= 32) {                                          \
+    if (s.G == G_ && s.NV == NV_) {                                       \
+      if (C % N == 0) LN_END(G_, NV_, kExact);                            \
+      else LN_END(G_, NV_, kOverlap);                                     \
+      return check_launch("layer_norm_fwd");                              \
+    }                                                                     \
+  }
+  if (C < N) {
+    LN_END(4, 1, kTiny);
+    return check_launch("layer_norm_fwd");
   }
   LN_RUN(4, 1) LN_RUN(8, 1) LN_RUN(16, 1) LN_RUN(32, 1) LN_RUN(64, 1) LN_RUN(64, 2) LN_RUN(64, 4) LN_RUN(64, 8)
   LN_RUN(256, 1) LN_RUN(256, 2) LN_RUN(256, 4) LN_RUN(256, 8)
 #undef LN_RUN
+#undef LN_END
   set_error("layer_norm_fwd: no kernel for C = %d", C);
   return kUnsupported;
 }
@@ -395,7 +410,7 @@ int bwd_blocks(int64_t rows, int C, int N) {
 template <typename T, typename W>
 int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, int64_t rows, int C, const void* w, void* dx,
            void* dw, void* db, float* part, hipStream_t st) {
-  constexpr int N = RowVec<T>::N;
+  constexpr int N = vec_len<T>();
   const T *xt = static_cast<const T*>(x), *dyt = static_cast<const T*>(dy);
   const W* wt = static_cast<const W*>(w);
   T* dxt = static_cast<T*>(dx);
@@ -416,16 +431,24 @@ int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, 
   const unsigned grid = bwd_blocks(rows, C, N);
   if (!params) part = nullptr;
   int rc = kUnsupported;
-#define LN_RUN(G_, NV_)                                                                                                 \
-  if constexpr (NV_ * N <= 16) {                                                                                        \
-    if (s.G == G_ && s.NV == NV_) {                                                                                     \
-      ln_bwd_kernel<T, W, G_, NV_><<<grid, G_ > kThreads ? G_ : kThreads, 0, st>>>(xt, mean, rstd, dyt, rows, C, wt, dxt, part); \
-      rc = check_launch("layer_norm_bwd");                                                                              \
-    }                                                                                                                   \
+#define LN_END(G_, NV_, END_)                                                                                            \
+  ln_bwd_kernel<T, W, G_, NV_, END_><<<grid, G_ > kThreads ? G_ : kThreads, 0, st>>>(xt, mean, rstd, dyt, rows, C, wt, dxt, part)
+#define LN_RUN(G_, NV_)                                                   \
+  if constexpr (NV_ * N <= 16) {                                          \
+    if (C >= N && s.G == G_ && s.NV == NV_) {                             \
+      if (C % N == 0) LN_END(G_, NV_, kExact);                            \
+      else LN_END(G_, NV_, kOverlap);                                     \
+      rc = check_launch("layer_norm_bwd");                                \
+    }                                                                     \
+  }
+  if (C < N) {
+    LN_END(4, 1, kTiny);
+    rc = check_launch("layer_norm_bwd");
   }
   LN_RUN(4, 1) LN_RUN(8, 1) LN_RUN(16, 1) LN_RUN(32, 1) LN_RUN(64, 1) LN_RUN(64, 2) LN_RUN(64, 4)
   LN_RUN(256, 1) LN_RUN(256, 2) LN_RUN(256, 4) LN_RUN(512, 16 / N)
 #undef LN_RUN
+#undef LN_END
   if (rc) return rc;
   if (params) {
     ln_param_reduce_kernel<W><<<ceil_div(2 * (int64_t)C, 32), 1024, 0, st>>>(part, (int)grid, C, dwt, dbt);
