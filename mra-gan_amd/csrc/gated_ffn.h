@@ -94,8 +94,11 @@ __global__ __launch_bounds__(256) void ffn_pack_kernel(const PackArgs a) {
     if (i >= total) break;
     const int64_t r = i / quads, k = (i - r * quads) * 4;
     float v[4];
-    if ((q.K & 3) == 0 && k < q.K) {
-      load_vec<T, 4>(src + r * q.K + k, v);
+    if (k + 4 <= q.K) {                                              // of any alignment where K is odd
+      T t[4];
+      __builtin_memcpy(t, src + r * q.K + k, sizeof(t));
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = (float)t[e];
     } else {
 #pragma unroll
       for (int e = 0; e < 4; e++) v[e] = k + e < q.K ? (float)src[r * q.K + k + e] : 0.f;
@@ -153,6 +156,28 @@ __global__ __launch_bounds__(64 * SLOTS) void ffn_reduce_kernel(const float* par
     if (bias) v += (float)bias[i % N];
     out[i] = (TO)v;
   }
+}
+
+// the same for few parts of many elements: four elements a thread (total and N multiples of 4)
+template <typename TO>
+__global__ __launch_bounds__(256) void ffn_reduce4_kernel(const float* part, int parts, int64_t total, int N, const TO* bias,
+                                                          TO* out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= total) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int p = 0; p < parts; p++) {
+    float t[4];
+    load_vec<float, 4>(part + p * total + i, t);
+#pragma unroll
+    for (int q = 0; q < 4; q++) v[q] += t[q];
+  }
+  if (bias) {
+    const int n = (int)(i % N);
+#pragma unroll
+    for (int q = 0; q < 4; q++) v[q] += (float)bias[n + q];
+  }
+  store_vec<TO, 4>(out + i, v);
 }
 
 // db of both projections from the column sums [rows][2][F] of the dg / du launch
@@ -950,9 +975,11 @@ struct Tiling {
   int bm, bn, tiles_m, tiles_n, splits, per_split;   // bn: columns of the output
 };
 // The largest of three tiles that still gives the 256 CUs a block each: 256×256, 128×128 (two blocks a
-// CU), 64×64 (kEpiGate: half as many columns of g and of u each, 64×64 with 64).  Where even the smallest gives
-// fewer blocks, a product whose partial sums may be stored splits k into runs of at least 4 stages, up
-// to about two blocks a CU.
+// CU), 64×64 (kEpiGate: half as many columns of g and of u each, 64×64 with 64).  A product of small
+// tiles whose partial sums may be stored splits k into runs of at least 4 stages: up to two blocks a CU
+// where there is not one, up to three for 64 stages and more, over which one block a CU waits longer than
+// the sums cost (fp32 8192 × 128 from 2 × 512, 96 stages: 37.8 us unsplit, 32 split; from 512, 48 stages:
+// 18.9 and 21).
 Tiling tile(int64_t M, int64_t N, int batches, int stages, bool gate, bool may_split) {
   Tiling t{};
   for (int b : {256, 128, 64}) {
@@ -962,8 +989,8 @@ Tiling tile(int64_t M, int64_t N, int batches, int stages, bool gate, bool may_s
   }
   t.splits = 1;
   const int64_t tiles = (int64_t)t.tiles_m * t.tiles_n * batches;
-  if (may_split && tiles < 224) {
-    int64_t s = 512 / tiles;
+  if (may_split && t.bm == 64 && (tiles < 224 || (stages >= 64 && tiles < 512))) {
+    int64_t s = (tiles < 224 ? 512 : 768) / tiles;
     if (s > stages / 4) s = stages / 4;
     const int64_t cap = (int64_t)(kPartialCap / ((size_t)M * N * batches * 4));
     if (s > cap) s = cap;
@@ -1074,6 +1101,10 @@ struct Ffn {
   int reduce(const float* part, int parts, int64_t total, int N, const void* bias, void* out) {
     const unsigned grid = (unsigned)((total + 63) / 64);
     const TO* b = static_cast<const TO*>(bias);
+    if (N % 4 == 0 && (parts <= 8 || total >= (1 << 18))) {
+      ffn_reduce4_kernel<TO><<<(unsigned)((total / 4 + 255) / 256), 256, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
+      return check_launch("ffn_reduce");
+    }
     if (parts > 8) ffn_reduce_kernel<TO, 16><<<grid, 1024, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
     else ffn_reduce_kernel<TO, 4><<<grid, 256, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
     return check_launch("ffn_reduce");

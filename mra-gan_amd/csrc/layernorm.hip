@@ -347,7 +347,9 @@ constexpr int kMaxBwdBlocks = 1024;
 
 // Lanes per row and 16-byte vectors per lane.  A wave or a part of one per row as long as `most`
 // channels a lane suffice, else the block.  Few rows (≤ 1024: fewer waves than the chip's SIMDs hold
-// one each of) of more than 64 vectors take a block each, so that more CUs share the loads.
+// one each of) of more than 64 vectors take a block each, so that more CUs share the loads.  The
+// backward holds half as many channels a lane (`most`): 8192 rows of 2048 bf16 channels take 27.7 us
+// with a block a row, 29.2 us with 32 channels a lane of a wave.
 struct Shape {
   int G, NV;
 };
