@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void ffn_pack_kernel(const PackArgs a) {
   for (int n = 0; n < kPackQuads / 256; n++) {
     const int64_t i = i0 + n * 256 + threadIdx.x;
     if (i >= total) break;
-    const int64_t r = i / quads, k = (i - r * quads) * 4;
+    const int64_t r = total >> 32 ? i / quads : (uint32_t)i / (uint32_t)quads, k = (i - r * quads) * 4;
     float v[4];
     if (k + 4 <= q.K) {                                              // of any alignment where K is odd
       T t[4];
