@@ -134,11 +134,12 @@ __global__ __launch_bounds__(256) void ffn_col_sum_kernel(const T* src, int64_t 
   if (wave == 0 && c < cols) part[(int64_t)blockIdx.y * cols + c] = s[0][lane] + s[1][lane] + s[2][lane] + s[3][lane];
 }
 
-// out[i] = Σ_s part[s][i] (+ bias[i mod N]): 64 elements a block, SLOTS threads each that take every
+// out[i] = Σ_s part[s][i] (+ bias[i mod N]), and of a second set of parts → out2: 64 elements a block, SLOTS threads each that take every
 // SLOTS-th part and join in order
 template <typename TO, int SLOTS>
 __global__ __launch_bounds__(64 * SLOTS) void ffn_reduce_kernel(const float* part, int parts, int64_t total, int N, const TO* bias,
-                                                                TO* out) {
+                                                                TO* out, TO* out2) {
+  if (blockIdx.y) part += parts * total, out = out2;
   __shared__ float s[SLOTS][64];
   const int lane = threadIdx.x & 63, slot = threadIdx.x >> 6;
   const int64_t i = (int64_t)blockIdx.x * 64 + lane;
@@ -161,7 +162,8 @@ __global__ __launch_bounds__(64 * SLOTS) void ffn_reduce_kernel(const float* par
 // the same for few parts of many elements: four elements a thread (total and N multiples of 4)
 template <typename TO>
 __global__ __launch_bounds__(256) void ffn_reduce4_kernel(const float* part, int parts, int64_t total, int N, const TO* bias,
-                                                          TO* out) {
+                                                          TO* out, TO* out2) {
+  if (blockIdx.y) part += parts * total, out = out2;
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= total) return;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -230,13 +232,14 @@ struct GemmArgs {
 
 // A wave's 64 × 16 bytes from a buffer straight into LDS at `lds` + 16·lane.  As assembly, with the
 // waits below: after the builtin the compiler waits for every such load before any transposed LDS
-// read, whichever stage it reads, and the loads of the next stages would never be in flight.
+// read, whichever stage it reads, and the loads of the next stages would never be in flight.  The
+// nops cover the wait states of a descriptor register that a vector instruction wrote (5) and of m0.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, unsigned lds, unsigned voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voffset), "s"(rsrc)
-               : "memory");
+               : "memory", "m0");
 }
 // all but the N newest of this wave's loads have landed, its LDS reads are done, and so for every wave
 template <int N>
@@ -398,9 +401,10 @@ __device__ __forceinline__ void store_planes8(H* base, unsigned lane, int64_t pl
 // chunks of a row, which spreads the fragment reads over the banks, is made on the global address.
 //   k contiguous:    [rows][8 chunks], chunk ^ swz(row).  A: row & 7, fragments read 16 successive
 //                    rows.  B: fragment rows are fours 8 apart (see `nrow`), so row & 3 and bit 3.
-//   rows contiguous: [64 k][ROWS / 8 chunks], chunk ^ (k & 3 | (k >> 3 & 3) << 2): the 16 k rows that
-//                    a wave's transposed reads touch land on 16 different chunks (64 rows, 8 chunks
-//                    an LDS row, two LDS rows over all banks: bits 1, 3 and 4 of k).
+//   rows contiguous: [64 k][ROWS / 8 chunks], chunk ^ swz_t(k).  A cycle serves 16 lanes of a transposed
+//                    read: four k rows (k & 3) of four 8-byte quads, in one chunk pair (A) or four
+//                    chunks (B); k & 3 moves them by four chunks, onto sixteen different ones.  With 64
+//                    rows two LDS rows span all banks: bit 0 of k is in the address, bit 1 moves.
 template <int ROWS, bool T>
 struct TileMap {
   static constexpr int kChunks = T ? ROWS / 8 : 8;               // per LDS row
@@ -408,7 +412,7 @@ struct TileMap {
 };
 template <int ROWS>
 __device__ __forceinline__ int swz_t(int k) {
-  return ROWS == 64 ? (k >> 1 & 1) | (k >> 2 & 6) : (k & 3) | ((k >> 3 & 3) << 2);
+  return ROWS == 64 ? (k >> 1 & 1) << 2 | (k >> 3 & 3) : (k & 3) << 2 | (k >> 3 & 3);
 }
 
 // One block: a BM×BN tile of D (kEpiGate: BM×BN/2 of g and of u), WM×WN waves of 16×16×32 MFMAs, k in
@@ -584,6 +588,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     for (int i = 0; i < NR; i++) read(0, 0, i, f0);
     auto both_steps = [&](auto more_c, auto load_c) {                // stages kt + 1, kt + NS follow
       constexpr bool more = decltype(more_c)::value, load = decltype(load_c)::value;
+      // each fragment's address is an exclusive or away: not to be kept in a register over the loop
+      if constexpr (TA) asm volatile("" : "+v"(atA), "+v"(atB));
 #pragma unroll
       for (int i = 0; i < FM; i++) {
 #pragma unroll
@@ -1091,22 +1097,20 @@ struct Ffn {
     if (int rc = check_launch(EPI == kEpiStore ? "ffn_gemm" : EPI == kEpiGate ? "ffn_gemm_gate" : "ffn_gemm_gate_bwd")) return rc;
     if (t.splits > 1) {
       const int64_t total = (int64_t)a.M * a.N;
-      for (int b = 0; b < a.batches; b++)
-        if (int rc = reduce(a.partial + b * t.splits * total, t.splits, total, a.N, a.bias, b ? a.out2 : a.out)) return rc;
+      return reduce(a.partial, t.splits, total, a.N, a.bias, a.out, a.batches == 2 ? a.out2 : nullptr);
     }
     return kOk;
   }
 
   // many parts of few elements: more threads an element
-  int reduce(const float* part, int parts, int64_t total, int N, const void* bias, void* out) {
-    const unsigned grid = (unsigned)((total + 63) / 64);
+  int reduce(const float* part, int parts, int64_t total, int N, const void* bias, void* out, void* out2 = nullptr) {
+    const dim3 grid((unsigned)((total + 63) / 64), out2 ? 2 : 1);
     const TO* b = static_cast<const TO*>(bias);
-    if (N % 4 == 0 && (parts <= 8 || total >= (1 << 18))) {
-      ffn_reduce4_kernel<TO><<<(unsigned)((total / 4 + 255) / 256), 256, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
-      return check_launch("ffn_reduce");
-    }
-    if (parts > 8) ffn_reduce_kernel<TO, 16><<<grid, 1024, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
-    else ffn_reduce_kernel<TO, 4><<<grid, 256, 0, st>>>(part, parts, total, N, b, static_cast<TO*>(out));
+    TO *o = static_cast<TO*>(out), *o2 = static_cast<TO*>(out2);
+    if (N % 4 == 0 && (parts <= 8 || total >= (1 << 18)))
+      ffn_reduce4_kernel<TO><<<dim3((unsigned)((total / 4 + 255) / 256), grid.y), 256, 0, st>>>(part, parts, total, N, b, o, o2);
+    else if (parts > 8) ffn_reduce_kernel<TO, 16><<<grid, 1024, 0, st>>>(part, parts, total, N, b, o, o2);
+    else ffn_reduce_kernel<TO, 4><<<grid, 256, 0, st>>>(part, parts, total, N, b, o, o2);
     return check_launch("ffn_reduce");
   }
 

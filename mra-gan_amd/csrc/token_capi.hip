@@ -9,7 +9,8 @@ using namespace mragan;
 
 namespace {
 constexpr int64_t kMaxGrid = (int64_t)1 << 31;
-constexpr int64_t kMaxSide = ((int64_t)1 << 23) - 64;     // rows of an FFN operand: 32-bit offsets inside a tile
+constexpr int64_t kMaxSide = ((int64_t)1 << 22) - 64;     // row length of an FFN operand: 256 rows below 2^31 bytes
+constexpr int64_t kMaxRows = (int64_t)1 << 30;
 
 bool all_aligned(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
@@ -55,7 +56,8 @@ int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, c
 
 static int ffn_shape(int64_t M, int C, int F, int O, int dtype, int act) {
   MRAGAN_CHECK_ARG(M >= 0 && C > 0 && F > 0 && O > 0, "gated_ffn: bad shape M %lld, C %d, F %d, O %d", (long long)M, C, F, O);
-  MRAGAN_CHECK_ARG(M <= kMaxSide && C <= kMaxSide && F <= kMaxSide && O <= kMaxSide, "gated_ffn: a side above 2^23 - 64");
+  MRAGAN_CHECK_ARG(M <= kMaxRows && C <= kMaxSide && F <= kMaxSide && O <= kMaxSide,
+                   "gated_ffn: more than 2^30 rows, or C, F, O: a side above 2^22 - 64");
   MRAGAN_CHECK_ARG(dtype_ok(dtype), "gated_ffn: unknown dtype %d", dtype);
   MRAGAN_CHECK_ARG(act >= MRAGAN_ACT_NONE && act <= MRAGAN_ACT_GELU, "gated_ffn: unknown activation %d", act);
   return kOk;

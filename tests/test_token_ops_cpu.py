@@ -54,11 +54,14 @@ P = 1 << 20      # an aligned address that is never dereferenced: each call belo
     ("dtype", "mragan_gated_ffn_fwd", (P, 4, 8, 8, 8, -1, P, P, P, None, None, None, 5, P, None, P, 1 << 40, None)),
     ("aligned", "mragan_gated_ffn_fwd", (P + 8, 4, 8, 8, 8, 0, P, P, P, None, None, None, 5, P, None, P, 1 << 40, None)),
     ("workspace", "mragan_gated_ffn_fwd", (P, 4, 8, 8, 8, 0, P, P, P, None, None, None, 5, P, None, P, 64, None)),
-    ("side above", "mragan_gated_ffn_fwd", (P, 4, 1 << 23, 8, 8, 0, P, P, P, None, None, None, 5, P, None, P, 1 << 40, None)),
+    ("side above", "mragan_gated_ffn_fwd", (P, (1 << 30) + 1, 8, 8, 8, 0, P, P, P, None, None, None, 5, P, None, P, 1 << 60, None)),
+    ("side above", "mragan_gated_ffn_fwd", (P, 4, 1 << 22, 8, 8, 0, P, P, P, None, None, None, 5, P, None, P, 1 << 40, None)),
     ("no rows", "mragan_gated_ffn_bwd", (P, 0, 8, 8, 8, 0, P, P, P, None, None, 5, P, None) + (P,) * 7 + (P, 1 << 40, None)),
     ("workspace", "mragan_gated_ffn_bwd", (P, 4, 8, 8, 8, 0, P, P, P, None, None, 5, P, None) + (P,) * 7 + (P, 64, None)),
     ("bad shape", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1, 0, 8, 0, 0, P, P, P, None, 0, None)),
     ("reverse", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1, 4, 8, 0, 2, P, P, P, None, 0, None)),
+    ("time strides", "mragan_linear_recurrence_fwd", (P, 8, 1 << 22, P, 8, 8, None, 0, 0, None, 1, 4, 8, 0, 0, P, P, P, None, 0, None)),
+    ("time strides", "mragan_linear_recurrence_fwd", (P, 8, -8, P, 8, 8, None, 0, 0, None, 1, 4, 8, 0, 0, P, P, P, None, 0, None)),
     ("null pointer", "mragan_linear_recurrence_fwd", (P, 8, 8, None, 8, 8, None, 0, 0, None, 1, 4, 8, 0, 0, P, P, P, None, 0, None)),
     ("null pointer", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1, 4, 8, 0, 0, P, None, P, None, 0, None)),
     ("too many", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1 << 40, 4, 8, 0, 0, P, P, P, None, 0, None)),
