@@ -779,23 +779,27 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
 // between the two launches and enters the second as two planes (16-bit tensors).
 constexpr int kSkinnyRows = 64;
 
-// eight elements from k as the fragments of P planes; zeros at and behind K (a multiple of eight)
-template <typename H, typename T, int P>
-__device__ __forceinline__ void load_frags(const T* row, int64_t k, int64_t K, bf16x8 (&out)[P]) {
-  if constexpr (sizeof(T) == 2 && P == 1) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (k < K) v = *reinterpret_cast<const uint4*>(row + k);
-    out[0] = __builtin_bit_cast(bf16x8, v);
-  } else {
-    float v[8];
+// eight elements from k < K (K a multiple of eight); behind K zeros, by a load of the row's start and a
+// selection: a branch around each load would wait for one before the next
+template <typename T>
+__device__ __forceinline__ Words<T, 8> load_words8(const T* row, int64_t k, int64_t K) {
+  Words<T, 8> r;
+  __builtin_memcpy(&r, row + (k < K ? k : 0), sizeof(r));
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = 0.f;
-    if (k < K) load_vec<T, 8>(row + k, v);
+  for (int i = 0; i < (int)(sizeof(r) / 4); i++) r.w[i] = k < K ? r.w[i] : 0u;
+  return r;
+}
+// the same as the fragments of P planes
+template <typename H, typename T, int P>
+__device__ __forceinline__ void split_frags(const Words<T, 8>& r, bf16x8 (&out)[P]) {
+  if constexpr (sizeof(T) == 2 && P == 1) {
+    out[0] = __builtin_bit_cast(bf16x8, r);
+  } else {
     Pack<H, 8> w[3];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       H e[3];
-      split_planes<H>(v[i], P, e);
+      split_planes<H>(r.get(i), P, e);
 #pragma unroll
       for (int p = 0; p < 3; p++) w[p].v[i] = e[p];
     }
@@ -814,12 +818,6 @@ __device__ __forceinline__ float gate_act(float g, int act) {
 // every CU takes part in reading the weight (the MFMA form below gives N / 16 blocks).  Lanes walk the
 // column's weight row 16 bytes at a time.  1 row, 4096 → 1024 bf16: 6.6 us against 9.0.
 constexpr int kDotRows = 2, kDotCols = 4096;
-template <typename T>
-__device__ __forceinline__ Words<T, 8> load_words8(const T* row, int64_t k, int64_t K) {   // K a multiple of 8
-  Words<T, 8> r{};
-  if (k < K) r = *reinterpret_cast<const Words<T, 8>*>(row + k);
-  return r;
-}
 // round: the operand rounding of the one-plane modes of fp32 tensors (op_round)
 template <typename TX, typename TO, int NB, int MR>
 __global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_t K, const TO* w0, const TO* w1, const TO* b0,
@@ -888,26 +886,34 @@ __global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TX* x, int
     for (int m = 0; m < MF; m++) acc[b][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int64_t steps = (K + 31) / 32, per = (steps + WAVES - 1) / WAVES, s1 = (wave + 1) * per < steps ? (wave + 1) * per : steps;
   for (int64_t s = wave * per; s < s1; s += U) {
-    bf16x8 fw[U][NB][PW], fx[U][MF][PX];
+    Words<TO, 8> qw[U][NB];
+    Words<TX, 8> qx[U][MF];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int64_t k = (s + u) * 32 + fk * 8, end = s + u < s1 ? K : 0;
 #pragma unroll
-      for (int b = 0; b < NB; b++) load_frags<H, TO, PW>(w[b], k, end, fw[u][b]);
+      for (int b = 0; b < NB; b++) qw[u][b] = load_words8(w[b], k, end);
 #pragma unroll
-      for (int m = 0; m < MF; m++) load_frags<H, TX, PX>(x + (int64_t)(m * 16 + fr < M ? m * 16 + fr : M - 1) * K, k, end, fx[u][m]);
+      for (int m = 0; m < MF; m++) qx[u][m] = load_words8(x + (int64_t)(m * 16 + fr < M ? m * 16 + fr : M - 1) * K, k, end);
     }
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int u = 0; u < U; u++) {
+      bf16x8 fw[NB][PW];
 #pragma unroll
-      for (int b = 0; b < NB; b++)
+      for (int b = 0; b < NB; b++) split_frags<H>(qw[u][b], fw[b]);
 #pragma unroll
-        for (int m = 0; m < MF; m++)
+      for (int m = 0; m < MF; m++) {
+        bf16x8 fx[PX];
+        split_frags<H>(qx[u][m], fx);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
 #pragma unroll
           for (int o = kOrder - 1; o >= 0; o--)
 #pragma unroll
             for (int i = 0; i < PX; i++)
-              if (o - i >= 0 && o - i < PW) acc[b][m] = mfma16<H>(fw[u][b][o - i < 0 || o - i >= PW ? 0 : o - i], fx[u][m][i], acc[b][m]);
+              if (o - i >= 0 && o - i < PW) acc[b][m] = mfma16<H>(fw[b][o - i < 0 || o - i >= PW ? 0 : o - i], fx[i], acc[b][m]);
+      }
+    }
   }
 #pragma unroll
   for (int b = 0; b < NB; b++)

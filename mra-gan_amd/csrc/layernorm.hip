@@ -16,6 +16,9 @@
 namespace mragan {
 namespace {
 
+#ifndef LN_MIN
+#define LN_MIN 8
+#endif
 constexpr int kThreads = 256;
 
 // A lane's 16 bytes of a row.  Rows of any channel count start at any element; gfx950 takes global
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* part
 }
 
 // Rows of more channels than the registers of a block hold (C > kMaxRow): the block walks the row
-// in memory, once per sum; the parameter gradients take a column per thread over all rows.
+// in memory, once per sum; the parameter gradients take a column per thread over a run of rows.
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* x, int C, const W* w, const W* b, float eps, T* y,
                                                            float* mean, float* rstd) {
@@ -324,19 +327,23 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* x, const flo
     dx[row * C + c] = (T)(r * (p - m1 - xh * m2));
   }
 }
-template <typename T, typename W>
+// part: [gridDim.y][2][C], rows dealt to gridDim.y in runs of `per`
+template <typename T>
 __global__ __launch_bounds__(256) void ln_param_long_kernel(const T* x, const float* mean, const float* rstd, const T* dy,
-                                                            int64_t rows, int C, W* dw, W* db) {
+                                                            int64_t rows, int64_t per, int C, float* part) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= C) return;
+  const int64_t k0 = blockIdx.y * per, k1 = k0 + per < rows ? k0 + per : rows;
   float sw = 0.f, sb = 0.f;
-  for (int64_t k = 0; k < rows; k++) {
+#pragma unroll 8
+  for (int64_t k = k0; k < k1; k++) {
     const float d = (float)dy[k * C + c];
     sw += d * (((float)x[k * C + c] - mean[k]) * rstd[k]);
     sb += d;
   }
-  if (dw) dw[c] = (W)sw;
-  if (db) db[c] = (W)sb;
+  float* out = part + (int64_t)blockIdx.y * 2 * C;
+  out[c] = sw;
+  out[C + c] = sb;
 }
 
 // The largest row that a block holds: 16 channels a thread of 512 (backward: their 256 registers also
@@ -346,19 +353,17 @@ constexpr int kMaxRow = 8192;
 constexpr int kMaxBwdBlocks = 1024;
 
 // Lanes per row and 16-byte vectors per lane.  A wave or a part of one per row as long as `most`
-// channels a lane suffice, else the block.  Few rows (≤ 1024: fewer waves than the chip's SIMDs hold
-// one each of) of more than 64 vectors take a block each, so that more CUs share the loads.  The
-// backward holds half as many channels a lane (`most`): 8192 rows of 2048 bf16 channels take 27.7 us
-// with a block a row, 29.2 us with 32 channels a lane of a wave.
+// channels a lane suffice, else the block.  Rows of more than 64 vectors take a block each where there
+// are no more than `few`, so that more CUs share the loads.
 struct Shape {
   int G, NV;
 };
-Shape pick(int64_t rows, int C, int N, int most) {
+Shape pick(int64_t rows, int C, int N, int most, int few) {
   const int V = ceil_div(C, N);
   for (int g = 4; g <= 64; g *= 2)
     if (V <= g) return {g, 1};
   for (int g : {64, 256}) {
-    if (g == 64 && rows <= 1024) continue;
+    if (g == 64 && rows <= few) continue;
     for (int nv = 1; nv * N <= most; nv *= 2)
       if (V <= g * nv) return {g, nv};
   }
@@ -376,7 +381,9 @@ int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, flo
     ln_fwd_long_kernel<T, W><<<(unsigned)rows, 1024, 0, st>>>(xt, C, wt, bt, eps, yt, mean, rstd);
     return check_launch("layer_norm_fwd_long");
   }
-  const Shape s = pick(rows, C, N, 32);
+  // bf16, 2048 channels: 64 rows take 2.6 us with a block each, 3.3 with a wave; 1024 channels: 256 rows
+  // 2.5 and 2.7, 1024 rows 3.3 and 3.0
+  const Shape s = pick(rows, C, N, 32, 512);
   const int64_t per = kThreads / s.G, blocks = (rows + per - 1) / per, most = 2048;
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
 #define LN_END(G_, NV_, END_)                                                                                            \
@@ -401,13 +408,21 @@ int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, flo
   return kUnsupported;
 }
 
-Shape bwd_shape(int64_t rows, int C, int N) { return pick(rows, C, N, 16); }
+// Half the forward's channels a lane: 8192 rows of 2048 bf16 channels take 27.7 us with a block a row,
+// 29.2 with 32 channels a lane of a wave.  No block a row for few rows: each block's sums are as long as
+// a row, and 1024 rows of 1024 channels take 14.5 us with 1024 such blocks, 7.3 with a wave a row.
+Shape bwd_shape(int C, int N) { return pick(0, C, N, 16, -1); }
+// As many blocks as the chip holds, but at least LN_MIN row groups each where that leaves one for every CU.
 int bwd_blocks(int64_t rows, int C, int N) {
-  const Shape s = bwd_shape(rows, C, N);
+  const Shape s = bwd_shape(C, N);
   const int per = s.G > kThreads ? 1 : kThreads / s.G;
-  const int64_t blocks = (rows + per - 1) / per, most = s.G > kThreads ? kMaxBwdBlocks / 2 : kMaxBwdBlocks;
+  const int64_t groups = (rows + per - 1) / per, most = s.G > kThreads ? kMaxBwdBlocks / 2 : kMaxBwdBlocks;
+  const int64_t few = groups < 256 ? groups : 256, blocks = groups / LN_MIN > few ? groups / LN_MIN : few;
   return (int)(blocks < most ? blocks : most);
 }
+
+// row runs of the long rows' parameter sums, 64 rows each up to 64 runs
+int long_chunks(int64_t rows) { return rows > 64 * 64 ? 64 : (int)((rows + 63) / 64); }
 
 template <typename T, typename W>
 int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, int64_t rows, int C, const void* w, void* dx,
@@ -423,13 +438,15 @@ int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, 
       ln_bwd_long_kernel<T, W><<<(unsigned)rows, 1024, 0, st>>>(xt, mean, rstd, dyt, C, wt, dxt);
       if (int rc = check_launch("layer_norm_bwd_long")) return rc;
     }
-    if (params) {
-      ln_param_long_kernel<T, W><<<ceil_div(C, 256), 256, 0, st>>>(xt, mean, rstd, dyt, rows, C, dwt, dbt);
-      return check_launch("layer_norm_param_long");
-    }
-    return kOk;
+    if (!params) return kOk;
+    const int chunks = long_chunks(rows);
+    ln_param_long_kernel<T><<<dim3(ceil_div(C, 256), chunks), 256, 0, st>>>(xt, mean, rstd, dyt, rows, (rows + chunks - 1) / chunks, C,
+                                                                            part);
+    if (int rc = check_launch("layer_norm_param_long")) return rc;
+    ln_param_reduce_kernel<W><<<ceil_div(2 * (int64_t)C, 32), 1024, 0, st>>>(part, chunks, C, dwt, dbt);
+    return check_launch("layer_norm_param_reduce");
   }
-  const Shape s = bwd_shape(rows, C, N);
+  const Shape s = bwd_shape(C, N);
   const unsigned grid = bwd_blocks(rows, C, N);
   if (!params) part = nullptr;
   int rc = kUnsupported;
@@ -470,8 +487,8 @@ __global__ void ln_zero_kernel(W* dw, W* db, int C) {
 }  // namespace
 
 size_t layer_norm_bwd_ws_bytes(int64_t rows, int C, int dtype) {
-  if (C > kMaxRow || rows == 0) return 0;
-  return (size_t)bwd_blocks(rows, C, dtype == kF32 ? 4 : 8) * 2 * C * sizeof(float);
+  if (rows == 0) return 0;
+  return (size_t)(C > kMaxRow ? long_chunks(rows) : bwd_blocks(rows, C, dtype == kF32 ? 4 : 8)) * 2 * C * sizeof(float);
 }
 
 int layer_norm_fwd(const void* x, int64_t rows, int C, int dtype, const void* w, const void* b, int wdtype, float eps, void* y,
