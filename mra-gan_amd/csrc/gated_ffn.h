@@ -775,9 +775,14 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
 // ---- few rows ---------------------------------------------------------------------------------
 // Up to kSkinnyRows rows in inference: the time is that of reading the weights once, so nothing is
 // staged.  A block takes 16 rows of a weight, its waves split k; a lane loads 16 bytes of a weight row
-// and of each 16 rows of x straight into MFMA fragments, the waves' sums meet in LDS.  h stays in fp32
-// between the two launches and enters the second as two planes (16-bit tensors).
-constexpr int kSkinnyRows = 64;
+// and of each 16 rows of x straight into MFMA fragments, the waves' sums meet in LDS.  h is rounded to the
+// tensors' type between the two launches, as the products of more rows take it.
+// The larger products instead read x once for 128 columns of a block, not once for 16, but have fewer
+// blocks and a chain of C / 64 stages each: their time over this form's falls as M·F grows, and they take
+// 16-bit tensors from kSkinnyArea on (bf16: 16 rows, C = 1024, F = 4096 15.4 us here and 17.4 there, F =
+// 8192, C = 2048 31.6 and 30.1; 64 rows, F = 1024, C = 4096 31.9 and 44.9, F = 2048, C = 512 17.7 and 14.2).
+// fp32 weights would have to be split into planes in memory first (64 rows, 2048 → 8192: 122 us and 243).
+constexpr int kSkinnyRows = 64, kSkinnyArea = 65536;
 
 // eight elements from k < K (K a multiple of eight); behind K zeros, by a load of the row's start and a
 // selection: a branch around each load would wait for one before the next
@@ -814,14 +819,16 @@ __device__ __forceinline__ float gate_act(float g, int act) {
   return f;
 }
 
-// Up to kDotRows rows of fewer than kDotCols columns: a wave per column and plain fp32 products, so that
-// every CU takes part in reading the weight (the MFMA form below gives N / 16 blocks).  Lanes walk the
-// column's weight row 16 bytes at a time.  1 row, 4096 → 1024 bf16: 6.6 us against 9.0.
-constexpr int kDotRows = 2, kDotCols = 4096;
-// round: the operand rounding of the one-plane modes of fp32 tensors (op_round)
-template <typename TX, typename TO, int NB, int MR>
-__global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_t K, const TO* w0, const TO* w1, const TO* b0,
-                                                      const TO* b1, int N, int act, int round, void* out) {
+// Up to kDotRows rows: a wave per column and plain fp32 products, so that every CU takes part in reading
+// the weight (the MFMA form below gives N / 16 blocks).  Lanes walk the column's weight row 16 bytes at a
+// time.  bf16, 1024 → 4096 → 1024: 6.6 us with one row and 10.4 with four, against 11.8 and 12.8;
+// 2048 → 8192 → 2048, 100 MB of weights: 18.5 us, 5.4 TB/s.
+constexpr int kDotRows = 4;
+// ROUND: operands rounded to H, as the one-plane modes of fp32 tensors have them
+template <typename H, typename TO, int NB, int MR, bool ROUND>
+__global__ __launch_bounds__(256) void ffn_dot_kernel(const TO* x, int M, int64_t K, const TO* w0, const TO* w1, const TO* b0,
+                                                      const TO* b1, int N, int act, TO* out) {
+  auto in = [](float v) { return ROUND ? (float)(H)v : v; };
   constexpr int U = 8 / NB / MR;                                   // loads of a weight row in flight
   const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= N) return;
@@ -833,7 +840,7 @@ __global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_
     for (int m = 0; m < MR; m++) acc[b][m] = 0.f;
   for (int64_t k0 = lane * 8; k0 < K; k0 += 512 * U) {
     Words<TO, 8> wv[U][NB];
-    Words<TX, 8> xv[U][MR];
+    Words<TO, 8> xv[U][MR];
 #pragma unroll
     for (int u = 0; u < U; u++) {
 #pragma unroll
@@ -848,7 +855,7 @@ __global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-          for (int i = 0; i < 8; i++) acc[b][m] += op_round(xv[u][m].get(i), round) * op_round(wv[u][b].get(i), round);
+          for (int i = 0; i < 8; i++) acc[b][m] += in(xv[u][m].get(i)) * in(wv[u][b].get(i));
   }
 #pragma unroll
   for (int m = 0; m < MR; m++) {
@@ -857,23 +864,18 @@ __global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_
     for (int b = 0; b < NB; b++) v[b] = group_sum<64>(acc[b][m]);
     if (lane == 0 && m < M) {
       float r = v[0] + (b0 ? (float)b0[n] : 0.f);
-      if constexpr (NB == 2) {
-        r = gate_act(r, act) * (v[1] + (b1 ? (float)b1[n] : 0.f));
-        static_cast<float*>(out)[(int64_t)m * N + n] = r;
-      } else {
-        static_cast<TO*>(out)[(int64_t)m * N + n] = (TO)r;
-      }
+      if constexpr (NB == 2) r = gate_act(r, act) * (v[1] + (b1 ? (float)b1[n] : 0.f));
+      out[(int64_t)m * N + n] = (TO)r;
     }
   }
 }
 
-// NB weights (gate and up, or down alone) times x [M][K] (TX): PX planes of x, PW of the weights.
-// out: h [M][N] in fp32 (NB = 2) or y [M][N]
-template <typename H, typename TX, typename TO, int NB, int MF, int PX, int PW, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TX* x, int M, int64_t K, const TO* w0, const TO* w1,
-                                                                const TO* b0, const TO* b1, int N, int act, void* out) {
-  constexpr int kOrder = PX > PW ? PX : PW, kFrags = MF * PX + NB * PW;
-  constexpr int U = kFrags <= 4 ? 4 : kFrags <= 8 ? 2 : 1;            // k steps whose loads are in flight
+// NB weights (gate and up, or down alone) times x [M][K], both as P planes: h = act(g)·u (NB = 2) or y
+template <typename H, typename TO, int NB, int MF, int P, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TO* x, int M, int64_t K, const TO* w0, const TO* w1,
+                                                                const TO* b0, const TO* b1, int N, int act, TO* out) {
+  constexpr int kLoads = (NB + MF) * (int)sizeof(TO) / 2;             // 16-byte loads a k step
+  constexpr int U = kLoads <= 4 ? 4 : kLoads <= 8 ? 2 : 1;            // k steps whose loads are in flight
   __shared__ f32x4 part[WAVES][NB * MF][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fk = lane >> 4;
   const int n0 = blockIdx.x * 16;
@@ -887,7 +889,7 @@ __global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TX* x, int
   const int64_t steps = (K + 31) / 32, per = (steps + WAVES - 1) / WAVES, s1 = (wave + 1) * per < steps ? (wave + 1) * per : steps;
   for (int64_t s = wave * per; s < s1; s += U) {
     Words<TO, 8> qw[U][NB];
-    Words<TX, 8> qx[U][MF];
+    Words<TO, 8> qx[U][MF];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int64_t k = (s + u) * 32 + fk * 8, end = s + u < s1 ? K : 0;
@@ -898,20 +900,19 @@ __global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TX* x, int
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      bf16x8 fw[NB][PW];
+      bf16x8 fw[NB][P];
 #pragma unroll
       for (int b = 0; b < NB; b++) split_frags<H>(qw[u][b], fw[b]);
 #pragma unroll
       for (int m = 0; m < MF; m++) {
-        bf16x8 fx[PX];
+        bf16x8 fx[P];
         split_frags<H>(qx[u][m], fx);
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-          for (int o = kOrder - 1; o >= 0; o--)
+          for (int o = P - 1; o >= 0; o--)                           // the small products first
 #pragma unroll
-            for (int i = 0; i < PX; i++)
-              if (o - i >= 0 && o - i < PW) acc[b][m] = mfma16<H>(fw[b][o - i < 0 || o - i >= PW ? 0 : o - i], fx[i], acc[b][m]);
+            for (int i = 0; i <= o; i++) acc[b][m] = mfma16<H>(fw[b][o - i], fx[i], acc[b][m]);
       }
     }
   }
@@ -935,12 +936,8 @@ __global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TX* x, int
       const int n = n0 + fk * 4 + q;
       if (n < N) {
         float r = v[0][q] + (b0 ? (float)b0[n] : 0.f);
-        if constexpr (NB == 2) {
-          r = gate_act(r, act) * (v[1][q] + (b1 ? (float)b1[n] : 0.f));
-          static_cast<float*>(out)[(int64_t)m * N + n] = r;
-        } else {
-          static_cast<TO*>(out)[(int64_t)m * N + n] = (TO)r;
-        }
+        if constexpr (NB == 2) r = gate_act(r, act) * (v[1][q] + (b1 ? (float)b1[n] : 0.f));
+        out[(int64_t)m * N + n] = (TO)r;
       }
     }
   }
@@ -1142,35 +1139,38 @@ struct Ffn {
     return gemm<kEpiGate, false, false>(a, tile(f.M, f.F, 1, a.pairs * a.ktiles, true, false), nullptr);
   }
 
-  // One launch for few rows, x [M][K]: NB = 2 gate, up → h in fp32; NB = 1 down → y.  PX, PW: planes of x, w.
-  template <int NB, int PX, int PW, typename TX>
-  int skinny(const TX* x, int64_t K, const void* w0, const void* w1, const void* b0, const void* b1, int N, void* out) {
-    const TO *v0 = static_cast<const TO*>(w0), *v1 = static_cast<const TO*>(w1), *c0 = static_cast<const TO*>(b0),
-             *c1 = static_cast<const TO*>(b1);
+  // One launch for few rows, x [M][K]: NB = 2 gate, up → h; NB = 1 down → y.  P: planes of the operands.
+  template <int NB, int P>
+  int skinny(const void* x, int64_t K, const void* w0, const void* w1, const void* b0, const void* b1, int N, void* out) {
+    const TO *xt = static_cast<const TO*>(x), *v0 = static_cast<const TO*>(w0), *v1 = static_cast<const TO*>(w1),
+             *c0 = static_cast<const TO*>(b0), *c1 = static_cast<const TO*>(b1);
+    TO* o = static_cast<TO*>(out);
     const int M = (int)f.M;
-    if (M <= kDotRows && N < kDotCols) {
-      const int round = mode.pack && planes == 1 ? (__is_same(H, _Float16) ? kPrecF16 : kPrecBf16) : 0;
+    if (M <= kDotRows) {
+      constexpr bool R = sizeof(TO) == 4 && P == 1;
       const unsigned grid = (unsigned)ceil_div(N, 4);
-      if (M == 1) ffn_dot_kernel<TX, TO, NB, 1><<<grid, 256, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, round, out);
-      else ffn_dot_kernel<TX, TO, NB, 2><<<grid, 256, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, round, out);
+      if (M == 1) ffn_dot_kernel<H, TO, NB, 1, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
+      else if (M == 2) ffn_dot_kernel<H, TO, NB, 2, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
+      else ffn_dot_kernel<H, TO, NB, 4, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
       return check_launch("ffn_dot");
     }
     constexpr int W = 8;
     const unsigned grid = (unsigned)ceil_div(N, 16);
-    if (M <= 16) ffn_skinny_kernel<H, TX, TO, NB, 1, PX, PW, W><<<grid, 64 * W, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, out);
-    else if (M <= 32) ffn_skinny_kernel<H, TX, TO, NB, 2, PX, PW, W><<<grid, 64 * W, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, out);
-    else ffn_skinny_kernel<H, TX, TO, NB, 4, PX, PW, W><<<grid, 64 * W, 0, st>>>(x, M, K, v0, v1, c0, c1, N, f.act, out);
+    if (M <= 16) ffn_skinny_kernel<H, TO, NB, 1, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
+    else if (M <= 32) ffn_skinny_kernel<H, TO, NB, 2, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
+    else ffn_skinny_kernel<H, TO, NB, 4, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
     return check_launch("ffn_skinny");
   }
   template <int P>
-  int few_rows(void* y, float* h) {
-    if (int rc = skinny<2, P, P, TO>(static_cast<const TO*>(f.x), f.C, f.wg, f.wu, f.bg, f.bu, f.F, h)) return rc;
-    return skinny<1, sizeof(TO) == 2 ? 2 : P, P, float>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, y);
+  int few_rows(void* y, void* h) {
+    if (int rc = skinny<2, P>(f.x, f.C, f.wg, f.wu, f.bg, f.bu, f.F, h)) return rc;
+    return skinny<1, P>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, y);
   }
 
   int forward(void* y, void* kept) {
-    if (!kept && f.M <= kSkinnyRows && f.C % 8 == 0 && f.F % 8 == 0) {
-      float* h = static_cast<float*>(ws.take((size_t)f.M * f.F * sizeof(float)));
+    const bool area = sizeof(TO) == 4 || f.M * f.F <= kSkinnyArea || f.M <= kDotRows;
+    if (!kept && f.M <= kSkinnyRows && area && f.C % 8 == 0 && f.F % 8 == 0) {
+      void* h = ws.take((size_t)f.M * f.F * sizeof(TO));
       if (dry) return kOk;
       if constexpr (sizeof(TO) == 2) return few_rows<1>(y, h);
       else return planes == 3 ? few_rows<3>(y, h) : planes == 2 ? few_rows<2>(y, h) : few_rows<1>(y, h);
