@@ -776,7 +776,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
 // Up to kSkinnyRows rows in inference: the time is that of reading the weights once, so nothing is
 // staged.  A block takes 16 rows of a weight, its waves split k; a lane loads 16 bytes of a weight row
 // and of each 16 rows of x straight into MFMA fragments, the waves' sums meet in LDS.  h is rounded to the
-// tensors' type between the two launches, as the products of more rows take it.
+// tensors' type between the two launches, as the products of more rows take it (16 bits: the second launch
+// reads it once per 16 columns; two planes of it took 39 us instead of 31.6 for 16 rows, 2048 → 8192 → 2048).
 // The larger products instead read x once for 128 columns of a block, not once for 16, but have fewer
 // blocks and a chain of C / 64 stages each: their time over this form's falls as M·F grows, and they take
 // 16-bit tensors from kSkinnyArea on (bf16: 16 rows, C = 1024, F = 4096 15.4 us here and 17.4 there, F =
@@ -824,10 +825,11 @@ __device__ __forceinline__ float gate_act(float g, int act) {
 // time.  bf16, 1024 → 4096 → 1024: 6.6 us with one row and 10.4 with four, against 11.8 and 12.8;
 // 2048 → 8192 → 2048, 100 MB of weights: 18.5 us, 5.4 TB/s.
 constexpr int kDotRows = 4;
+// h stays in fp32 between the two launches (TX, TY: the types of x and of the result).
 // ROUND: operands rounded to H, as the one-plane modes of fp32 tensors have them
-template <typename H, typename TO, int NB, int MR, bool ROUND>
-__global__ __launch_bounds__(256) void ffn_dot_kernel(const TO* x, int M, int64_t K, const TO* w0, const TO* w1, const TO* b0,
-                                                      const TO* b1, int N, int act, TO* out) {
+template <typename H, typename TX, typename TO, typename TY, int NB, int MR, bool ROUND>
+__global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_t K, const TO* w0, const TO* w1, const TO* b0,
+                                                      const TO* b1, int N, int act, TY* out) {
   auto in = [](float v) { return ROUND ? (float)(H)v : v; };
   constexpr int U = 8 / NB / MR;                                   // loads of a weight row in flight
   const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -840,7 +842,7 @@ __global__ __launch_bounds__(256) void ffn_dot_kernel(const TO* x, int M, int64_
     for (int m = 0; m < MR; m++) acc[b][m] = 0.f;
   for (int64_t k0 = lane * 8; k0 < K; k0 += 512 * U) {
     Words<TO, 8> wv[U][NB];
-    Words<TO, 8> xv[U][MR];
+    Words<TX, 8> xv[U][MR];
 #pragma unroll
     for (int u = 0; u < U; u++) {
 #pragma unroll
@@ -865,7 +867,7 @@ __global__ __launch_bounds__(256) void ffn_dot_kernel(const TO* x, int M, int64_
     if (lane == 0 && m < M) {
       float r = v[0] + (b0 ? (float)b0[n] : 0.f);
       if constexpr (NB == 2) r = gate_act(r, act) * (v[1] + (b1 ? (float)b1[n] : 0.f));
-      out[(int64_t)m * N + n] = (TO)r;
+      out[(int64_t)m * N + n] = (TY)r;
     }
   }
 }
@@ -1146,14 +1148,6 @@ struct Ffn {
              *c0 = static_cast<const TO*>(b0), *c1 = static_cast<const TO*>(b1);
     TO* o = static_cast<TO*>(out);
     const int M = (int)f.M;
-    if (M <= kDotRows) {
-      constexpr bool R = sizeof(TO) == 4 && P == 1;
-      const unsigned grid = (unsigned)ceil_div(N, 4);
-      if (M == 1) ffn_dot_kernel<H, TO, NB, 1, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
-      else if (M == 2) ffn_dot_kernel<H, TO, NB, 2, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
-      else ffn_dot_kernel<H, TO, NB, 4, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
-      return check_launch("ffn_dot");
-    }
     constexpr int W = 8;
     const unsigned grid = (unsigned)ceil_div(N, 16);
     if (M <= 16) ffn_skinny_kernel<H, TO, NB, 1, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
@@ -1161,8 +1155,25 @@ struct Ffn {
     else ffn_skinny_kernel<H, TO, NB, 4, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
     return check_launch("ffn_skinny");
   }
+  template <int NB, int P, typename TX, typename TY>
+  int dot(const void* x, int64_t K, const void* w0, const void* w1, const void* b0, const void* b1, int N, TY* out) {
+    constexpr bool R = sizeof(TO) == 4 && P == 1;
+    const TX* xt = static_cast<const TX*>(x);
+    const TO *v0 = static_cast<const TO*>(w0), *v1 = static_cast<const TO*>(w1), *c0 = static_cast<const TO*>(b0),
+             *c1 = static_cast<const TO*>(b1);
+    const int M = (int)f.M;
+    const unsigned grid = (unsigned)ceil_div(N, 4);
+    if (M == 1) ffn_dot_kernel<H, TX, TO, TY, NB, 1, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
+    else if (M == 2) ffn_dot_kernel<H, TX, TO, TY, NB, 2, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
+    else ffn_dot_kernel<H, TX, TO, TY, NB, 4, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
+    return check_launch("ffn_dot");
+  }
   template <int P>
   int few_rows(void* y, void* h) {
+    if (f.M <= kDotRows) {
+      if (int rc = dot<2, P, TO>(f.x, f.C, f.wg, f.wu, f.bg, f.bu, f.F, static_cast<float*>(h))) return rc;
+      return dot<1, P, float>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, static_cast<TO*>(y));
+    }
     if (int rc = skinny<2, P>(f.x, f.C, f.wg, f.wu, f.bg, f.bu, f.F, h)) return rc;
     return skinny<1, P>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, y);
   }
@@ -1170,7 +1181,7 @@ struct Ffn {
   int forward(void* y, void* kept) {
     const bool area = sizeof(TO) == 4 || f.M * f.F <= kSkinnyArea || f.M <= kDotRows;
     if (!kept && f.M <= kSkinnyRows && area && f.C % 8 == 0 && f.F % 8 == 0) {
-      void* h = ws.take((size_t)f.M * f.F * sizeof(TO));
+      void* h = ws.take((size_t)f.M * f.F * (f.M <= kDotRows ? sizeof(float) : sizeof(TO)));
       if (dry) return kOk;
       if constexpr (sizeof(TO) == 2) return few_rows<1>(y, h);
       else return planes == 3 ? few_rows<3>(y, h) : planes == 2 ? few_rows<2>(y, h) : few_rows<1>(y, h);

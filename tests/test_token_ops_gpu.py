@@ -109,6 +109,14 @@ def test_layer_norm(ops, shape, dtype):
                randn(3, C, dtype=dtype, scale=0.3), dy=randn(4, *shape, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(150, 8200), (4500, 8195), (513, 1024), (2000, 512), (260, 2050), (2300, 2048), (33, 8192)])
+def test_layer_norm_row_groups(ops, shape, dtype):
+    """Row counts on both sides of every split of the rows over blocks and runs."""
+    C = shape[-1]
+    check_norm(ops, randn(1, *shape, dtype=dtype), randn(2, C, dtype=dtype), randn(3, C, dtype=dtype), dy=randn(4, *shape, dtype=dtype))
+
+
 @pytest.mark.parametrize("dtype", DTYPES[1:], ids=str)
 @pytest.mark.parametrize("shape", [(9, 40), (1500, 256), (3, 8195)])
 def test_layer_norm_float32_parameters(ops, shape, dtype):
@@ -253,6 +261,31 @@ def test_gated_ffn_few_rows(ops, size, dtype):
         check_ffn(ops, a, b, dy, "silu", mode=mode, keep=False, need=(False,) * 7)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("size", [(3, 40, 88, 16), (4, 520, 1032, 130), (5, 512, 8, 40), (8, 72, 8192, 64), (9, 72, 8192, 64),
+                                  (48, 64, 1368, 64), (64, 64, 1024, 33)])
+def test_gated_ffn_few_rows_forms(ops, size, dtype):
+    """Rows and hidden channels on both sides of every change of form."""
+    check_ffn(ops, *ffn_inputs(*size, dtype), "gelu", keep=False, need=(False,) * 7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows", [1, 2, 4, 7, 33, 70])
+def test_gated_ffn_non_finite_rows_stay_apart(ops, rows, dtype):
+    """A row of infinities and NaN changes no other row, and a weight's infinite row only its hidden channel."""
+    a, b, _ = ffn_inputs(rows + 1, 40, 88, 24, dtype)
+    y, _ = ops.gated_ffn_fwd(*a, *b)
+    x = a[0].clone()
+    x[rows, ::2], x[rows, 1::2] = float("inf"), float("nan")
+    y2, _ = ops.gated_ffn_fwd(x, *a[1:], *b)
+    assert torch.equal(y2[:rows], y[:rows]) and not y2[rows].isfinite().any()
+    wd = a[3].clone()
+    wd[5, 0] = float("inf")
+    y3, _ = ops.gated_ffn_fwd(*a[:3], wd, *b)
+    keep = [i for i in range(24) if i != 5]
+    assert torch.equal(y3[:, keep], y[:, keep]) and not y3[:, 5].isfinite().any()
+
+
 @pytest.mark.parametrize("need", [(1, 0, 0, 0, 0, 0, 0), (0, 1, 0, 0, 0, 0, 0), (0, 0, 1, 0, 0, 0, 1), (0, 0, 0, 1, 0, 0, 0),
                                   (0, 0, 0, 0, 1, 0, 0), (0, 0, 0, 0, 0, 1, 0), (0,) * 7])
 def test_gated_ffn_some_gradients(ops, need):
@@ -350,6 +383,14 @@ RECUR_SIZES = [(1, 1, 1), (3, 1, 70), (2, 5, 64), (2, 16, 3), (2, 17, 65), (1, 1
 def test_linear_recurrence(ops, size, dtype):
     x, d, z, h0, dy, dlast = recurrence_inputs(*size, dtype)
     check_recurrence(ops, x, d, z, h0, dy, dlast, False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("size", [(70, 1, 130), (5, 2, 37), (7, 3, 130), (5, 4, 37), (40, 7, 9), (2, 15, 64), (130, 16, 128)])
+def test_linear_recurrence_short(ops, size, reverse, dtype):
+    x, d, z, h0, dy, dlast = recurrence_inputs(*size, dtype, gate=not reverse)
+    check_recurrence(ops, x, d, z, h0, dy, dlast, reverse)
 
 
 @pytest.mark.parametrize("size", RECUR_SIZES)
