@@ -413,7 +413,7 @@ enum mragan_dtype { MRAGAN_DT_F32 = 0, MRAGAN_DT_BF16 = 1, MRAGAN_DT_F16 = 2 };
  * weight / bias ([C], type wdtype: dtype or fp32) may be NULL (1 / 0); mean and rstd ([rows]) are
  * outputs the backward reads.  bwd: dx, dweight, dbias (types as x and weight) may each be NULL to
  * skip it; dweight and dbias are reduced over the rows in a fixed order.  No tensor may overlap an
- * output. */
+ * output.  Rows below 2³¹, C up to 2³⁰. */
 int mragan_layer_norm_fwd(const void* x, int64_t rows, int C, int dtype, const void* weight, const void* bias, int wdtype,
                           float eps, void* y, float* mean, float* rstd, void* stream);
 size_t mragan_layer_norm_bwd_workspace(int64_t rows, int C, int dtype);
@@ -424,12 +424,14 @@ int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, c
 /* Gated feed-forward block on x [M][C] with weights w_gate, w_up [F][C] and w_down [O][F]:
  *   g = x·w_gateᵀ + b_gate,  u = x·w_upᵀ + b_up,  h = act(g)·u,  y = h·w_downᵀ + b_down   ([M][O])
  * act: mragan_act or one of the two below (GELU is the erf form).  Biases may be NULL.  One dtype
- * throughout; 16-byte aligned contiguous tensors; C, F and O below 2²².  fp32 tensors are multiplied in the process
- * mode of mragan_set_conv_precision (f32 here: three bf16 planes per operand, six products, fp32
- * accumulation, ≤ 2⁻²² relative error per product; an infinite operand gives NaN); 16-bit tensors as they are, and what the
- * products take from each other (h, dg, du) is rounded to that type.  kept (fp32: [3][M][F], 16-bit
- * types: [4][M][F], the last two factors with 24 bits) holds h, act'(g)·u and act(g): fwd writes it
- * when given, bwd reads it, or recomputes it from x when NULL.  bwd: any gradient may be NULL to skip it. */
+ * throughout; 16-byte aligned contiguous tensors; C, F and O below 2²².  fp32 tensors are multiplied
+ * in the process mode of mragan_set_conv_precision (f32 here: three bf16 planes per operand, six
+ * products, fp32 accumulation, ≤ 2⁻²² relative error per product; an infinite operand gives NaN);
+ * 16-bit tensors as they are, and what the products take from each other (h, dg, du) is rounded to
+ * that type, but h stays in fp32 for up to four rows without kept where C and F are multiples of 8.
+ * kept (fp32: [3][M][F], 16-bit types: [4][M][F], the last two factors with 24 bits) holds h,
+ * act'(g)·u and act(g): fwd writes it when given, bwd reads it, or recomputes it from x when NULL.
+ * bwd: any gradient may be NULL to skip it. */
 enum mragan_gate_act { MRAGAN_ACT_SILU = 5, MRAGAN_ACT_GELU = 6 };
 size_t mragan_gated_ffn_workspace(int64_t M, int C, int F, int O, int dtype, int backward, int recompute);
 int mragan_gated_ffn_fwd(const void* x, int64_t M, int C, int F, int O, int dtype, const void* w_gate, const void* w_up,
@@ -444,7 +446,8 @@ int mragan_gated_ffn_bwd(const void* x, int64_t M, int C, int F, int O, int dtyp
  *   a_t = σ(decay_t),  h_t = a_t·h_{t−1} + σ(−decay_t)·x_t,  y_t = h_t·silu(gate_t)   (y = h: gate NULL)
  * from h_{−1} = h0 ([B][C] fp32, NULL = 0), or from the last position to the first with reverse = 1.
  * x, decay, gate, dy: element (b, t, c) at b·stride_b + t·stride_t + c (strides in elements, slices
- * of one projection or expanded tensors; stride_t and C below 2²²); y, dx, ddecay, dgate: contiguous [B][T][C].
+ * of one projection or expanded tensors; stride_t and C below 2²²); y, dx, ddecay, dgate: contiguous
+ * [B][T][C].
  * last [B][C] fp32: the state after the last step.  carry [B][mragan_linear_recurrence_carries(T, C)][C]
  * fp32: states at fixed steps that the backward restarts from (NULL in an inference call).
  * decay = +inf leaves the state as it is (a padded position), −inf restarts from x_t; x and h

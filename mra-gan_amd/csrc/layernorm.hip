@@ -11,14 +11,14 @@
 // flight, and w and b are loaded once per block.  The weight's gradient is summed per lane over the
 // rows of its block in fp32, then over the block's row groups in LDS, then over the blocks by a
 // second launch: a fixed order, no atomics.
+// Measured: 524288 rows of 32 fp32 channels 26 us forward (134 MB, 5.2 TB/s), 33 + 4 us backward (201 MB);
+// 8192 rows of 2048 bf16 channels 14.3 us forward (67 MB, 4.7 TB/s), 27.4 + 4.1 us backward (101 MB).  A copy
+// of 256 MB moves 5.4 TB/s.
 #include "token_ops.h"
 
 namespace mragan {
 namespace {
 
-#ifndef LN_MIN
-#define LN_MIN 8
-#endif
 constexpr int kThreads = 256;
 
 // A lane's 16 bytes of a row.  Rows of any channel count start at any element; gfx950 takes global
@@ -289,42 +289,46 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* part
 // Rows of more channels than the registers of a block hold (C > kMaxRow): the block walks the row
 // in memory, once per sum; the parameter gradients take a column per thread over a run of rows.
 template <typename T, typename W>
-__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* x, int C, const W* w, const W* b, float eps, T* y,
-                                                           float* mean, float* rstd) {
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* x, int64_t rows, int C, const W* w, const W* b, float eps,
+                                                           T* y, float* mean, float* rstd) {
   __shared__ float red[2][16];
-  const int64_t row = blockIdx.x;
-  const T* xr = x + row * C;
-  float s = 0.f, q = 0.f;
-  for (int c = threadIdx.x; c < C; c += 1024) s += (float)xr[c];
-  const float mu = row_sum<1024>(s, red[0]) / (float)C;
-  for (int c = threadIdx.x; c < C; c += 1024) {
-    const float d = (float)xr[c] - mu;
-    q += d * d;
-  }
-  const float r = rsqrtf(row_sum<1024>(q, red[1]) / (float)C + eps);
-  for (int c = threadIdx.x; c < C; c += 1024)
-    y[row * C + c] = (T)(((float)xr[c] - mu) * r * (w ? (float)w[c] : 1.f) + (b ? (float)b[c] : 0.f));
-  if (threadIdx.x == 0) {
-    mean[row] = mu;
-    rstd[row] = r;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* xr = x + row * C;
+    float s = 0.f, q = 0.f;
+    for (int c = threadIdx.x; c < C; c += 1024) s += (float)xr[c];
+    const float mu = row_sum<1024>(s, red[0]) / (float)C;
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const float d = (float)xr[c] - mu;
+      q += d * d;
+    }
+    const float r = rsqrtf(row_sum<1024>(q, red[1]) / (float)C + eps);
+    for (int c = threadIdx.x; c < C; c += 1024)
+      y[row * C + c] = (T)(((float)xr[c] - mu) * r * (w ? (float)w[c] : 1.f) + (b ? (float)b[c] : 0.f));
+    if (threadIdx.x == 0) {
+      mean[row] = mu;
+      rstd[row] = r;
+    }
+    __syncthreads();                                                 // red is read before the next row writes it
   }
 }
 template <typename T, typename W>
-__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* x, const float* mean, const float* rstd, const T* dy, int C,
-                                                           const W* w, T* dx) {
+__global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* x, const float* mean, const float* rstd, const T* dy,
+                                                           int64_t rows, int C, const W* w, T* dx) {
   __shared__ float red[2][16];
-  const int64_t row = blockIdx.x;
-  const float mu = mean[row], r = rstd[row];
-  float s1 = 0.f, s2 = 0.f;
-  for (int c = threadIdx.x; c < C; c += 1024) {
-    const float p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
-    s1 += p;
-    s2 += p * ((float)x[row * C + c] - mu) * r;
-  }
-  const float m1 = row_sum<1024>(s1, red[0]) / (float)C, m2 = row_sum<1024>(s2, red[1]) / (float)C;
-  for (int c = threadIdx.x; c < C; c += 1024) {
-    const float xh = ((float)x[row * C + c] - mu) * r, p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
-    dx[row * C + c] = (T)(r * (p - m1 - xh * m2));
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float mu = mean[row], r = rstd[row];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const float p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
+      s1 += p;
+      s2 += p * ((float)x[row * C + c] - mu) * r;
+    }
+    const float m1 = row_sum<1024>(s1, red[0]) / (float)C, m2 = row_sum<1024>(s2, red[1]) / (float)C;
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      const float xh = ((float)x[row * C + c] - mu) * r, p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
+      dx[row * C + c] = (T)(r * (p - m1 - xh * m2));
+    }
+    __syncthreads();
   }
 }
 // part: [gridDim.y][2][C], rows dealt to gridDim.y in runs of `per`
@@ -349,6 +353,8 @@ __global__ __launch_bounds__(256) void ln_param_long_kernel(const T* x, const fl
 // The largest row that a block holds: 16 channels a thread of 512 (backward: their 256 registers also
 // carry the next row, the weight and two accumulators), 32 a thread of 256 (forward).
 constexpr int kMaxRow = 8192;
+// blocks of the longer rows' kernels: a launch takes fewer than 2^32 threads
+unsigned long_grid(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
 // Most blocks of a backward launch: four on each of the 256 CUs, whose partial sums the second launch reads
 constexpr int kMaxBwdBlocks = 1024;
 
@@ -378,7 +384,7 @@ int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, flo
   const W *wt = static_cast<const W*>(w), *bt = static_cast<const W*>(b);
   T* yt = static_cast<T*>(y);
   if (C > kMaxRow) {
-    ln_fwd_long_kernel<T, W><<<(unsigned)rows, 1024, 0, st>>>(xt, C, wt, bt, eps, yt, mean, rstd);
+    ln_fwd_long_kernel<T, W><<<long_grid(rows), 1024, 0, st>>>(xt, rows, C, wt, bt, eps, yt, mean, rstd);
     return check_launch("layer_norm_fwd_long");
   }
   // bf16, 2048 channels: 64 rows take 2.6 us with a block each, 3.3 with a wave; 1024 channels: 256 rows
@@ -412,12 +418,14 @@ int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, flo
 // 29.2 with 32 channels a lane of a wave.  No block a row for few rows: each block's sums are as long as
 // a row, and 1024 rows of 1024 channels take 14.5 us with 1024 such blocks, 7.3 with a wave a row.
 Shape bwd_shape(int C, int N) { return pick(0, C, N, 16, -1); }
-// As many blocks as the chip holds, but at least LN_MIN row groups each where that leaves one for every CU.
+// As many blocks as the chip holds, but at least eight row groups each where that leaves one block for
+// every CU, as each block adds 8·C bytes of sums: 2048 rows of 2048 bf16 channels take 15.2 us, 17.0 with
+// four groups each, 24.8 with one.
 int bwd_blocks(int64_t rows, int C, int N) {
   const Shape s = bwd_shape(C, N);
   const int per = s.G > kThreads ? 1 : kThreads / s.G;
   const int64_t groups = (rows + per - 1) / per, most = s.G > kThreads ? kMaxBwdBlocks / 2 : kMaxBwdBlocks;
-  const int64_t few = groups < 256 ? groups : 256, blocks = groups / LN_MIN > few ? groups / LN_MIN : few;
+  const int64_t few = groups < 256 ? groups : 256, blocks = groups / 8 > few ? groups / 8 : few;
   return (int)(blocks < most ? blocks : most);
 }
 
@@ -435,7 +443,7 @@ int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, 
   const bool params = dw || db;
   if (C > kMaxRow) {
     if (dx) {
-      ln_bwd_long_kernel<T, W><<<(unsigned)rows, 1024, 0, st>>>(xt, mean, rstd, dyt, C, wt, dxt);
+      ln_bwd_long_kernel<T, W><<<long_grid(rows), 1024, 0, st>>>(xt, mean, rstd, dyt, rows, C, wt, dxt);
       if (int rc = check_launch("layer_norm_bwd_long")) return rc;
     }
     if (!params) return kOk;

@@ -7,13 +7,17 @@
 // Both recursions are products of affine maps s ↦ P·s + E, which compose associatively, so time is
 // split: a lane takes S = 8 steps of two channels in order, the time lanes of a wave join their maps
 // in registers and the waves of a block through LDS (a chunk of 128 steps), and a block walks over
-// the chunks with the fp32 state of its channels in registers, the next chunk's loads in flight.  HBM is the bound: each tensor is read or written once.  Where B and C give too few blocks
-// to fill the chip, the chunks are also split into segments over blocks: a first launch reduces each
-// segment to its (P, E), the second starts each segment from the fold of the ones before it (its
-// inputs then come a second time, as a rule from the 256 MB cache).
+// the chunks with the fp32 state of its channels in registers, the next chunk's loads in
+// flight.  HBM is the bound: each tensor is read or written once.  Where B and C give too few blocks to
+// fill the chip, the chunks are also split into segments over blocks: a first launch reduces each segment
+// to its (P, E), the second starts each segment from the fold of the ones before it (its inputs then come
+// a second time, as a rule from the 256 MB cache).
 // Steps behind the end of a sequence and channels behind C enter as d = +inf, x = 0: the identity.
 // The forward leaves the fp32 state entering each chunk; the backward recomputes the states of a
 // chunk from it in registers and walks the chunks backwards, so that no state is read or written.
+// Measured: 16 × 2048 × 1024 bf16 with gate 71 us forward (268 MB, 3.8 TB/s) and 106 us backward (470 MB,
+// 4.4 TB/s), one block of 8 waves a CU; 2 × 32768 × 128 fp32 in segments 14 + 18 us forward (67 MB read
+// twice, 34 MB written) and 16 + 33 us backward.
 #include "token_ops.h"
 
 namespace mragan {
@@ -679,6 +683,8 @@ Geo geometry(int64_t B, int64_t T, int C, int reverse) {
   return g;
 }
 
+int64_t blocks_of(const Geo& g) { return g.T <= kShort ? (g.B * g.tiles + 127) / 128 : g.B * g.tiles * g.segs; }
+
 // run the statement block with the channel lanes as LC
 #define MRAGAN_RECUR_LC(lc, ...) \
   if (lc == 32) {                \
@@ -697,9 +703,9 @@ Strided<T> strided(const void* p, int64_t sb, int64_t st) {
 }  // namespace
 
 int64_t recurrence_carries(int64_t T) { return T <= 0 ? 0 : (T + kChunk - 1) / kChunk; }
-int64_t recurrence_blocks(int64_t B, int64_t T, int C) {
+int64_t recurrence_threads(int64_t B, int64_t T, int C) {
   const Geo g = geometry(B, T, C, 0);
-  return T <= kShort ? (B * g.tiles + 127) / 128 : B * g.tiles * g.segs;
+  return blocks_of(g) * (T <= kShort ? 128 : g.lc * kLT);
 }
 
 size_t recurrence_ws_bytes(int64_t B, int64_t T, int C) {
@@ -710,7 +716,7 @@ size_t recurrence_ws_bytes(int64_t B, int64_t T, int C) {
 
 int recurrence_fwd(const RecurArgs& r, const float* h0, void* y, float* last, float* carry, float* ws, hipStream_t st) {
   const Geo g = geometry(r.B, r.T, r.C, r.reverse);
-  const unsigned grid = (unsigned)recurrence_blocks(r.B, r.T, r.C);
+  const unsigned grid = (unsigned)blocks_of(g);
   MRAGAN_DTYPE_DISPATCH(r.dtype, T, {
     const auto x = strided<T>(r.x, r.x_sb, r.x_st), d = strided<T>(r.decay, r.d_sb, r.d_st), z = strided<T>(r.gate, r.g_sb, r.g_st);
     T* yt = static_cast<T*>(y);
@@ -737,7 +743,7 @@ int recurrence_fwd(const RecurArgs& r, const float* h0, void* y, float* last, fl
 int recurrence_bwd(const RecurArgs& r, const float* carry, const void* dy, int64_t dy_sb, int64_t dy_st, const float* dlast,
                    void* dx, void* dd, void* dz, float* dh0, float* ws, hipStream_t st) {
   const Geo g = geometry(r.B, r.T, r.C, r.reverse);
-  const unsigned grid = (unsigned)recurrence_blocks(r.B, r.T, r.C);
+  const unsigned grid = (unsigned)blocks_of(g);
   MRAGAN_DTYPE_DISPATCH(r.dtype, T, {
     const auto x = strided<T>(r.x, r.x_sb, r.x_st), d = strided<T>(r.decay, r.d_sb, r.d_st), z = strided<T>(r.gate, r.g_sb, r.g_st),
                gy = strided<T>(dy, dy_sb, dy_st);

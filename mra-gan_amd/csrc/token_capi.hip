@@ -8,7 +8,8 @@
 using namespace mragan;
 
 namespace {
-constexpr int64_t kMaxGrid = (int64_t)1 << 31;
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;         // of a launch, exclusive
+constexpr int64_t kMaxChannels = (int64_t)1 << 30;        // of a normalized row: strided walks stay in an int
 constexpr int64_t kMaxSide = ((int64_t)1 << 22) - 64;     // row length of an FFN operand: 256 rows below 2^31 bytes
 constexpr int64_t kMaxRows = (int64_t)1 << 30;
 
@@ -27,7 +28,7 @@ int mragan_layer_norm_fwd(const void* x, int64_t rows, int C, int dtype, const v
   MRAGAN_CHECK_ARG(rows == 0 || (x && y && mean && rstd), "layer_norm: null pointer");
   MRAGAN_CHECK_ARG(dtype_ok(dtype) && (wdtype == dtype || wdtype == kF32), "layer_norm: bad types %d / %d", dtype, wdtype);
   MRAGAN_CHECK_ARG(eps >= 0.f, "layer_norm: eps must not be negative");
-  MRAGAN_CHECK_ARG(rows < kMaxGrid, "layer_norm: too many rows");
+  MRAGAN_CHECK_ARG(rows < kMaxRows * 2 && C <= kMaxChannels, "layer_norm: too many rows or channels (rows from 2^31 on, C above 2^30)");
   return layer_norm_fwd(x, rows, C, dtype, weight, bias, wdtype, eps, y, mean, rstd, static_cast<hipStream_t>(stream));
 }
 
@@ -41,7 +42,7 @@ int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, c
   MRAGAN_CHECK_ARG(rows >= 0 && C > 0, "layer_norm_bwd: bad shape [%lld][%d]", (long long)rows, C);
   MRAGAN_CHECK_ARG(rows == 0 || (x && mean && rstd && dy), "layer_norm_bwd: null pointer");
   MRAGAN_CHECK_ARG(dtype_ok(dtype) && (wdtype == dtype || wdtype == kF32), "layer_norm_bwd: bad types %d / %d", dtype, wdtype);
-  MRAGAN_CHECK_ARG(rows < kMaxGrid, "layer_norm_bwd: too many rows");
+  MRAGAN_CHECK_ARG(rows < kMaxRows * 2 && C <= kMaxChannels, "layer_norm_bwd: too many rows or channels (rows from 2^31 on, C above 2^30)");
   if (!dx && !dweight && !dbias) return kOk;
   if (dweight || dbias) {
     const size_t need = rows ? layer_norm_bwd_ws_bytes(rows, C, dtype) : 0;
@@ -127,7 +128,7 @@ static int recur_check(const RecurArgs& r, const void* ws, size_t ws_bytes) {
   MRAGAN_CHECK_ARG(r.x && r.decay, "linear_recurrence: null pointer");
   MRAGAN_CHECK_ARG(time_stride_ok(r.x_st) && time_stride_ok(r.d_st) && time_stride_ok(r.g_st) && time_stride_ok(r.C),
                    "linear_recurrence: time strides and C must be in [0, 2^22)");
-  MRAGAN_CHECK_ARG(recurrence_blocks(r.B, r.T, r.C) < kMaxGrid, "linear_recurrence: too many sequences");
+  MRAGAN_CHECK_ARG(r.B <= kMaxThreads && recurrence_threads(r.B, r.T, r.C) < kMaxThreads, "linear_recurrence: too many sequences");
   const size_t need = recurrence_ws_bytes(r.B, r.T, r.C);
   if (need && (!ws || ws_bytes < need)) {
     set_error("linear_recurrence: workspace %zu < %zu bytes (query mragan_linear_recurrence_workspace)", ws_bytes, need);

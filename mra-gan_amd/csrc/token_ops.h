@@ -18,7 +18,7 @@ struct RecurArgs {
   int C, dtype, reverse;
 };
 int64_t recurrence_carries(int64_t T);
-int64_t recurrence_blocks(int64_t B, int64_t T, int C);   // of the largest launch
+int64_t recurrence_threads(int64_t B, int64_t T, int C);   // of the largest launch
 size_t recurrence_ws_bytes(int64_t B, int64_t T, int C);
 int recurrence_fwd(const RecurArgs& r, const float* h0, void* y, float* last, float* carry, float* ws, hipStream_t st);
 int recurrence_bwd(const RecurArgs& r, const float* carry, const void* dy, int64_t dy_sb, int64_t dy_st, const float* dlast,

@@ -1117,7 +1117,7 @@ def _like(t: Optional[torch.Tensor], name: str, ref: torch.Tensor, shape, dtype=
     """t of this shape, of ref's device and (unless given) type; None passes."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != (dtype or ref.dtype):
         raise ValueError(f"{name}: expected {dtype or ref.dtype}, got {t.dtype}")
@@ -1177,7 +1177,7 @@ def layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty_like(x)
-    mean = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     fn = lambda: _call_on(x, "mragan_layer_norm_fwd", _ptr(x), mean.numel(), C, dt, _ptr(weight), _ptr(bias), _DTYPE[wd], eps,
                           _ptr(y), _ptr(mean), _ptr(rstd))
@@ -1203,8 +1203,8 @@ def layer_norm_bwd(x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, dy: 
     x, dy, mean, rstd = x.contiguous(), dy.contiguous(), mean.contiguous(), rstd.contiguous()
     weight = None if weight is None else weight.contiguous()
     dx = torch.empty_like(x)
-    dw = None if weight is None else torch.empty(C, device=x.device, dtype=wd)
-    db = torch.empty(C, device=x.device, dtype=wd) if bias else None
+    dw = None if weight is None else x.new_empty(C, dtype=wd)
+    db = x.new_empty(C, dtype=wd) if bias else None
     nbytes = query("mragan_layer_norm_bwd_workspace", mean.numel(), C, dt) if dw is not None or bias else 0
     ws = _scratch(nbytes, x)
     fn = lambda: _call_on(x, "mragan_layer_norm_bwd", _ptr(x), _ptr(mean), _ptr(rstd), _ptr(dy), mean.numel(), C, dt,
@@ -1244,8 +1244,8 @@ def gated_ffn_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_d
     dt, C, F, O = _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
     x, w_gate, w_up, w_down, b_gate, b_up, b_down = map(_dense, (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
     M = x.numel() // C
-    y = torch.empty(x.shape[:-1] + (O,), device=x.device, dtype=x.dtype)
-    kept = torch.empty(_kept_shape(x, M, F), device=x.device, dtype=x.dtype) if keep else None
+    y = x.new_empty((*x.shape[:-1], O))
+    kept = x.new_empty(_kept_shape(x, M, F)) if keep else None
     nbytes = query("mragan_gated_ffn_workspace", M, C, F, O, dt, 0, 0)
     ws = _scratch(nbytes, x)
     fn = lambda: _call_on(x, "mragan_gated_ffn_fwd", _ptr(x), M, C, F, O, dt, _ptr(w_gate), _ptr(w_up), _ptr(w_down),
@@ -1266,7 +1266,7 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_d
     M = x.numel() // C
     _like(kept, "gated_ffn_bwd.kept", x, _kept_shape(x, M, F))
     like = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-    grads = [torch.empty(t.shape, device=x.device, dtype=x.dtype) if n and t is not None else None for t, n in zip(like, need)]
+    grads = [x.new_empty(t.shape) if n and t is not None else None for t, n in zip(like, need)]
     if M == 0:                                             # no rows: empty sums
         return tuple(None if g is None else g.zero_() for g in grads)
     x, w_gate, w_up, w_down, b_gate, b_up, dy, kept = map(_dense, (x, w_gate, w_up, w_down, b_gate, b_up, dy, kept))
@@ -1309,12 +1309,12 @@ def linear_recurrence_fwd(x: torch.Tensor, decay: torch.Tensor, gate: Optional[t
     gs = _sequence(gate, "linear_recurrence.gate", x)
     _like(h0, "linear_recurrence.h0", x, (B, C), torch.float32)
     h0 = None if h0 is None else h0.contiguous()
-    y = torch.empty((B, T, C), device=x.device, dtype=x.dtype)
-    carry = torch.empty((B, query("mragan_linear_recurrence_carries", T, C), C), device=x.device, dtype=torch.float32)
+    y = x.new_empty((B, T, C))
+    carry = x.new_empty((B, query("mragan_linear_recurrence_carries", T, C), C), dtype=torch.float32)
     if T == 0 or B == 0:
         last = torch.zeros((B, C), device=x.device, dtype=torch.float32) if h0 is None else h0.clone()
         return y, last, carry
-    last = torch.empty((B, C), device=x.device, dtype=torch.float32)
+    last = x.new_empty((B, C), dtype=torch.float32)
     nbytes = query("mragan_linear_recurrence_workspace", B, T, C, 0)
     ws = _scratch(nbytes, x)
     fn = lambda: _call_on(x, "mragan_linear_recurrence_fwd", _ptr(xs[0]), xs[1], xs[2], _ptr(ds[0]), ds[1], ds[2], _ptr(gs[0]),
@@ -1338,12 +1338,12 @@ def linear_recurrence_bwd(x: torch.Tensor, decay: torch.Tensor, carry: torch.Ten
     _like(dlast, "linear_recurrence_bwd.dlast", x, (B, C), torch.float32)
     carry = carry.contiguous()
     dlast = None if dlast is None else dlast.contiguous()
-    new = lambda n: torch.empty((B, T, C), device=x.device, dtype=x.dtype) if n else None
+    new = lambda n: x.new_empty((B, T, C)) if n else None
     dx, dd, dz = new(need[0]), new(need[1]), new(need[2] and gate is not None)
     if T == 0 or B == 0:
         dh0 = (torch.zeros((B, C), device=x.device, dtype=torch.float32) if dlast is None else dlast.clone()) if need[3] else None
         return dx, dd, dz, dh0
-    dh0 = torch.empty((B, C), device=x.device, dtype=torch.float32) if need[3] else None
+    dh0 = x.new_empty((B, C), dtype=torch.float32) if need[3] else None
     nbytes = query("mragan_linear_recurrence_workspace", B, T, C, 1)
     ws = _scratch(nbytes, x)
     fn = lambda: _call_on(x, "mragan_linear_recurrence_bwd", _ptr(xs[0]), xs[1], xs[2], _ptr(ds[0]), ds[1], ds[2], _ptr(gs[0]),

@@ -65,6 +65,10 @@ P = 1 << 20      # an aligned address that is never dereferenced: each call belo
     ("null pointer", "mragan_linear_recurrence_fwd", (P, 8, 8, None, 8, 8, None, 0, 0, None, 1, 4, 8, 0, 0, P, P, P, None, 0, None)),
     ("null pointer", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1, 4, 8, 0, 0, P, None, P, None, 0, None)),
     ("too many", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1 << 40, 4, 8, 0, 0, P, P, P, None, 0, None)),
+    ("too many", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1 << 23, 17, 64, 0, 0, P, P, P, None, 0, None)),
+    ("too many", "mragan_linear_recurrence_fwd", (P, 8, 8, P, 8, 8, None, 0, 0, None, 1 << 32, 1, 4, 0, 0, P, P, P, None, 0, None)),
+    ("too many rows or channels", "mragan_layer_norm_fwd", (P, 1, (1 << 30) + 1, 0, None, None, 0, 1e-5, P, P, P, None)),
+    ("too many rows or channels", "mragan_layer_norm_bwd", (P, P, P, P, 1 << 31, 8, 0, None, 0, P, None, None, None, 0, None)),
     ("without a gate", "mragan_linear_recurrence_bwd", (P, 8, 8, P, 8, 8, None, 0, 0, P, P, 8, 8, None, 1, 4, 8, 0, 0, P, P, P, P, None, 0, None)),
 ])
 def test_entry_points_refuse(match, name, args):

@@ -117,6 +117,15 @@ def test_layer_norm_row_groups(ops, shape, dtype):
     check_norm(ops, randn(1, *shape, dtype=dtype), randn(2, C, dtype=dtype), randn(3, C, dtype=dtype), dy=randn(4, *shape, dtype=dtype))
 
 
+def test_layer_norm_more_long_rows_than_blocks(ops):
+    x, dy = randn(1, 65600, 8200, dtype=torch.bfloat16), randn(2, 65600, 8200, dtype=torch.bfloat16)
+    w, tail = randn(3, 8200, dtype=torch.bfloat16), slice(65500, None)
+    whole, part = ops.layer_norm_fwd(x, w), ops.layer_norm_fwd(x[tail], w)
+    assert all(torch.equal(a[tail], b) for a, b in zip(whole, part))
+    dx = ops.layer_norm_bwd(x, *whole[1:], dy, w)[0]
+    assert torch.equal(dx[tail], ops.layer_norm_bwd(x[tail], *part[1:], dy[tail], w)[0])
+
+
 @pytest.mark.parametrize("dtype", DTYPES[1:], ids=str)
 @pytest.mark.parametrize("shape", [(9, 40), (1500, 256), (3, 8195)])
 def test_layer_norm_float32_parameters(ops, shape, dtype):
