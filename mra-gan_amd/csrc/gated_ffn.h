@@ -217,8 +217,9 @@ struct GemmArgs {
   const void* A2[kMaxPairs];      // of a second product with the same B (batches = 2), to out2
   const void* B[kMaxPairs];       // [N][ldb] or [K][ldb]; kEpiGate: the gate weight
   const void* B2[kMaxPairs];      // kEpiGate: the up weight
-  int pairs, ktiles, batches;     // operand pairs, stages of kBK of one pair
+  int pairs, ktiles, batches;     // operand pairs (NP > 1: of first planes), stages of kBK of one pair
   int64_t lda, ldb, K;            // elements
+  int64_t plane_a, plane_b;       // bytes from an operand's plane to its next
   int M, N;
   int tiles_m, tiles_n, splits, per_split;   // stages of all pairs cut into `splits` runs of per_split
   // kEpiStore: out[m][n] (+ bias[n]); splits > 1: fp32 partials [batch][split][M][N]
@@ -425,13 +426,30 @@ __device__ __forceinline__ int swz_t(int k) {
 // operand's fragment is the first MFMA operand, and its fragment rows are chosen so that a lane ends
 // with eight consecutive n of a row m, four lanes with 32 (nrow): the epilogue moves 16 bytes a lane, 64
 // a row, at a time.
-template <typename H, typename TO, int EPI, bool TA, bool TB, int BM, int BN, int WM, int WN, int NS>
+// NP > 1: a stage holds that k run of NP planes of both operands and enters all their products that count,
+// p + q < NP, so each tile is loaded once for several products (NP = 1: plane pairs are pairs like others).
+template <int P>
+struct PlaneProducts;
+template <>
+struct PlaneProducts<1> {
+  static constexpr int n = 1, a[1] = {0}, b[1] = {0};
+};
+template <>
+struct PlaneProducts<2> {                                        // the small products first
+  static constexpr int n = 3, a[3] = {0, 1, 0}, b[3] = {1, 0, 0};
+};
+template <>
+struct PlaneProducts<3> {
+  static constexpr int n = 6, a[6] = {0, 1, 2, 0, 1, 0}, b[6] = {2, 1, 0, 1, 0, 0};
+};
+template <typename H, typename TO, int EPI, bool TA, bool TB, int BM, int BN, int WM, int WN, int NS, int NP = 1>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2))) void ffn_gemm_kernel(const GemmArgs a) {
   constexpr int kWaves = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int NF = EPI == kEpiGate ? FN / 2 : FN;              // n fragments of one output
   constexpr int LA = BM / 8 / kWaves, LB = BN / 8 / kWaves;      // loads of a wave per stage
   static_assert(NF == 4 || NF == 2, "");
-  __shared__ uint4 lds[NS][(BM + BN) * 8];
+  constexpr int kImage = (BM + BN) * 128, kSlot = NP * kImage;    // bytes of a plane's two tiles, of a stage
+  __shared__ uint4 lds[NS][kSlot / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 
   // Blocks are dealt to the 8 XCDs in turn: give each XCD a contiguous run of tiles, walked in
@@ -507,15 +525,17 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     }
   };
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)&lds[0][0];
-  // load `i` of this wave's LA + LB of a stage, into the ring's slot
-  auto issue = [&](int i, int slot) {
-    const unsigned l = lds0 + slot * ((BM + BN) * 128);
+  // load `n` of this wave's NP·(LA + LB) of a stage, into the ring's slot
+  auto issue = [&](int n, int slot) {
+    const int p = n / (LA + LB), i = n % (LA + LB);
+    const unsigned l = lds0 + slot * kSlot + p * kImage;
+    auto of = [&](const Window& w, int64_t plane) { return Window{w.p + p * plane, w.left}.rsrc(); };
     if (i < LA) {
-      load_to_lds(wa.rsrc(), l + (wave * LA + i) * 1024, offA[i < LA ? i : 0]);
+      load_to_lds(of(wa, a.plane_a), l + (wave * LA + i) * 1024, offA[i < LA ? i : 0]);
     } else {
       const int j = i - LA;
       const bool up = EPI == kEpiGate && (wave * LB + j) * 8 >= BN / 2;
-      load_to_lds(up ? wb2.rsrc() : wb.rsrc(), l + BM * 128 + (wave * LB + j) * 1024, offB[j < 0 ? 0 : j]);
+      load_to_lds(of(up ? wb2 : wb, a.plane_b), l + BM * 128 + (wave * LB + j) * 1024, offB[j < 0 ? 0 : j]);
     }
   };
 
@@ -534,12 +554,12 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
   // A fragment of a tile whose rows are contiguous: `at` addresses this lane's quad of the wave's first
   // fragment in the k rows fk·8 + fr / 4; other fragments differ in bits of the chunk only, which the
   // permutation leaves a difference by exclusive or, other k rows by a multiple of 4 (no change to it).
-  auto frag_t = [&](auto tile_rows, unsigned at, unsigned other, int slot, int ks) {
+  auto frag_t = [&](auto tile_rows, unsigned at, unsigned other, int image, int ks) {
     constexpr int rows = decltype(tile_rows)::value;
     s16x4 half[2];
 #pragma unroll
     for (int hb = 0; hb < 2; hb++)
-      half[hb] = read_transposed(reinterpret_cast<const char*>(lds) + ((at ^ other) + slot * ((BM + BN) * 128)) + (ks * 32 + hb * 4) * rows * 2);
+      half[hb] = read_transposed(reinterpret_cast<const char*>(lds) + ((at ^ other) + image) + (ks * 32 + hb * 4) * rows * 2);
     return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
   unsigned atA = 0, atB = 0;
@@ -549,31 +569,41 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
     if constexpr (TB) atB = BM * 128 + k * BN * 2 + (((wn * (2 * NF) + (fr & 3)) ^ swz_t<BN>(k)) << 4);
   }
   struct Frags {
-    bf16x8 a[FM], b[FN];
+    bf16x8 a[NP][FM], b[NP][FN];
   };
-  // fragment `i` of FN + FM of k step ks in a slot
-  auto read = [&](int slot, int ks, int i, Frags& f) {
-    const uint4* la = lds[slot];
-    const uint4* lb = lds[slot] + BM * 8;
+  // fragment `n` of NP·(FN + FM) of k step ks in a slot
+  auto read = [&](int slot, int ks, int n, Frags& f) {
+    const int p = n / (FN + FM), i = n % (FN + FM), image = slot * kSlot + p * kImage;
+    const uint4* la = &lds[0][0] + image / 16;
+    const uint4* lb = la + BM * 8;
     if (i < FN) {
       if constexpr (TB) {
-        f.b[i] = frag_t(IntConst<BN>{}, atB, (i >> 1) * 64 + (i & 1) * 8, slot, ks);
+        f.b[p][i] = frag_t(IntConst<BN>{}, atB, (i >> 1) * 64 + (i & 1) * 8, image, ks);
       } else {
         const int r = nrow(i, fr);
-        f.b[i] = __builtin_bit_cast(bf16x8, lb[r * 8 + ((ks * 4 + fk) ^ ((r & 3) | ((r >> 3 & 1) << 2)))]);
+        f.b[p][i] = __builtin_bit_cast(bf16x8, lb[r * 8 + ((ks * 4 + fk) ^ ((r & 3) | ((r >> 3 & 1) << 2)))]);
       }
     } else {
-      if constexpr (TA) f.a[i - FN] = frag_t(IntConst<BM>{}, atA, (i - FN) * 32, slot, ks);
-      else f.a[i - FN] = __builtin_bit_cast(bf16x8, la[(wm * (BM / WM) + (i - FN) * 16 + fr) * 8 + ((ks * 4 + fk) ^ (fr & 7))]);
+      if constexpr (TA) f.a[p][i - FN] = frag_t(IntConst<BM>{}, atA, (i - FN) * 32, image, ks);
+      else f.a[p][i - FN] = __builtin_bit_cast(bf16x8, la[(wm * (BM / WM) + (i - FN) * 16 + fr) * 8 + ((ks * 4 + fk) ^ (fr & 7))]);
     }
   };
+  // the products of a k step come in S groups: by rows of fragments (NP = 1) or by plane pairs
+  constexpr int S = NP == 1 ? FM : PlaneProducts<NP>::n;
+  auto products = [&](int s, const Frags& f) {
+    const int p = NP == 1 ? 0 : PlaneProducts<NP>::a[NP == 1 ? 0 : s], q = NP == 1 ? 0 : PlaneProducts<NP>::b[NP == 1 ? 0 : s];
+#pragma unroll
+    for (int i = NP == 1 ? s : 0; i < (NP == 1 ? s + 1 : FM); i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) acc[i][j] = mfma16<H>(f.b[q][j], f.a[p][i], acc[i][j]);
+  };
 
-  // A stage is two k steps of 32.  A k step's products go row by row of fragments, and between the rows
+  // A stage is two k steps of 32.  A k step's products go group by group, and between the groups
   // go the reads of the next step's fragments and, in the second step, the loads of stage kt + NS (the
   // matrix unit runs on while the wave issues them; sched_barrier keeps the order).  Between the two
   // steps all waves meet: the next stage has landed for each, and the slot of this one, read by all,
   // is free for the loads.
-  constexpr int L = LA + LB, NR = FM + FN;
+  constexpr int L = NP * (LA + LB), NR = NP * (FM + FN);
   static_assert(kBK == 64, "");
   int get = 0;
   if (kt < kend) {
@@ -595,11 +625,10 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
       // each fragment's address is an exclusive or away: not to be kept in a register over the loop
       if constexpr (TA) asm volatile("" : "+v"(atA), "+v"(atB));
 #pragma unroll
-      for (int i = 0; i < FM; i++) {
+      for (int s = 0; s < S; s++) {
+        products(s, f0);
 #pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mfma16<H>(f0.b[j], f0.a[i], acc[i][j]);
-#pragma unroll
-        for (int r = i * NR / FM; r < (i + 1) * NR / FM; r++) read(get, 1, r, f1);
+        for (int r = s * NR / S; r < (s + 1) * NR / S; r++) read(get, 1, r, f1);
         __builtin_amdgcn_sched_barrier(0);
       }
       const int slot = get;
@@ -609,16 +638,15 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
         get = get + 1 == NS ? 0 : get + 1;
       }
 #pragma unroll
-      for (int i = 0; i < FM; i++) {
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mfma16<H>(f1.b[j], f1.a[i], acc[i][j]);
+      for (int s = 0; s < S; s++) {
+        products(s, f1);
         if constexpr (more) {
 #pragma unroll
-          for (int r = i * NR / FM; r < (i + 1) * NR / FM; r++) read(get, 0, r, f0);
+          for (int r = s * NR / S; r < (s + 1) * NR / S; r++) read(get, 0, r, f0);
         }
         if constexpr (load) {
 #pragma unroll
-          for (int r = i * L / FM; r < (i + 1) * L / FM; r++) issue(r, slot);
+          for (int r = s * L / S; r < (s + 1) * L / S; r++) issue(r, slot);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -990,23 +1018,29 @@ struct Tiling {
   int bm, bn, tiles_m, tiles_n, splits, per_split;   // bn: columns of the output
 };
 // The largest of three tiles that still gives the 256 CUs a block each: 256×256, 128×128 (two blocks a
-// CU), 64×64 (kEpiGate: half as many columns of g and of u each, 64×64 with 64).  A product of small
-// tiles whose partial sums may be stored splits k into runs of at least 4 stages: up to two blocks a CU
-// where there is not one, up to three for 64 stages and more, over which one block a CU waits longer than
-// the sums cost (fp32 8192 × 128 from 2 × 512, 96 stages: 37.8 us unsplit, 32 split; from 512, 48 stages:
-// 18.9 and 21).
-Tiling tile(int64_t M, int64_t N, int batches, int stages, bool gate, bool may_split) {
+// CU), 64×64 (kEpiGate: half as many columns of g and of u each, 64×64 with 64).  `stages`: of one plane
+// pair; `products`: plane pairs.  Small tiles take all planes of a k run in one stage (NP): they are bound
+// by their loads (fp32 8192 rows, 128 → 512 → 128: forward and backward 145 us, 181 with a plane pair a
+// stage; the forward takes 49 us, 55 with such stages in place of the 128×128 tiles too).
+// A product of small tiles whose partial sums may be stored splits k into runs of at least 4 stages (2 of
+// all planes): up to two blocks a CU where there is not one (one with three planes, whose stages fill its
+// LDS: 512 × 128 from 8192, 21.2 us, 23.6 with two), and with one plane up to three for 64 stages and more,
+// over which one block a CU waits longer than the sums cost (8192 × 128, 96 stages: 37.8 us unsplit, 32
+// split; 48 stages: 18.9 and 21).
+Tiling tile(int64_t M, int64_t N, int batches, int stages, int products, bool gate, bool may_split) {
   Tiling t{};
   for (int b : {256, 128, 64}) {
     t.bm = b, t.bn = gate && b > 64 ? b / 2 : b;
     t.tiles_m = (int)((M + t.bm - 1) / t.bm), t.tiles_n = (int)((N + t.bn - 1) / t.bn);
     if ((int64_t)t.tiles_m * t.tiles_n * batches >= 224) break;
   }
+  if (t.bm > 64) stages *= products;
   t.splits = 1;
   const int64_t tiles = (int64_t)t.tiles_m * t.tiles_n * batches;
-  if (may_split && t.bm == 64 && (tiles < 224 || (stages >= 64 && tiles < 512))) {
-    int64_t s = (tiles < 224 ? 512 : 768) / tiles;
-    if (s > stages / 4) s = stages / 4;
+  if (may_split && t.bm == 64 && (tiles < 224 || (products == 1 && stages >= 64 && tiles < 512))) {
+    int64_t s = (products > 3 ? 256 : tiles < 224 ? 512 : 768) / tiles;
+    const int run = products > 1 ? 2 : 4;
+    if (s > stages / run) s = stages / run;
     const int64_t cap = (int64_t)(kPartialCap / ((size_t)M * N * batches * 4));
     if (s > cap) s = cap;
     if (s > 1) t.splits = (int)s;
@@ -1089,6 +1123,7 @@ struct Ffn {
       a.B2[a.pairs] = B2 ? B2->p + pb[i] * B2->rows * B2->ld * 2 : nullptr;
     }
     a.lda = A.ld, a.ldb = B.ld, a.K = K;
+    a.plane_a = A.rows * A.ld * 2, a.plane_b = B.rows * B.ld * 2;
     a.ktiles = (int)(round_k(K) / kBK);
     a.batches = A2 ? 2 : 1;
   }
@@ -1102,7 +1137,17 @@ struct Ffn {
     constexpr int GM = EPI == kEpiGate ? 4 : 2;              // waves along m: 128-byte rows of the gate's outputs a wave
     if (t.bm == 256) ffn_gemm_kernel<H, TO, EPI, TA, TB, 256, 256, GM, 8 / GM, 2><<<grid, 512, 0, st>>>(a);
     else if (t.bm == 128) ffn_gemm_kernel<H, TO, EPI, TA, TB, 128, 128, 2, 2, 2><<<grid, 256, 0, st>>>(a);
-    else ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 3><<<grid, 256, 0, st>>>(a);
+    else if (planes == 1) ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 3><<<grid, 256, 0, st>>>(a);
+    else if constexpr (sizeof(TO) == 4 && !__is_same(H, _Float16)) {   // fp32 as two or three bf16 planes
+      const int n = npairs();
+      a.pairs /= n;
+      for (int g = 0; g < a.pairs; g++) {                              // the last of a run of pairs is that of the first planes
+        const int k = g * n + n - 1;
+        a.A[g] = a.A[k], a.A2[g] = a.A2[k], a.B[g] = a.B[k], a.B2[g] = a.B2[k];
+      }
+      if (planes == 2) ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 2, 2><<<grid, 256, 0, st>>>(a);
+      else ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 2, 3><<<grid, 256, 0, st>>>(a);
+    }
     if (int rc = check_launch(EPI == kEpiStore ? "ffn_gemm" : EPI == kEpiGate ? "ffn_gemm_gate" : "ffn_gemm_gate_bwd")) return rc;
     if (t.splits > 1) {
       const int64_t total = (int64_t)a.M * a.N;
@@ -1142,7 +1187,7 @@ struct Ffn {
     a.bias_g = f.bg, a.bias_u = f.bu, a.act = f.act, a.planes = planes;
     a.kept = kept;
     a.h = const_cast<char*>(h.p), a.ldf = h.ld;
-    return gemm<kEpiGate, false, false>(a, tile(f.M, f.F, 1, a.pairs * a.ktiles, true, false), nullptr);
+    return gemm<kEpiGate, false, false>(a, tile(f.M, f.F, 1, a.ktiles, npairs(), true, false), nullptr);
   }
 
   // One launch for few rows, x [M][K]: NB = 2 gate, up → h; NB = 1 down → y.  P: planes of the operands.
@@ -1198,7 +1243,7 @@ struct Ffn {
     const Operand wd = operand(f.wd, f.O, f.F, false);
     if (int rc = flush()) return rc;
     if (int rc = gate(in, direct && kept ? Operand{} : h, kept)) return rc;
-    const Tiling t = tile(f.M, f.O, 1, npairs() * (int)(h.ld / kBK), false, true);
+    const Tiling t = tile(f.M, f.O, 1, (int)(h.ld / kBK), npairs(), false, true);
     void* partial = ws.take(partial_bytes(t, f.M, f.O, 1));
     if (dry) return kOk;
     GemmArgs a{};
@@ -1242,7 +1287,7 @@ struct Ffn {
     }
     if (inner) {
       dg = planes_of(f.M, f.F), du = planes_of(f.M, f.F);
-      const Tiling t = tile(f.M, f.F, 1, npairs() * (int)(round_k(f.O) / kBK), false, false);
+      const Tiling t = tile(f.M, f.F, 1, (int)(round_k(f.O) / kBK), npairs(), false, false);
       const int rows = t.tiles_m * 2;                        // two waves along m in every tile
       float* part = o.dbg || o.dbu ? static_cast<float*>(ws.take((size_t)rows * 2 * f.F * sizeof(float))) : nullptr;
       if (!dry) {
@@ -1261,7 +1306,7 @@ struct Ffn {
       }
     }
     if (o.dx) {
-      const Tiling t = tile(f.M, f.C, 1, 2 * npairs() * (int)(dg.ld / kBK), false, true);
+      const Tiling t = tile(f.M, f.C, 1, 2 * (int)(dg.ld / kBK), npairs(), false, true);
       void* partial = ws.take(partial_bytes(t, f.M, f.C, 1));
       if (!dry) {
         GemmArgs a{};
@@ -1274,7 +1319,7 @@ struct Ffn {
     }
     if (weights) {
       const int both = o.dwg && o.dwu ? 2 : 1;
-      const Tiling t = tile(f.F, f.C, both, npairs() * (int)(round_k(f.M) / kBK), false, true);
+      const Tiling t = tile(f.F, f.C, both, (int)(round_k(f.M) / kBK), npairs(), false, true);
       void* partial = ws.take(partial_bytes(t, f.F, f.C, both));
       if (!dry) {
         GemmArgs a{};
@@ -1285,7 +1330,7 @@ struct Ffn {
       }
     }
     if (o.dwd) {
-      const Tiling t = tile(f.O, f.F, 1, npairs() * (int)(round_k(f.M) / kBK), false, true);
+      const Tiling t = tile(f.O, f.F, 1, (int)(round_k(f.M) / kBK), npairs(), false, true);
       void* partial = ws.take(partial_bytes(t, f.O, f.F, 1));
       if (!dry) {
         GemmArgs a{};
