@@ -405,15 +405,16 @@ int mragan_crop_patches(const float* vol, int X, int Y, int Z, const int* starts
 
 /* ---- layers of a token block on channels-last tensors -----------------------------------------
  * Activations are [rows][C] with the channels contiguous (an NDHWC volume is N·D·H·W rows) and may
- * be fp32, bf16 or fp16 (mragan_dtype); statistics, states and every sum are fp32.  These entry
- * points are additions: the version number above is unchanged by them. */
+ * be fp32, bf16 or fp16 (mragan_dtype); statistics, states and every sum are fp32.  No output or
+ * workspace may overlap another tensor of the call.  These entry points are additions: the version
+ * number above is unchanged by them. */
 enum mragan_dtype { MRAGAN_DT_F32 = 0, MRAGAN_DT_BF16 = 1, MRAGAN_DT_F16 = 2 };
 
 /* LayerNorm over the channels: y = (x − μ)·rstd·weight + bias, rstd = (mean((x − μ)²) + eps)^−½.
  * weight / bias ([C], type wdtype: dtype or fp32) may be NULL (1 / 0); mean and rstd ([rows]) are
  * outputs the backward reads.  bwd: dx, dweight, dbias (types as x and weight) may each be NULL to
- * skip it; dweight and dbias are reduced over the rows in a fixed order.  No tensor may overlap an
- * output.  Rows below 2³¹, C up to 2³⁰. */
+ * skip it; dweight and dbias are reduced over the rows in a fixed order.  Rows below 2³¹, C
+ * up to 2³⁰. */
 int mragan_layer_norm_fwd(const void* x, int64_t rows, int C, int dtype, const void* weight, const void* bias, int wdtype,
                           float eps, void* y, float* mean, float* rstd, void* stream);
 size_t mragan_layer_norm_bwd_workspace(int64_t rows, int C, int dtype);
