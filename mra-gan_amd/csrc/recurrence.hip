@@ -12,7 +12,7 @@
 // fill the chip, the chunks are also split into segments over blocks: a first launch reduces each segment
 // to its (P, E), the second starts each segment from the fold of the ones before it (its inputs then come
 // a second time, as a rule from the 256 MB cache).
-// Steps behind the end of a sequence and channels behind C enter as d = +inf, x = 0: the identity.
+// Steps behind the end of a sequence enter as d = +inf, x = 0: the identity.
 // The forward leaves the fp32 state entering each chunk; the backward recomputes the states of a
 // chunk from it in registers and walks the chunks backwards, so that no state is read or written.
 // Measured: 16 × 2048 × 1024 bf16 with gate 71 us forward (268 MB, 3.8 TB/s) and 106 us backward (470 MB,
@@ -86,16 +86,27 @@ struct Geo {
   __device__ __forceinline__ int64_t at(int64_t t) const { return reverse ? T - 1 - t : t; }
 };
 
-// this block's (sequence, segment, first channel) and this thread's channels and time lane
+// This block's (sequence, segment, first channel) and this thread's channels and time lane.  Lanes that
+// would pass the last channel are moved back to end with it and compute and write channels of their
+// neighbours again, with the same values: no tile has another path for its channels (B = 4, T = 49191, 117
+// bf16 channels, forward and backward: 181 us instead of 237).  Only a single channel, less than a lane's, is guarded.
 struct Place {
   int64_t b, k0, k1;
   int seg, c0, wave, half, odd, lt, cl, c, n;                       // half, odd: bits of the time lane in its wave
+  int last;                                                         // the last lane's first channel
+  // the channel of slot `i` of the tile (slot cl + v: this lane's channel c + v)
+  __device__ __forceinline__ int channel(int i) const {
+    const int c = c0 + i / kVC * kVC;
+    return (c < last ? c : last) + i % kVC;
+  }
 };
 template <int LC>
 __device__ __forceinline__ Place place(const Geo& g) {
   Place p;
   int64_t id = blockIdx.x;
+  p.last = g.C > kVC ? g.C - kVC : 0;
   p.c0 = (int)(id % g.tiles) * Shape<LC>::kCT;
+  p.c0 = p.c0 < p.last ? p.c0 : p.last;
   id /= g.tiles;
   p.seg = (int)(id % g.segs);
   p.b = id / g.segs;
@@ -106,15 +117,14 @@ __device__ __forceinline__ Place place(const Geo& g) {
   p.odd = (threadIdx.x >> 4) & 1;
   p.lt = threadIdx.x / LC;
   p.cl = (threadIdx.x % LC) * kVC;
-  p.c = p.c0 + p.cl;
+  p.c = p.channel(p.cl);
   p.n = g.C - p.c;
   return p;
 }
 
 // Where this lane's steps of chunk k lie: a wave-uniform address per step (of the chunk's lowest
 // position in memory, which a chunk cut off by the sequence's end may place before the tensor) plus
-// one 32-bit offset of the lane — per-lane 64-bit addresses of every step and tensor would fill the
-// registers.  Steps behind the end and channels behind C read as `fill` and are not written.
+// one 32-bit offset of the lane — per-lane 64-bit addresses of every step and tensor would registers.  Steps behind the end (and C = 1's second channel) read as `fill` and are not written.
 template <typename T>
 struct Steps {
   T* base;                                                           // step 0 of time lane 0 (reverse: of the last)
@@ -123,7 +133,7 @@ struct Steps {
   __device__ __forceinline__ Steps(T* q, int64_t sb, int64_t st, const Geo& g, const Place& p, int64_t k) {
     const int64_t low = g.reverse ? g.T - (k + 1) * kChunk + kS - 1 : k * kChunk;
     base = q + (p.b * sb + low * st + p.c0);
-    off = (unsigned)(g.reverse ? kLT - 1 - p.lt : p.lt) * (unsigned)(kS * st) + p.cl;
+    off = (unsigned)(g.reverse ? kLT - 1 - p.lt : p.lt) * (unsigned)(kS * st) + (unsigned)(p.c - p.c0);
     step = g.reverse ? -st : st;
   }
   __device__ __forceinline__ T* at(int s) const { return base + s * step + off; }
@@ -149,11 +159,10 @@ __device__ __forceinline__ void store_step(const Steps<T>& a, const Geo& g, cons
   if (WHOLE) __builtin_memcpy(a.at(s), &r, sizeof(r));
   else if (k * kChunk + p.lt * kS + s < g.T && p.n > 0) group_store<kVC>(a.at(s), p.n, r);
 }
-// chunks from k0 on that lie inside the sequence with all channels of the tile: the loop over them
-// has no other path, whose merges would wait for the loads in flight
-template <int LC>
+// chunks from k0 on that lie inside the sequence: the loop over them has no other path, whose merges
+// would wait for the loads in flight
 __device__ __forceinline__ int64_t whole_chunks_end(const Geo& g, const Place& p) {
-  const int64_t e = p.c0 + Shape<LC>::kCT <= g.C ? g.T / kChunk : p.k0;
+  const int64_t e = g.C >= kVC ? g.T / kChunk : p.k0;
   return e < p.k0 ? p.k0 : e < p.k1 ? e : p.k1;
 }
 
@@ -216,8 +225,8 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_segment_kernel(Stri
 #pragma unroll
   for (int v = 0; v < kVC; v++) sP[p.lt][p.cl + v] = P[v], sE[p.lt][p.cl + v] = E[v];
   __syncthreads();
-  if (threadIdx.x < kCT && p.c0 + (int)threadIdx.x < g.C) {
-    const int ch = threadIdx.x;
+  const int ch = threadIdx.x;
+  if (ch < kCT && p.channel(ch) < g.C) {
     float m = 1.f, s = 0.f;
 #pragma unroll
     for (int j = 0; j < kLT; j++) {
@@ -225,7 +234,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_segment_kernel(Stri
       s = sP[l][ch] * s + sE[l][ch];
       m *= sP[l][ch];
     }
-    float* out = agg + ((p.b * g.segs + p.seg) * 2) * g.C + p.c0 + ch;
+    float* out = agg + ((p.b * g.segs + p.seg) * 2) * g.C + p.channel(ch);
     out[0] = m;
     out[g.C] = s;
   }
@@ -245,8 +254,8 @@ __device__ __forceinline__ void enter(const float* s0, const float* agg, const G
   const int lo = BWD ? p.seg + 1 : 0, cnt = BWD ? g.segs - 1 - p.seg : p.seg;
   const int part = (cnt + kParts - 1) / kParts, j0 = at * part, j1 = j0 + part < cnt ? j0 + part : cnt;
   float m = 1.f, s = 0.f;
-  if (p.c0 + ch < g.C) {
-    const float* q = agg + (p.b * g.segs + lo) * 2 * (int64_t)g.C + p.c0 + ch;
+  if (p.channel(ch) < g.C) {
+    const float* q = agg + (p.b * g.segs + lo) * 2 * (int64_t)g.C + p.channel(ch);
 #pragma unroll 4
     for (int j = j0; j < j1; j++) {
       const int64_t o = 2 * (int64_t)(BWD ? cnt - 1 - j : j) * g.C;
@@ -284,7 +293,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_fwd_kernel(Strided<
     load_steps<W>(d, g, p, k, __builtin_inff(), n.d);
     if constexpr (GATE) load_steps<W>(z, g, p, k, 0.f, n.z);
   };
-  const int64_t whole_end = whole_chunks_end<LC>(g, p);
+  const int64_t whole_end = whole_chunks_end(g, p);
   auto chunk = [&](auto whole, int64_t k, Raw& n) {
     constexpr bool W = decltype(whole)::value;
     const int par = k & 1;
@@ -391,7 +400,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_bwd_kernel(Strided<
 #pragma unroll
     for (int v = 0; v < kVC; v++) n.h[v] = W || v < p.n ? carry[(p.b * g.chunks + k) * g.C + p.c + v] : 0.f;
   };
-  const int64_t whole_end = whole_chunks_end<LC>(g, p);
+  const int64_t whole_end = whole_chunks_end(g, p);
   auto chunk = [&](auto whole, int64_t k, Raw& n) {
     constexpr bool W = decltype(whole)::value;
     const int par = k & 1;
@@ -668,7 +677,8 @@ __global__ __launch_bounds__(128) void recur_bwd_short_kernel(Strided<T> x, Stri
 // Tiles of 64 channels, of 32 where C has no more (fp32, 16384 steps of 32 channels,
 // 16 sequences with gate: 35 us forward and 59 backward against 51 and 96 with half the lanes idle).
 // Segments: none once sequences × channel tiles give each of the 256 CUs a block; else as many as
-// bring the launch to about two blocks a CU, each at least four chunks long.
+// bring the launch up to two blocks a CU (B = 3, T = 9705, 680 fp16 channels, forward and backward: 201 us, 229
+// with 16 blocks more), each at least four chunks long.
 Geo geometry(int64_t B, int64_t T, int C, int reverse) {
   Geo g{};
   g.B = B, g.T = T, g.C = C, g.reverse = reverse;
@@ -676,7 +686,7 @@ Geo geometry(int64_t B, int64_t T, int C, int reverse) {
   g.lc = C <= 32 ? 16 : 32;
   g.tiles = T <= kShort ? ceil_div(C, kShortVC) : ceil_div(C, g.lc * kVC);
   const int64_t base = B * g.tiles;
-  int64_t segs = base >= 256 ? 1 : (512 + base - 1) / base;
+  int64_t segs = base >= 256 ? 1 : 512 / base;
   if (segs > g.chunks / 4) segs = g.chunks / 4 > 0 ? g.chunks / 4 : 1;
   g.per_seg = (g.chunks + segs - 1) / segs;
   g.segs = (int)((g.chunks + g.per_seg - 1) / g.per_seg);

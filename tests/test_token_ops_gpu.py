@@ -660,3 +660,13 @@ def test_refusals(ops):
     with pytest.raises(MraganError, match="workspace"):
         call("mragan_gated_ffn_fwd", a[0].data_ptr(), 5, 8, 12, 6, 0, a[1].data_ptr(), a[2].data_ptr(), a[3].data_ptr(), None, None,
              None, 5, dy.data_ptr(), None, None, 0, None)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("size", [(2, 140, 1), (3, 300, 2), (2, 200, 15), (2, 300, 33), (2, 400, 63), (3, 1300, 117), (1, 5000, 65),
+                                  (2, 300, 129)])
+def test_linear_recurrence_last_channels(ops, size, dtype):
+    """Channel counts that end inside a tile, in one segment and in several, in both directions."""
+    x, d, z, h0, dy, dlast = recurrence_inputs(*size, dtype)
+    check_recurrence(ops, x, d, z, h0, dy, dlast, False)
+    check_recurrence(ops, x, d, None, h0, dy, dlast, True)
