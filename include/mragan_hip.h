@@ -429,7 +429,7 @@ int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, c
  * in the process mode of mragan_set_conv_precision (f32 here: three bf16 planes per operand, six
  * products, fp32 accumulation, ≤ 2⁻²² relative error per product; an infinite operand gives NaN);
  * 16-bit tensors as they are, and what the products take from each other (h, dg, du) is rounded to
- * that type, but h stays in fp32 for up to four rows without kept where C and F are multiples of 8.
+ * that type, but h stays in fp32 for up to four rows without kept where C and F are 8 or more.
  * kept (fp32: [3][M][F], 16-bit types: [4][M][F], the last two factors with 24 bits) holds h,
  * act'(g)·u and act(g): fwd writes it when given, bwd reads it, or recomputes it from x when NULL.
  * bwd: any gradient may be NULL to skip it. */

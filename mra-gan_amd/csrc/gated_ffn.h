@@ -817,14 +817,28 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)
 // fp32 weights would have to be split into planes in memory first (64 rows, 2048 → 8192: 122 us and 243).
 constexpr int kSkinnyRows = 64, kSkinnyArea = 65536;
 
-// eight elements from k < K (K a multiple of eight); behind K zeros, by a load of the row's start and a
-// selection: a branch around each load would wait for one before the next
-template <typename T>
-__device__ __forceinline__ Words<T, 8> load_words8(const T* row, int64_t k, int64_t K) {
+// Eight elements from k on, zeros behind K and where `live` is not set: by a load from inside the row and
+// a selection, as a branch around each load would wait for one before the next.  ODD (K ≥ 8 no multiple of
+// eight): the row's last eight elements are loaded as they end with it, and those before k are zeros; the
+// other operand's are moved alike.
+template <bool ODD, typename T>
+__device__ __forceinline__ Words<T, 8> load_words8(const T* row, int64_t k, int64_t K, bool live = true) {
   Words<T, 8> r;
-  __builtin_memcpy(&r, row + (k < K ? k : 0), sizeof(r));
+  if constexpr (ODD) {
+    const int64_t at = live && k + 8 <= K ? k : K - 8;
+    const int skip = live && k < K ? (int)(k - at) : 8;
+    __builtin_memcpy(&r, row + at, sizeof(r));
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(r) / 4); i++) r.w[i] = k < K ? r.w[i] : 0u;
+    for (int i = 0; i < (int)(sizeof(r) / 4); i++) {
+      if constexpr (sizeof(T) == 4) r.w[i] = i >= skip ? r.w[i] : 0u;
+      else r.w[i] &= 2 * i >= skip ? ~0u : 2 * i + 1 >= skip ? 0xffff0000u : 0u;
+    }
+  } else {
+    const bool in = live && k < K;
+    __builtin_memcpy(&r, row + (in ? k : 0), sizeof(r));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(r) / 4); i++) r.w[i] = in ? r.w[i] : 0u;
+  }
   return r;
 }
 // the same as the fragments of P planes
@@ -859,7 +873,7 @@ __device__ __forceinline__ float gate_act(float g, int act) {
 constexpr int kDotRows = 4;
 // h stays in fp32 between the two launches (TX, TY: the types of x and of the result).
 // ROUND: operands rounded to H, as the one-plane modes of fp32 tensors have them
-template <typename H, typename TX, typename TO, typename TY, int NB, int MR, bool ROUND>
+template <typename H, typename TX, typename TO, typename TY, int NB, int MR, bool ROUND, bool ODD>
 __global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_t K, const TO* w0, const TO* w1, const TO* b0,
                                                       const TO* b1, int N, int act, TY* out) {
   auto in = [](float v) { return ROUND ? (float)(H)v : v; };
@@ -878,9 +892,9 @@ __global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_
 #pragma unroll
     for (int u = 0; u < U; u++) {
 #pragma unroll
-      for (int b = 0; b < NB; b++) wv[u][b] = load_words8(w[b], k0 + u * 512, K);
+      for (int b = 0; b < NB; b++) wv[u][b] = load_words8<ODD>(w[b], k0 + u * 512, K);
 #pragma unroll
-      for (int m = 0; m < MR; m++) xv[u][m] = load_words8(x + (int64_t)(m < M ? m : M - 1) * K, k0 + u * 512, K);
+      for (int m = 0; m < MR; m++) xv[u][m] = load_words8<ODD>(x + (int64_t)(m < M ? m : M - 1) * K, k0 + u * 512, K);
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -905,7 +919,7 @@ __global__ __launch_bounds__(256) void ffn_dot_kernel(const TX* x, int M, int64_
 }
 
 // NB weights (gate and up, or down alone) times x [M][K], both as P planes: h = act(g)·u (NB = 2) or y
-template <typename H, typename TO, int NB, int MF, int P, int WAVES>
+template <typename H, typename TO, int NB, int MF, int P, int WAVES, bool ODD>
 __global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TO* x, int M, int64_t K, const TO* w0, const TO* w1,
                                                                 const TO* b0, const TO* b1, int N, int act, TO* out) {
   constexpr int kLoads = (NB + MF) * (int)sizeof(TO) / 2;             // 16-byte loads a k step
@@ -926,11 +940,12 @@ __global__ __launch_bounds__(64 * WAVES) void ffn_skinny_kernel(const TO* x, int
     Words<TO, 8> qx[U][MF];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int64_t k = (s + u) * 32 + fk * 8, end = s + u < s1 ? K : 0;
+      const int64_t k = (s + u) * 32 + fk * 8;
+      const bool live = s + u < s1;
 #pragma unroll
-      for (int b = 0; b < NB; b++) qw[u][b] = load_words8(w[b], k, end);
+      for (int b = 0; b < NB; b++) qw[u][b] = load_words8<ODD>(w[b], k, K, live);
 #pragma unroll
-      for (int m = 0; m < MF; m++) qx[u][m] = load_words8(x + (int64_t)(m * 16 + fr < M ? m * 16 + fr : M - 1) * K, k, end);
+      for (int m = 0; m < MF; m++) qx[u][m] = load_words8<ODD>(x + (int64_t)(m * 16 + fr < M ? m * 16 + fr : M - 1) * K, k, K, live);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -1191,7 +1206,7 @@ struct Ffn {
   }
 
   // One launch for few rows, x [M][K]: NB = 2 gate, up → h; NB = 1 down → y.  P: planes of the operands.
-  template <int NB, int P>
+  template <int NB, int P, bool ODD>
   int skinny(const void* x, int64_t K, const void* w0, const void* w1, const void* b0, const void* b1, int N, void* out) {
     const TO *xt = static_cast<const TO*>(x), *v0 = static_cast<const TO*>(w0), *v1 = static_cast<const TO*>(w1),
              *c0 = static_cast<const TO*>(b0), *c1 = static_cast<const TO*>(b1);
@@ -1199,12 +1214,12 @@ struct Ffn {
     const int M = (int)f.M;
     constexpr int W = 8;
     const unsigned grid = (unsigned)ceil_div(N, 16);
-    if (M <= 16) ffn_skinny_kernel<H, TO, NB, 1, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
-    else if (M <= 32) ffn_skinny_kernel<H, TO, NB, 2, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
-    else ffn_skinny_kernel<H, TO, NB, 4, P, W><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
+    if (M <= 16) ffn_skinny_kernel<H, TO, NB, 1, P, W, ODD><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
+    else if (M <= 32) ffn_skinny_kernel<H, TO, NB, 2, P, W, ODD><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
+    else ffn_skinny_kernel<H, TO, NB, 4, P, W, ODD><<<grid, 64 * W, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, o);
     return check_launch("ffn_skinny");
   }
-  template <int NB, int P, typename TX, typename TY>
+  template <int NB, int P, bool ODD, typename TX, typename TY>
   int dot(const void* x, int64_t K, const void* w0, const void* w1, const void* b0, const void* b1, int N, TY* out) {
     constexpr bool R = sizeof(TO) == 4 && P == 1;
     const TX* xt = static_cast<const TX*>(x);
@@ -1212,24 +1227,30 @@ struct Ffn {
              *c1 = static_cast<const TO*>(b1);
     const int M = (int)f.M;
     const unsigned grid = (unsigned)ceil_div(N, 4);
-    if (M == 1) ffn_dot_kernel<H, TX, TO, TY, NB, 1, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
-    else if (M == 2) ffn_dot_kernel<H, TX, TO, TY, NB, 2, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
-    else ffn_dot_kernel<H, TX, TO, TY, NB, 4, R><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
+    if (M == 1) ffn_dot_kernel<H, TX, TO, TY, NB, 1, R, ODD><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
+    else if (M == 2) ffn_dot_kernel<H, TX, TO, TY, NB, 2, R, ODD><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
+    else ffn_dot_kernel<H, TX, TO, TY, NB, 4, R, ODD><<<grid, 256, 0, st>>>(xt, M, K, v0, v1, c0, c1, N, f.act, out);
     return check_launch("ffn_dot");
+  }
+  template <int P, bool ODD>
+  int first(void* h) {
+    if (f.M <= kDotRows) return dot<2, P, ODD, TO>(f.x, f.C, f.wg, f.wu, f.bg, f.bu, f.F, static_cast<float*>(h));
+    return skinny<2, P, ODD>(f.x, f.C, f.wg, f.wu, f.bg, f.bu, f.F, h);
+  }
+  template <int P, bool ODD>
+  int second(const void* h, void* y) {
+    if (f.M <= kDotRows) return dot<1, P, ODD, float>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, static_cast<TO*>(y));
+    return skinny<1, P, ODD>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, y);
   }
   template <int P>
   int few_rows(void* y, void* h) {
-    if (f.M <= kDotRows) {
-      if (int rc = dot<2, P, TO>(f.x, f.C, f.wg, f.wu, f.bg, f.bu, f.F, static_cast<float*>(h))) return rc;
-      return dot<1, P, float>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, static_cast<TO*>(y));
-    }
-    if (int rc = skinny<2, P>(f.x, f.C, f.wg, f.wu, f.bg, f.bu, f.F, h)) return rc;
-    return skinny<1, P>(h, f.F, f.wd, nullptr, f.bd, nullptr, f.O, y);
+    if (int rc = f.C % 8 ? first<P, true>(h) : first<P, false>(h)) return rc;
+    return f.F % 8 ? second<P, true>(h, y) : second<P, false>(h, y);
   }
 
   int forward(void* y, void* kept) {
     const bool area = sizeof(TO) == 4 || f.M * f.F <= kSkinnyArea || f.M <= kDotRows;
-    if (!kept && f.M <= kSkinnyRows && area && f.C % 8 == 0 && f.F % 8 == 0) {
+    if (!kept && f.M <= kSkinnyRows && area && f.C >= 8 && f.F >= 8) {
       void* h = ws.take((size_t)f.M * f.F * (f.M <= kDotRows ? sizeof(float) : sizeof(TO)));
       if (dry) return kOk;
       if constexpr (sizeof(TO) == 2) return few_rows<1>(y, h);

@@ -272,7 +272,8 @@ def test_gated_ffn_few_rows(ops, size, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("size", [(3, 40, 88, 16), (4, 520, 1032, 130), (5, 512, 8, 40), (8, 72, 8192, 64), (9, 72, 8192, 64),
-                                  (48, 64, 1368, 64), (64, 64, 1024, 33)])
+                                  (48, 64, 1368, 64), (64, 64, 1024, 33), (1, 959, 333, 70), (2, 515, 1333, 9),
+                                  (4, 9, 11, 5), (3, 8, 15, 3), (7, 13, 517, 33), (30, 101, 77, 9), (64, 35, 100, 20), (20, 40, 1001, 8)])
 def test_gated_ffn_few_rows_forms(ops, size, dtype):
     """Rows and hidden channels on both sides of every change of form."""
     check_ffn(ops, *ffn_inputs(*size, dtype), "gelu", keep=False, need=(False,) * 7)
