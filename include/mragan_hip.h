@@ -432,7 +432,7 @@ int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, c
  * that type, but h stays in fp32 for up to four rows without kept where C and F are 8 or more.
  * kept (fp32: [3][M][F], 16-bit types: [4][M][F], the last two factors with 24 bits) holds h,
  * act'(g)·u and act(g): fwd writes it when given, bwd reads it, or recomputes it from x when NULL.
- * bwd: any gradient may be NULL to skip it. */
+ * bwd: any gradient may be NULL to skip it; the queried workspace is enough for any choice. */
 enum mragan_gate_act { MRAGAN_ACT_SILU = 5, MRAGAN_ACT_GELU = 6 };
 size_t mragan_gated_ffn_workspace(int64_t M, int C, int F, int O, int dtype, int backward, int recompute);
 int mragan_gated_ffn_fwd(const void* x, int64_t M, int C, int F, int O, int dtype, const void* w_gate, const void* w_up,

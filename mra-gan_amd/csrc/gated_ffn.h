@@ -1340,8 +1340,16 @@ struct Ffn {
     }
     if (weights) {
       const int both = o.dwg && o.dwu ? 2 : 1;
-      const Tiling t = tile(f.F, f.C, both, (int)(round_k(f.M) / kBK), npairs(), false, true);
-      void* partial = ws.take(partial_bytes(t, f.F, f.C, both));
+      const int stages = (int)(round_k(f.M) / kBK);
+      const Tiling t = tile(f.F, f.C, both, stages, npairs(), false, true);
+      // one product has half the tiles of two and may split k where those do not: room for either, so that the
+      // size asked for with both gradients holds for one
+      size_t bytes = 0;
+      for (int n : {1, 2}) {
+        const size_t b = partial_bytes(tile(f.F, f.C, n, stages, npairs(), false, true), f.F, f.C, n);
+        bytes = b > bytes ? b : bytes;
+      }
+      void* partial = ws.take(bytes);
       if (!dry) {
         GemmArgs a{};
         pairs(a, o.dwg ? dg : du, both == 2 ? &du : nullptr, x, nullptr, f.M);
@@ -1389,6 +1397,11 @@ size_t ffn_ws(const FfnArgs& shape, Mode mode, int backward, int recompute) {
 #define MRAGAN_FFN_ENTRIES(name, H, TO)                                                                                       \
   size_t ffn_ws_##name(const FfnArgs& f, int planes, int pack, int backward, int recompute) {                                 \
     return ffn_ws<H, TO>(f, Mode{planes, pack != 0}, backward, recompute);                                                    \
+  }                                                                                                                           \
+  size_t ffn_bwd_bytes_##name(const FfnArgs& f, int planes, int pack, const void* dy, const void* kept, const FfnGrads& o) {  \
+    Ffn<H, TO> r(f, Mode{planes, pack != 0}, nullptr, nullptr);                                                               \
+    r.backward(dy, kept, o);                                                                                                  \
+    return r.ws.used;                                                                                                         \
   }                                                                                                                           \
   int ffn_fwd_##name(const FfnArgs& f, int planes, int pack, void* y, void* kept, void* ws, hipStream_t st) {                 \
     return Ffn<H, TO>(f, Mode{planes, pack != 0}, ws, st).forward(y, kept);                                                   \

@@ -7,6 +7,7 @@ namespace mragan {
 
 #define MRAGAN_FFN_DECLARE(name)                                                                                            \
   size_t ffn_ws_##name(const FfnArgs&, int planes, int pack, int backward, int recompute);                                  \
+  size_t ffn_bwd_bytes_##name(const FfnArgs&, int planes, int pack, const void* dy, const void* kept, const FfnGrads&);     \
   int ffn_fwd_##name(const FfnArgs&, int planes, int pack, void* y, void* kept, void* ws, hipStream_t);                     \
   int ffn_bwd_##name(const FfnArgs&, int planes, int pack, const void* dy, const void* kept, const FfnGrads&, void* ws, hipStream_t);
 MRAGAN_FFN_DECLARE(bf16)
@@ -25,6 +26,10 @@ MRAGAN_FFN_DECLARE(f32_f16)
 size_t gated_ffn_ws_bytes(const FfnArgs& f, int pmode, int backward, int recompute) {
 #define MRAGAN_FFN_WS(name, planes, pack) ffn_ws_##name(f, planes, pack, backward, recompute)
   return MRAGAN_FFN_DISPATCH(f, pmode, MRAGAN_FFN_WS);
+}
+size_t gated_ffn_bwd_bytes(const FfnArgs& f, int pmode, const void* dy, const void* kept, const FfnGrads& o) {
+#define MRAGAN_FFN_BYTES(name, planes, pack) ffn_bwd_bytes_##name(f, planes, pack, dy, kept, o)
+  return MRAGAN_FFN_DISPATCH(f, pmode, MRAGAN_FFN_BYTES);
 }
 int gated_ffn_fwd(const FfnArgs& f, int pmode, void* y, void* kept, void* ws, hipStream_t st) {
 #define MRAGAN_FFN_FWD(name, planes, pack) ffn_fwd_##name(f, planes, pack, y, kept, ws, st)

@@ -102,7 +102,7 @@ int mragan_gated_ffn_bwd(const void* x, int64_t M, int C, int F, int O, int dtyp
   if (!dx && !dw_gate && !dw_up && !dw_down && !db_gate && !db_up && !db_down) return kOk;
   const FfnArgs f{x, M, C, F, O, dtype, w_gate, w_up, w_down, b_gate, b_up, nullptr, act};
   const int mode = mragan_get_conv_precision();
-  const size_t need = gated_ffn_ws_bytes(f, mode, 1, !kept);
+  const size_t need = gated_ffn_bwd_bytes(f, mode, dy, kept, o);
   if (!ws || ws_bytes < need) {
     set_error("gated_ffn_bwd: workspace %zu < %zu bytes (query mragan_gated_ffn_workspace)", ws_bytes, need);
     return kWorkspace;

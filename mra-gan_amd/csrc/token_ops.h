@@ -33,6 +33,8 @@ struct FfnGrads {                            // each may be null
   void *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd;
 };
 size_t gated_ffn_ws_bytes(const FfnArgs& f, int pmode, int backward, int recompute);
+// what gated_ffn_bwd takes of its workspace for these gradients
+size_t gated_ffn_bwd_bytes(const FfnArgs& f, int pmode, const void* dy, const void* kept, const FfnGrads& o);
 int gated_ffn_fwd(const FfnArgs& f, int pmode, void* y, void* kept, void* ws, hipStream_t st);
 int gated_ffn_bwd(const FfnArgs& f, int pmode, const void* dy, const void* kept, const FfnGrads& o, void* ws, hipStream_t st);
 

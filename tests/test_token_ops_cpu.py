@@ -1,5 +1,8 @@
 """Token-block operators without a GPU: fake shapes of the registered ops, refusals before any launch, and
 the host side of the C entry points (argument checks, workspace sizes)."""
+import random
+import re
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -100,3 +103,31 @@ def test_workspace_sizes():
     assert query("mragan_linear_recurrence_workspace", 1, 16, 64, 0) == 0
     assert query("mragan_linear_recurrence_workspace", 1, 65536, 64, 0) > 0
     assert [query("mragan_linear_recurrence_carries", t, 8) for t in (0, 1, 128, 129)] == [0, 1, 1, 2]
+
+
+def test_gated_ffn_bwd_workspace_covers_every_subset():
+    """The queried size is enough for any choice of gradients: what each choice takes is read from the refusal of a
+    call without a workspace, which launches nothing."""
+    rng = random.Random(5)
+    size = lambda lo, hi, step: max(step, int(lo * (hi / lo) ** rng.random()) // step * step)
+    shapes = [(1024, 512, 1024, 512), (512, 512, 1024, 512), (4096, 1024, 1024, 1024), (4096, 1024, 1024, 64), (1, 1, 1, 1),
+              (16384, 2048, 8192, 2048), (257, 515, 333, 130), (3, 5, 7, 11)]
+    shapes += [(size(1, 16384, 1), *(size(8, hi, rng.choice((1, 8, 64))) for hi in (2048, 8192, 2048))) for _ in range(72)]
+    short = []
+    try:
+        for dtype, mode in ((1, "f32"), (2, "f32"), (0, "f32"), (0, "bf16x3"), (0, "bf16"), (0, "fp16")):
+            ops.set_conv_precision(mode)
+            for M, C, F, O in shapes:
+                for kept in (None, 5 * P):
+                    have = query("mragan_gated_ffn_workspace", M, C, F, O, dtype, 1, int(kept is None))
+                    for need in range(1, 128):
+                        grads = [P if need >> k & 1 else None for k in range(7)]
+                        with pytest.raises(MraganError, match="workspace") as e:
+                            call("mragan_gated_ffn_bwd", P, M, C, F, O, dtype, P, 2 * P, 3 * P, None, None, 5, 4 * P, kept, *grads,
+                                 None, 0, None)
+                        takes = int(re.search(r"workspace 0 < (\d+) bytes", str(e.value)).group(1))
+                        if takes > have:
+                            short.append((dtype, mode, M, C, F, O, kept is None, need, takes - have))
+    finally:
+        ops.set_conv_precision("f32")
+    assert not short, (len(short), short[:5])

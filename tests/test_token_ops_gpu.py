@@ -671,3 +671,39 @@ def test_linear_recurrence_last_channels(ops, size, dtype):
     x, d, z, h0, dy, dlast = recurrence_inputs(*size, dtype)
     check_recurrence(ops, x, d, z, h0, dy, dlast, False)
     check_recurrence(ops, x, d, None, h0, dy, dlast, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("frozen", ["gate", "up"])
+@pytest.mark.parametrize("size", [(1024, 512, 1024, 512), (512, 512, 1024, 512), (1000, 136, 1032, 40)])
+def test_gated_ffn_one_frozen_weight(ops, size, frozen, dtype):
+    """One of the two projections without a gradient, whose product alone splits where the two together do not: its
+    gradients, and nothing behind a workspace of the queried size."""
+    need = tuple(k != (1 if frozen == "gate" else 2) for k in range(7))
+    a, b, dy = ffn_inputs(*size, dtype)
+    check_ffn(ops, a, b, dy, "silu", need=need)
+    check_ffn(ops, a, b, dy, "silu", need=need, keep=False)
+    from mragan_hip._lib import call, query
+    M, C, F, O = size
+    code = DTYPES.index(dtype)
+    nbytes = query("mragan_gated_ffn_workspace", M, C, F, O, code, 1, 1)
+    ws = torch.full((nbytes + (64 << 20),), 0xA5, dtype=torch.uint8, device="cuda")
+    grads = [torch.empty_like(t) if n else None for t, n in zip([*a, *b], need)]
+    p = lambda t: None if t is None else t.data_ptr()
+    call("mragan_gated_ffn_bwd", p(a[0]), M, C, F, O, code, *map(p, a[1:]), p(b[0]), p(b[1]), 5, p(dy), None, *map(p, grads),
+         p(ws), nbytes, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert bool((ws[nbytes:] == 0xA5).all())
+    for got, want in zip(grads, ops.gated_ffn_bwd(*a, dy, None, *b, need=need)):
+        assert got is want is None or torch.equal(got, want)
+
+
+def test_gated_ffn_frozen_weight_registered(ops):
+    a, b, dy = ffn_inputs(1024, 512, 1024, 512, torch.bfloat16)
+    for k, t in enumerate(a):
+        t.requires_grad_(k != 2)
+    y = torch.ops.mragan.gated_ffn(*a, *b, "silu", True)[0]
+    got = torch.autograd.grad(y, [a[0], a[1], a[3]], dy)
+    _, kept = ops.gated_ffn_fwd(*a, *b, keep=True)
+    want = ops.gated_ffn_bwd(*a, dy, kept, *b, need=(True, True, False, True) + (False,) * 3)
+    assert all(torch.equal(g, w) for g, w in zip(got, (want[0], want[1], want[3])))
