@@ -131,3 +131,18 @@ def test_gated_ffn_bwd_workspace_covers_every_subset():
     finally:
         ops.set_conv_precision("f32")
     assert not short, (len(short), short[:5])
+
+
+def test_single_position_has_no_time_stride():
+    """A position of a time-major tensor: torch calls it contiguous whatever the stride of its only step."""
+    big = torch.empty(3, 1024, 4096, dtype=torch.bfloat16, device="meta")
+    x = big[1:2].transpose(0, 1)
+    assert x.stride() == (4096, 1024 * 4096, 1) and x.is_contiguous()
+    t, sb, st = ops._sequence(x, "x", x)
+    assert t is x and sb == 4096 and 0 <= st < 1 << 22
+    for st in (1 << 40, -8):                                  # past the strides' check: the next one refuses
+        with pytest.raises(MraganError, match="null pointer"):
+            call("mragan_linear_recurrence_fwd", P, 8, st, P, 8, st, P, 8, st, None, 1, 1, 8, 0, 0, None, None, None, None, 0, None)
+        with pytest.raises(MraganError, match="without a gate"):
+            call("mragan_linear_recurrence_bwd", P, 8, st, P, 8, st, None, 0, st, P, P, 8, st, None, 1, 1, 8, 0, 0, P, P, P, P, None, 0,
+                 None)

@@ -707,3 +707,11 @@ def test_gated_ffn_frozen_weight_registered(ops):
     _, kept = ops.gated_ffn_fwd(*a, *b, keep=True)
     want = ops.gated_ffn_bwd(*a, dy, kept, *b, need=(True, True, False, True) + (False,) * 3)
     assert all(torch.equal(g, w) for g, w in zip(got, (want[0], want[1], want[3])))
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_linear_recurrence_position_of_time_major(ops, reverse):
+    """One position of [T, B, C] tensors whose steps are 2^22 elements apart."""
+    seqs = [randn(k, 3, 1024, 4096, dtype=torch.bfloat16) for k in range(4)]
+    x, d, z, dy = (t[1:2].transpose(0, 1) for t in seqs)
+    check_recurrence(ops, x, d, z, randn(4, 1024, 4096), dy, randn(5, 1024, 4096), reverse)
