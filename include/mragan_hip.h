@@ -447,8 +447,8 @@ int mragan_gated_ffn_bwd(const void* x, int64_t M, int C, int F, int O, int dtyp
  *   a_t = σ(decay_t),  h_t = a_t·h_{t−1} + σ(−decay_t)·x_t,  y_t = h_t·silu(gate_t)   (y = h: gate NULL)
  * from h_{−1} = h0 ([B][C] fp32, NULL = 0), or from the last position to the first with reverse = 1.
  * x, decay, gate, dy: element (b, t, c) at b·stride_b + t·stride_t + c (strides in elements, slices
- * of one projection or expanded tensors; stride_t and C below 2²²; with T = 1 stride_t has no
- * meaning); y, dx, ddecay, dgate: contiguous [B][T][C].
+ * of one projection or expanded tensors; C below 2²⁵, stride_t C or below 2²²; with T = 1 it
+ * has no meaning); y, dx, ddecay, dgate: contiguous [B][T][C].
  * last [B][C] fp32: the state after the last step.  carry [B][mragan_linear_recurrence_carries(T, C)][C]
  * fp32: states at fixed steps that the backward restarts from (NULL in an inference call).
  * decay = +inf leaves the state as it is (a padded position), −inf restarts from x_t; x and h

@@ -116,8 +116,11 @@ size_t mragan_linear_recurrence_workspace(int64_t B, int64_t T, int C, int backw
   return C > 0 ? recurrence_ws_bytes(B, T, C) : 0;
 }
 
-// time strides whose offsets inside a chunk of 128 steps stay below 2³² bytes; a single step has none
-static bool time_stride_ok(int64_t T, int64_t st) { return T == 1 || (st >= 0 && st < ((int64_t)1 << 22)); }
+// Channels of a recurrence, exclusive: a lane's offset in its chunk, up to 120 rows and a tile of 64 channels,
+// stays below 2³² elements.
+constexpr int64_t kMaxRecurChannels = (int64_t)1 << 25;
+// Time strides: rows that follow each other, or less than 2²² apart.  A single step has none.
+static bool time_stride_ok(int64_t T, int64_t st, int C) { return T == 1 || st == C || (st >= 0 && st < ((int64_t)1 << 22)); }
 
 static int recur_check(const RecurArgs& r, const void* ws, size_t ws_bytes) {
   MRAGAN_CHECK_ARG(r.B >= 0 && r.T > 0 && r.C > 0, "linear_recurrence: bad shape [%lld][%lld][%d]", (long long)r.B,
@@ -126,8 +129,9 @@ static int recur_check(const RecurArgs& r, const void* ws, size_t ws_bytes) {
   MRAGAN_CHECK_ARG(r.reverse == 0 || r.reverse == 1, "linear_recurrence: reverse must be 0/1");
   if (r.B == 0) return kOk;
   MRAGAN_CHECK_ARG(r.x && r.decay, "linear_recurrence: null pointer");
-  MRAGAN_CHECK_ARG(time_stride_ok(r.T, r.x_st) && time_stride_ok(r.T, r.d_st) && time_stride_ok(r.T, r.g_st) && time_stride_ok(2, r.C),
-                   "linear_recurrence: time strides and C must be in [0, 2^22)");
+  MRAGAN_CHECK_ARG(r.C < kMaxRecurChannels && time_stride_ok(r.T, r.x_st, r.C) && time_stride_ok(r.T, r.d_st, r.C) &&
+                       (!r.gate || time_stride_ok(r.T, r.g_st, r.C)),
+                   "linear_recurrence: C must be below 2^25, time strides C or in [0, 2^22)");
   MRAGAN_CHECK_ARG(r.B <= kMaxThreads && recurrence_threads(r.B, r.T, r.C) < kMaxThreads, "linear_recurrence: too many sequences");
   const size_t need = recurrence_ws_bytes(r.B, r.T, r.C);
   if (need && (!ws || ws_bytes < need)) {
@@ -157,7 +161,7 @@ int mragan_linear_recurrence_bwd(const void* x, int64_t x_sb, int64_t x_st, cons
   if (int rc = recur_check(r, ws, ws_bytes)) return rc;
   if (B == 0 || (!dx && !ddecay && !dgate && !dh0)) return kOk;
   MRAGAN_CHECK_ARG(carry && dy, "linear_recurrence_bwd: null pointer");
-  MRAGAN_CHECK_ARG(time_stride_ok(T, dy_st), "linear_recurrence_bwd: time strides must be in [0, 2^22)");
+  MRAGAN_CHECK_ARG(time_stride_ok(T, dy_st, C), "linear_recurrence_bwd: time strides must be C or in [0, 2^22)");
   MRAGAN_CHECK_ARG(gate || !dgate, "linear_recurrence_bwd: dgate without a gate");
   return recurrence_bwd(r, carry, dy, dy_sb, dy_st, dlast, dx, ddecay, dgate, dh0, static_cast<float*>(ws),
                         static_cast<hipStream_t>(stream));

@@ -1281,7 +1281,7 @@ def gated_ffn_bwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_d
 
 def _sequence(t: Optional[torch.Tensor], name: str, ref: torch.Tensor):
     """(tensor, batch stride, time stride): t as it is where its channels are contiguous and its time stride
-    is one the library takes (below 2^22 elements), else a copy.  A single position has no time stride: torch
+    is one the library takes (below 2^22 elements, or the rows follow each other), else a copy.  A single position has no time stride: torch
     leaves any number there."""
     if t is None:
         return None, 0, 0
@@ -1290,7 +1290,7 @@ def _sequence(t: Optional[torch.Tensor], name: str, ref: torch.Tensor):
         if t.shape[2] > 1 and t.stride(2) != 1:
             t = t.contiguous()
         return t, t.stride(0), 0
-    if (t.shape[2] > 1 and t.stride(2) != 1) or t.stride(1) >= 1 << 22:
+    if (t.shape[2] > 1 and t.stride(2) != 1) or (t.stride(1) >= 1 << 22 and t.stride(1) != t.shape[2]):
         t = t.contiguous()
     return t, t.stride(0), t.stride(1)
 

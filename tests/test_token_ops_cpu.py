@@ -146,3 +146,25 @@ def test_single_position_has_no_time_stride():
         with pytest.raises(MraganError, match="without a gate"):
             call("mragan_linear_recurrence_bwd", P, 8, st, P, 8, st, None, 0, st, P, P, 8, st, None, 1, 1, 8, 0, 0, P, P, P, P, None, 0,
                  None)
+
+
+def test_recurrence_rows_up_to_2_25():
+    """A scan along the depth of a volume has H·W·C channels: 2^22 of them are a 256 x 256 plane of 64.  The first two
+    calls pass the strides' check and are refused by the next one."""
+    for C in (1 << 22, (1 << 25) - 1):
+        with pytest.raises(MraganError, match="null pointer"):
+            call("mragan_linear_recurrence_fwd", P, 0, C, P, 0, C, P, 0, C, None, 1, 40, C, 0, 0, None, None, None, P, 1 << 50, None)
+        with pytest.raises(MraganError, match="without a gate"):
+            call("mragan_linear_recurrence_bwd", P, 0, C, P, 0, C, None, 0, 0, P, P, 0, C, None, 1, 40, C, 0, 0, P, P, P, P, P, 1 << 50,
+                 None)
+        with pytest.raises(MraganError, match="time strides"):
+            call("mragan_linear_recurrence_fwd", P, 0, C, P, 0, 3 * C, P, 0, C, None, 1, 40, C, 0, 0, P, P, P, P, 1 << 50, None)
+    for T in (1, 40):
+        with pytest.raises(MraganError, match="time strides"):
+            call("mragan_linear_recurrence_fwd", P, 0, 1 << 25, P, 0, 1 << 25, P, 0, 1 << 25, None, 1, T, 1 << 25, 0, 0, P, P, P, P,
+                 1 << 50, None)
+    rows = torch.empty(2, 40, 1 << 22, dtype=torch.bfloat16, device="meta")
+    t, sb, st = ops._sequence(rows, "x", rows)
+    assert t is rows and (sb, st) == (40 << 22, 1 << 22)
+    part = torch.empty(2, 40, 3 << 22, dtype=torch.bfloat16, device="meta")[..., :1 << 22]
+    assert ops._sequence(part, "x", rows)[1:] == (40 << 22, 1 << 22)

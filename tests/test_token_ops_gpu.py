@@ -715,3 +715,29 @@ def test_linear_recurrence_position_of_time_major(ops, reverse):
     seqs = [randn(k, 3, 1024, 4096, dtype=torch.bfloat16) for k in range(4)]
     x, d, z, dy = (t[1:2].transpose(0, 1) for t in seqs)
     check_recurrence(ops, x, d, z, randn(4, 1024, 4096), dy, randn(5, 1024, 4096), reverse)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("T,C,dtype", [(9, 1 << 22, torch.float32), (17, 256 * 256 * 64, torch.bfloat16), (130, (1 << 23) + 70, torch.float16)])
+def test_linear_recurrence_wide_rows(ops, T, C, dtype, reverse):
+    """Scans along the depth of wide volumes, tensors of more than 2^31 bytes among them; channels do not mix, so the
+    first and the last ones are compared."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    new = lambda *s, t=dtype, shift=0.0: torch.empty(s, dtype=t, device="cuda").normal_(shift, 1.0, generator=gen)
+    x, d, z, dy = new(1, T, C), new(1, T, C, shift=2.0), new(1, T, C), new(1, T, C)
+    h0, dlast = new(1, C, t=torch.float32), new(1, C, t=torch.float32)
+
+    class Part:
+        """The operator on whole rows, seen through some of their channels."""
+        sel = None
+
+        def linear_recurrence_fwd(self, *_, reverse):
+            y, last, self.carry = ops.linear_recurrence_fwd(x, d, z, h0, reverse=reverse)
+            return y[..., self.sel], last[..., self.sel], None
+
+        def linear_recurrence_bwd(self, *_, reverse):
+            return [t[..., self.sel] for t in ops.linear_recurrence_bwd(x, d, self.carry, dy, z, dlast, reverse=reverse)]
+
+    part = Part()
+    for part.sel in (slice(0, 66), slice(C - 131, C)):
+        check_recurrence(part, *(t[..., part.sel] for t in (x, d, z, h0, dy, dlast)), reverse)
