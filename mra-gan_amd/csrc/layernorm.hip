@@ -261,28 +261,33 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(con
   }
 }
 
-// Σ over the nb blocks' partials: a block takes 32 of the 2C columns with 32 threads each
+// Σ over the nb blocks' partials: a block takes 32 of the 2C columns with 32 threads each, then the next
+// 32 behind those of the launch's other blocks
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* part, int nb, int C, W* dw, W* db) {
   __shared__ float s[32][33];
   const int cl = threadIdx.x & 31, slot = threadIdx.x >> 5;
-  const int64_t col = (int64_t)blockIdx.x * 32 + cl, n = 2 * (int64_t)C;
-  float v = 0.f;
-  if (col < n) {
+  const int64_t n = 2 * (int64_t)C, step = (int64_t)gridDim.x * 32;
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < n; c0 += step) {
+    const int64_t col = c0 + cl;
+    float v = 0.f;
+    if (col < n) {
 #pragma unroll 8
-    for (int k = slot; k < nb; k += 32) v += part[k * n + col];
-  }
-  s[slot][cl] = v;
-  __syncthreads();
-  if (slot == 0 && col < n) {
-    v = 0.f;
-#pragma unroll
-    for (int k = 0; k < 32; k++) v += s[k][cl];
-    if (col < C) {
-      if (dw) dw[col] = (W)v;
-    } else if (db) {
-      db[col - C] = (W)v;
+      for (int k = slot; k < nb; k += 32) v += part[k * n + col];
     }
+    s[slot][cl] = v;
+    __syncthreads();
+    if (slot == 0 && col < n) {
+      v = 0.f;
+#pragma unroll
+      for (int k = 0; k < 32; k++) v += s[k][cl];
+      if (col < C) {
+        if (dw) dw[col] = (W)v;
+      } else if (db) {
+        db[col - C] = (W)v;
+      }
+    }
+    if (c0 + step < n) __syncthreads();                                // s is read before the next columns write it
   }
 }
 
@@ -353,8 +358,9 @@ __global__ __launch_bounds__(256) void ln_param_long_kernel(const T* x, const fl
 // The largest row that a block holds: 16 channels a thread of 512 (backward: their 256 registers also
 // carry the next row, the weight and two accumulators), 32 a thread of 256 (forward).
 constexpr int kMaxRow = 8192;
-// blocks of the longer rows' kernels: a launch takes fewer than 2^32 threads
-unsigned long_grid(int64_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
+// A launch takes fewer than 2^32 threads, and says nothing of more (it leaves some of its blocks out): at most
+// 2^16 blocks of 1024, of the longer rows' kernels and of the parameter sums
+unsigned bounded_grid(int64_t blocks) { return (unsigned)(blocks < 65536 ? blocks : 65536); }
 // Most blocks of a backward launch: four on each of the 256 CUs, whose partial sums the second launch reads
 constexpr int kMaxBwdBlocks = 1024;
 
@@ -384,7 +390,7 @@ int ln_fwd(const void* x, int64_t rows, int C, const void* w, const void* b, flo
   const W *wt = static_cast<const W*>(w), *bt = static_cast<const W*>(b);
   T* yt = static_cast<T*>(y);
   if (C > kMaxRow) {
-    ln_fwd_long_kernel<T, W><<<long_grid(rows), 1024, 0, st>>>(xt, rows, C, wt, bt, eps, yt, mean, rstd);
+    ln_fwd_long_kernel<T, W><<<bounded_grid(rows), 1024, 0, st>>>(xt, rows, C, wt, bt, eps, yt, mean, rstd);
     return check_launch("layer_norm_fwd_long");
   }
   // bf16, 2048 channels: 64 rows take 2.6 us with a block each, 3.3 with a wave; 1024 channels: 256 rows
@@ -443,7 +449,7 @@ int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, 
   const bool params = dw || db;
   if (C > kMaxRow) {
     if (dx) {
-      ln_bwd_long_kernel<T, W><<<long_grid(rows), 1024, 0, st>>>(xt, mean, rstd, dyt, rows, C, wt, dxt);
+      ln_bwd_long_kernel<T, W><<<bounded_grid(rows), 1024, 0, st>>>(xt, mean, rstd, dyt, rows, C, wt, dxt);
       if (int rc = check_launch("layer_norm_bwd_long")) return rc;
     }
     if (!params) return kOk;
@@ -451,7 +457,7 @@ int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, 
     ln_param_long_kernel<T><<<dim3(ceil_div(C, 256), chunks), 256, 0, st>>>(xt, mean, rstd, dyt, rows, (rows + chunks - 1) / chunks, C,
                                                                             part);
     if (int rc = check_launch("layer_norm_param_long")) return rc;
-    ln_param_reduce_kernel<W><<<ceil_div(2 * (int64_t)C, 32), 1024, 0, st>>>(part, chunks, C, dwt, dbt);
+    ln_param_reduce_kernel<W><<<bounded_grid(ceil_div(2 * (int64_t)C, 32)), 1024, 0, st>>>(part, chunks, C, dwt, dbt);
     return check_launch("layer_norm_param_reduce");
   }
   const Shape s = bwd_shape(C, N);
@@ -478,7 +484,7 @@ int ln_bwd(const void* x, const float* mean, const float* rstd, const void* dy, 
 #undef LN_END
   if (rc) return rc;
   if (params) {
-    ln_param_reduce_kernel<W><<<ceil_div(2 * (int64_t)C, 32), 1024, 0, st>>>(part, (int)grid, C, dwt, dbt);
+    ln_param_reduce_kernel<W><<<bounded_grid(ceil_div(2 * (int64_t)C, 32)), 1024, 0, st>>>(part, (int)grid, C, dwt, dbt);
     return check_launch("layer_norm_param_reduce");
   }
   return kOk;

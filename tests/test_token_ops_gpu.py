@@ -741,3 +741,12 @@ def test_linear_recurrence_wide_rows(ops, T, C, dtype, reverse):
     part = Part()
     for part.sel in (slice(0, 66), slice(C - 131, C)):
         check_recurrence(part, *(t[..., part.sel] for t in (x, d, z, h0, dy, dlast)), reverse)
+
+
+def test_layer_norm_longest_rows(ops):
+    """Rows of 2^26 channels, whose parameter sums have more columns than one launch has threads for at 64 a column.
+    Bounds as in check_norm, with the additions that one of a block's 1024 threads makes."""
+    rows, C = 2, (1 << 26) + 5
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    new = lambda *s: torch.empty(s, dtype=torch.bfloat16, device="cuda").normal_(0.5, 1.0, generator=gen)
+    check_norm(ops, new(rows, C), new(C), new(C), dy=new(rows, C))
