@@ -73,8 +73,9 @@ __device__ __forceinline__ void split_planes(float v, int planes, H (&out)[3]) {
 }
 
 // src [R][K] (any type) → 16-bit planes dst [planes][R][ld], zeros from K to ld; several tensors a launch,
-// kPackQuads groups of four elements a block
-constexpr int kPackQuads = 1024, kMaxPacks = 8;
+// kPackQuads groups of four elements a block and pass.  At most kPackBlocks blocks: a launch of 2^32 threads and
+// more would leave some out without a word.
+constexpr int kPackQuads = 1024, kMaxPacks = 8, kPackBlocks = 65536;
 struct PackJob {
   const void* src;
   void* dst;
@@ -84,40 +85,43 @@ struct PackJob {
 struct PackArgs {
   PackJob job[kMaxPacks];
   int jobs, planes;
+  int64_t blocks;                 // of all jobs
 };
 template <typename T, typename H>
 __global__ __launch_bounds__(256) void ffn_pack_kernel(const PackArgs a) {
-  int j = 0;
-  while (j + 1 < a.jobs && blockIdx.x >= a.job[j + 1].first) j++;
-  const PackJob& q = a.job[j];
-  const T* src = static_cast<const T*>(q.src);
-  const int64_t quads = q.ld / 4, total = q.R * quads, plane = q.R * q.ld, i0 = (blockIdx.x - q.first) * kPackQuads;
+  for (int64_t block = blockIdx.x; block < a.blocks; block += gridDim.x) {
+    int j = 0;
+    while (j + 1 < a.jobs && block >= a.job[j + 1].first) j++;
+    const PackJob& q = a.job[j];
+    const T* src = static_cast<const T*>(q.src);
+    const int64_t quads = q.ld / 4, total = q.R * quads, plane = q.R * q.ld, i0 = (block - q.first) * kPackQuads;
 #pragma unroll
-  for (int n = 0; n < kPackQuads / 256; n++) {
-    const int64_t i = i0 + n * 256 + threadIdx.x;
-    if (i >= total) break;
-    const int64_t r = total >> 32 ? i / quads : (uint32_t)i / (uint32_t)quads, k = (i - r * quads) * 4;
-    float v[4];
-    if (k + 4 <= q.K) {                                              // of any alignment where K is odd
-      T t[4];
-      __builtin_memcpy(t, src + r * q.K + k, sizeof(t));
+    for (int n = 0; n < kPackQuads / 256; n++) {
+      const int64_t i = i0 + n * 256 + threadIdx.x;
+      if (i >= total) break;
+      const int64_t r = total >> 32 ? i / quads : (uint32_t)i / (uint32_t)quads, k = (i - r * quads) * 4;
+      float v[4];
+      if (k + 4 <= q.K) {                                              // of any alignment where K is odd
+        T t[4];
+        __builtin_memcpy(t, src + r * q.K + k, sizeof(t));
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = (float)t[e];
-    } else {
+        for (int e = 0; e < 4; e++) v[e] = (float)t[e];
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = k + e < q.K ? (float)src[r * q.K + k + e] : 0.f;
-    }
-    H w[4][3];
-#pragma unroll
-    for (int e = 0; e < 4; e++) split_planes<H>(v[e], a.planes, w[e]);
-#pragma unroll
-    for (int p = 0; p < 3; p++)
-      if (p < a.planes) {
-        Pack<H, 4> o;
-#pragma unroll
-        for (int e = 0; e < 4; e++) o.v[e] = w[e][p];
-        *reinterpret_cast<Pack<H, 4>*>(static_cast<H*>(q.dst) + p * plane + r * q.ld + k) = o;
+        for (int e = 0; e < 4; e++) v[e] = k + e < q.K ? (float)src[r * q.K + k + e] : 0.f;
       }
+      H w[4][3];
+#pragma unroll
+      for (int e = 0; e < 4; e++) split_planes<H>(v[e], a.planes, w[e]);
+#pragma unroll
+      for (int p = 0; p < 3; p++)
+        if (p < a.planes) {
+          Pack<H, 4> o;
+#pragma unroll
+          for (int e = 0; e < 4; e++) o.v[e] = w[e][p];
+          *reinterpret_cast<Pack<H, 4>*>(static_cast<H*>(q.dst) + p * plane + r * q.ld + k) = o;
+        }
+    }
   }
 }
 
@@ -1122,8 +1126,8 @@ struct Ffn {
     const int64_t blocks = pack_blocks;
     packs.jobs = 0, pack_blocks = 0;
     if (!n || dry) return kOk;
-    const PackArgs a = [&] { PackArgs c = packs; c.jobs = n; return c; }();
-    ffn_pack_kernel<TO, H><<<(unsigned)blocks, 256, 0, st>>>(a);
+    const PackArgs a = [&] { PackArgs c = packs; c.jobs = n, c.blocks = blocks; return c; }();
+    ffn_pack_kernel<TO, H><<<(unsigned)(blocks < kPackBlocks ? blocks : kPackBlocks), 256, 0, st>>>(a);
     return check_launch("ffn_pack");
   }
 

@@ -750,3 +750,13 @@ def test_layer_norm_longest_rows(ops):
     gen = torch.Generator(device="cuda").manual_seed(1)
     new = lambda *s: torch.empty(s, dtype=torch.bfloat16, device="cuda").normal_(0.5, 1.0, generator=gen)
     check_norm(ops, new(rows, C), new(C), new(C), dy=new(rows, C))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_gated_ffn_more_packed_rows_than_blocks(ops, dtype):
+    """Rows of odd length whose padded copy is longer than one pass of its launch (2^28 elements)."""
+    M, C, F, O = (1 << 20) + 77, 201, 8, 9
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    new = lambda *s, k=1: (torch.empty(s, device="cuda").normal_(generator=gen) * k ** -0.5).to(dtype)
+    a = [new(M, C), new(F, C, k=C), new(F, C, k=C), new(O, F, k=F)]
+    check_ffn(ops, a, [new(F), new(F), new(O)], new(M, O), "silu")
