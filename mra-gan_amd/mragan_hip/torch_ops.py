@@ -30,6 +30,7 @@ they need the process-wide loss scale at 1 (ops.set_loss_scale), which they chec
 """
 from __future__ import annotations
 
+import functools
 from typing import List, Optional, Tuple
 
 import torch
@@ -276,6 +277,37 @@ def _(param, grad, exp_avg, exp_avg_sq, lr, beta1, beta2, eps, step, grad_scale)
     return None
 
 
+class _FirstOrder(torch.autograd.Function):
+    """Gradients that a further backward may not pass."""
+
+    @staticmethod
+    def forward(ctx, name, *grads):
+        ctx.name = name
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"mragan::{ctx.name} has no second derivative")
+
+
+def _first_order(name):
+    """The gradients come from kernels that autograd does not see into: under create_graph a second backward would
+    take them for constants, so it raises instead."""
+    def mark(backward):
+        @functools.wraps(backward)
+        def wrapper(ctx, *grads):
+            again = torch.is_grad_enabled()
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            if not again:
+                return out
+            there = [t.requires_grad_() for t in out if t is not None]
+            marked = iter(_FirstOrder.apply(name, *there) if there else ())
+            return tuple(None if t is None else next(marked) for t in out)
+        return wrapper
+    return mark
+
+
 @torch.library.custom_op("mragan::layer_norm", mutates_args=(), device_types="cuda")
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
                eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -297,6 +329,7 @@ def _ln_setup(ctx, inputs, output):
     ctx.mark_non_differentiable(mean, rstd)
 
 
+@_first_order("layer_norm")
 def _ln_backward(ctx, dy, _dmean, _drstd):
     x, weight, mean, rstd = ctx.saved_tensors
     return ops.layer_norm_bwd(x, mean, rstd, dy, weight, bias=ctx.bias) + (None,)
@@ -328,6 +361,7 @@ def _ffn_setup(ctx, inputs, output):
     ctx.mark_non_differentiable(output[1])
 
 
+@_first_order("gated_ffn")
 def _ffn_backward(ctx, dy, _dkept):
     x, wg, wu, wd, bg, bu, bd, kept = ctx.saved_tensors
     return ops.gated_ffn_bwd(x, wg, wu, wd, dy, kept, bg, bu, bd, ctx.act, need=ctx.needs_input_grad[:7]) + (None, None)
@@ -357,6 +391,7 @@ def _recur_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)                   # an unused output has no gradient
 
 
+@_first_order("linear_recurrence")
 def _recur_backward(ctx, dy, dlast, _dcarry):
     x, decay, gate, carry = ctx.saved_tensors
     if dy is None:

@@ -760,3 +760,23 @@ def test_gated_ffn_more_packed_rows_than_blocks(ops, dtype):
     new = lambda *s, k=1: (torch.empty(s, device="cuda").normal_(generator=gen) * k ** -0.5).to(dtype)
     a = [new(M, C), new(F, C, k=C), new(F, C, k=C), new(O, F, k=F)]
     check_ffn(ops, a, [new(F), new(F), new(O)], new(M, O), "silu")
+
+
+def test_second_derivatives_refused(ops):
+    """A gradient penalty through one of the operators raises where it would need their second derivative; the first
+    one is the same with create_graph as without."""
+    m = torch.ops.mragan
+    a, b, _ = ffn_inputs(9, 24, 40, 16, torch.float32)
+    r = recurrence_inputs(2, 20, 12, torch.float32)
+    for x, fn in ((randn(1, 6, 40), lambda t: m.layer_norm(t, randn(2, 40), None, 1e-5)[0]),
+                  (a[0], lambda t: m.gated_ffn(t, *a[1:], *b, "silu", True)[0]),
+                  (a[0], lambda t: m.gated_ffn(t, *a[1:], *b, "silu", False)[0]),
+                  (r[0], lambda t: m.linear_recurrence(t, *r[1:4], False)[0]),
+                  (r[0], lambda t: m.linear_recurrence(t, *r[1:4], False)[1])):
+        x = x.clone().requires_grad_()
+        y = fn(x)
+        want = torch.autograd.grad(y.square().sum(), x, retain_graph=True)[0]
+        (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        assert torch.equal(g.detach(), want)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (y.sum() + g.square().sum()).backward()
