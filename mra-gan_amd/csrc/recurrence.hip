@@ -20,8 +20,15 @@
 // twice, 34 MB written) and 16 + 33 us backward.
 #include "token_ops.h"
 
+// A channel may be formed in either slot of a lane, by lanes moved back beside its own (see place), and on a
+// guarded or a whole path.  Its bits have to be the same in each, so the compiler joins no product and sum by
+// itself: where one rounding is meant for both, the code says fma.
+#pragma clang fp contract(off)
+
 namespace mragan {
 namespace {
+
+__device__ __forceinline__ float fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 
 constexpr int kVC = 2;                    // channels a lane
 constexpr int kS = 8;                     // steps of a time lane
@@ -69,7 +76,7 @@ __device__ __forceinline__ float silu(float z) { return z * __builtin_amdgcn_rcp
 __device__ __forceinline__ void silu_pair(float z, float& f, float& df) {
   const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
   f = z * s;
-  df = s * (1.f + z * (1.f - s));
+  df = s * fma(z, 1.f - s, 1.f);
 }
 
 template <bool V>
@@ -215,8 +222,8 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_segment_kernel(Stri
             float a, i;
             sigmoid_pair(qd[w].get(v), a, i);
             const float in = qe[w].get(v);
-            if constexpr (BWD) E[v] = a * (E[v] + (zp ? in * silu(qz[w].get(v)) : in));
-            else E[v] = a * E[v] + i * in;
+            if constexpr (BWD) E[v] = a * (zp ? fma(in, silu(qz[w].get(v)), E[v]) : E[v] + in);
+            else E[v] = fma(a, E[v], i * in);
             P[v] *= a;
           }
         }
@@ -231,7 +238,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_segment_kernel(Stri
 #pragma unroll
     for (int j = 0; j < kLT; j++) {
       const int l = BWD ? kLT - 1 - j : j;
-      s = sP[l][ch] * s + sE[l][ch];
+      s = fma(sP[l][ch], s, sE[l][ch]);
       m *= sP[l][ch];
     }
     float* out = agg + ((p.b * g.segs + p.seg) * 2) * g.C + p.channel(ch);
@@ -260,7 +267,7 @@ __device__ __forceinline__ void enter(const float* s0, const float* agg, const G
     for (int j = j0; j < j1; j++) {
       const int64_t o = 2 * (int64_t)(BWD ? cnt - 1 - j : j) * g.C;
       const float pj = q[o], ej = q[o + g.C];
-      s = pj * s + ej;
+      s = fma(pj, s, ej);
       m *= pj;
     }
   }
@@ -270,7 +277,7 @@ __device__ __forceinline__ void enter(const float* s0, const float* agg, const G
 #pragma unroll
   for (int w = 0; w < kParts; w++)
 #pragma unroll
-    for (int v = 0; v < kVC; v++) state[v] = fP[w][p.cl + v] * state[v] + fE[w][p.cl + v];
+    for (int v = 0; v < kVC; v++) state[v] = fma(fP[w][p.cl + v], state[v], fE[w][p.cl + v]);
 }
 
 // ---- forward ----------------------------------------------------------------------------------
@@ -306,7 +313,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_fwd_kernel(Strided<
       for (int v = 0; v < kVC; v++) {
         sigmoid_pair(n.d[s].get(v), A[s][v], I[s][v]);
         I[s][v] *= n.x[s].get(v);
-        E[v] = A[s][v] * E[v] + I[s][v];
+        E[v] = fma(A[s][v], E[v], I[s][v]);
         P[v] *= A[s][v];
         if constexpr (GATE) F[s][v] = n.z[s].get(v);
       }
@@ -320,13 +327,13 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_fwd_kernel(Strided<
         rows16(P[v], Pa[v], Ph);
         rows16(E[v], Ea[v], Eh);
         P[v] = Pa[v] * Ph;
-        E[v] = Ph * Ea[v] + Eh;
+        E[v] = fma(Ph, Ea[v], Eh);
       }
       halves(P[v], Pl[v], Ph);
       halves(E[v], El[v], Eh);
       if (threadIdx.x % 64 < LC) {
         sP[par][p.wave][p.cl + v] = Pl[v] * Ph;
-        sE[par][p.wave][p.cl + v] = Ph * El[v] + Eh;
+        sE[par][p.wave][p.cl + v] = fma(Ph, El[v], Eh);
       }
     }
     __syncthreads();
@@ -341,13 +348,13 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_fwd_kernel(Strided<
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
         if (w == p.wave) h[v] = state[v];
-        state[v] = sP[par][w][p.cl + v] * state[v] + sE[par][w][p.cl + v];
+        state[v] = fma(sP[par][w][p.cl + v], state[v], sE[par][w][p.cl + v]);
       }
     }
 #pragma unroll
     for (int v = 0; v < kVC; v++) {
-      h[v] = p.half ? Pl[v] * h[v] + El[v] : h[v];
-      if constexpr (LC == 16) h[v] = p.odd ? Pa[v] * h[v] + Ea[v] : h[v];
+      h[v] = p.half ? fma(Pl[v], h[v], El[v]) : h[v];
+      if constexpr (LC == 16) h[v] = p.odd ? fma(Pa[v], h[v], Ea[v]) : h[v];
     }
     const Steps<T> at(y, g.T * g.C, g.C, g, p, k);
 #pragma unroll
@@ -355,7 +362,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_fwd_kernel(Strided<
       Words<T, kVC> o;
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        h[v] = A[s][v] * h[v] + I[s][v];
+        h[v] = fma(A[s][v], h[v], I[s][v]);
         o.set(v, GATE ? h[v] * silu(F[s][v]) : h[v]);
       }
       store_step<W>(at, g, p, k, s, o);
@@ -425,7 +432,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_bwd_kernel(Strided<
         float a, i;
         sigmoid_pair(n.d[s].get(v), a, i);
         if constexpr (kHold) A[s][v] = a, I[s][v] = i;
-        E[v] = a * E[v] + i * n.x[s].get(v);
+        E[v] = fma(a, E[v], i * n.x[s].get(v));
         P[v] *= a;
         const float g_out = n.y[s].get(v);
         if constexpr (GATE) {
@@ -456,16 +463,16 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_bwd_kernel(Strided<
         rows16(E[v], Ea[v], Eh);
         rows16(Q[v], Ql, Qb[v]);
         P[v] = Pa[v] * Pb[v];
-        E[v] = Pb[v] * Ea[v] + Eh;
-        Q[v] = Pa[v] * Qb[v] + Ql;
+        E[v] = fma(Pb[v], Ea[v], Eh);
+        Q[v] = fma(Pa[v], Qb[v], Ql);
       }
       halves(P[v], Pl[v], Ph[v]);
       halves(E[v], El[v], Eh);
       halves(Q[v], Ql, Qh[v]);
       if (threadIdx.x % 64 < LC) {
         sP[par][p.wave][p.cl + v] = Pl[v] * Ph[v];
-        sE[par][p.wave][p.cl + v] = Ph[v] * El[v] + Eh;
-        sQ[par][p.wave][p.cl + v] = Pl[v] * Qh[v] + Ql;
+        sE[par][p.wave][p.cl + v] = fma(Ph[v], El[v], Eh);
+        sQ[par][p.wave][p.cl + v] = fma(Pl[v], Qh[v], Ql);
       }
     }
     __syncthreads();
@@ -474,19 +481,19 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_bwd_kernel(Strided<
     for (int w = 0; w < kWaves; w++) {
 #pragma unroll
       for (int v = 0; v < kVC; v++) {
-        if (w < p.wave) h[v] = sP[par][w][p.cl + v] * h[v] + sE[par][w][p.cl + v];
+        if (w < p.wave) h[v] = fma(sP[par][w][p.cl + v], h[v], sE[par][w][p.cl + v]);
         const int r = kWaves - 1 - w;
         if (r == p.wave) q[v] = state[v];
-        state[v] = sP[par][r][p.cl + v] * state[v] + sQ[par][r][p.cl + v];
+        state[v] = fma(sP[par][r][p.cl + v], state[v], sQ[par][r][p.cl + v]);
       }
     }
 #pragma unroll
     for (int v = 0; v < kVC; v++) {
-      h[v] = p.half ? Pl[v] * h[v] + El[v] : h[v];
-      q[v] = p.half ? q[v] : Ph[v] * q[v] + Qh[v];
+      h[v] = p.half ? fma(Pl[v], h[v], El[v]) : h[v];
+      q[v] = p.half ? q[v] : fma(Ph[v], q[v], Qh[v]);
       if constexpr (LC == 16) {
-        h[v] = p.odd ? Pa[v] * h[v] + Ea[v] : h[v];
-        q[v] = p.odd ? q[v] : Pb[v] * q[v] + Qb[v];
+        h[v] = p.odd ? fma(Pa[v], h[v], Ea[v]) : h[v];
+        q[v] = p.odd ? q[v] : fma(Pb[v], q[v], Qb[v]);
       }
     }
     float H[kS][kVC];                                                  // the state before each step
@@ -497,7 +504,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_bwd_kernel(Strided<
         float a, i;
         pair(s, v, a, i);
         H[s][v] = h[v];
-        h[v] = a * h[v] + i * cx[s].get(v);
+        h[v] = fma(a, h[v], i * cx[s].get(v));
       }
     const int64_t sb = g.T * g.C;
     const Steps<T> ax(dx, sb, g.C, g, p, k), ad(dd, sb, g.C, g, p, k), az(dz, sb, g.C, g, p, k);
@@ -511,7 +518,7 @@ __global__ __launch_bounds__(Shape<LC>::kThreads) void recur_bwd_kernel(Strided<
         const float xv = cx[s].get(v), G = q[v] + top[s][v], Gi = G * i;
         ox.set(v, Gi);
         od.set(v, Gi * (H[s][v] - xv) * a);
-        if constexpr (GATE) oz.set(v, yf[s][v] * (a * H[s][v] + i * xv));
+        if constexpr (GATE) oz.set(v, yf[s][v] * fma(a, H[s][v], i * xv));
         q[v] = a * G;
       }
       if (dx) store_step<W>(ax, g, p, k, s, ox);
@@ -571,7 +578,7 @@ __global__ __launch_bounds__(128) void recur_fwd_short_kernel(Strided<T> x, Stri
           for (int v = 0; v < kShortVC; v++) {
             float a, i;
             sigmoid_pair(qd[u].get(v), a, i);
-            h[v] = a * h[v] + i * qx[u].get(v);
+            h[v] = fma(a, h[v], i * qx[u].get(v));
             o.set(v, decltype(gated)::value ? h[v] * silu(qz[u].get(v)) : h[v]);
           }
           group_store<kShortVC>(y + (b * g.T + g.at(k0 + u)) * g.C + c, m, o);
@@ -623,7 +630,7 @@ __global__ __launch_bounds__(128) void recur_bwd_short_kernel(Strided<T> x, Stri
             float a, i;
             sigmoid_pair(qd[u].get(v), a, i);
             H[k0 + u][v] = h[v];
-            h[v] = a * h[v] + i * qx[u].get(v);
+            h[v] = fma(a, h[v], i * qx[u].get(v));
           }
       }
 #pragma unroll
@@ -648,10 +655,10 @@ __global__ __launch_bounds__(128) void recur_bwd_short_kernel(Strided<T> x, Stri
               sigmoid_pair(qd[u].get(v), a, i);
               const float xv = qx[u].get(v), yv = qy[u].get(v), hv = H[k0 + u][v];
               if (decltype(gated)::value) silu_pair(qz[u].get(v), f, df);
-              const float G = q[v] + yv * f;
+              const float G = fma(yv, f, q[v]);
               ox.set(v, G * i);
               od.set(v, G * (hv - xv) * a * i);
-              if (decltype(gated)::value) oz.set(v, yv * (a * hv + i * xv) * df);
+              if (decltype(gated)::value) oz.set(v, yv * fma(a, hv, i * xv) * df);
               q[v] = a * G;
             }
             const int64_t o = (b * g.T + g.at(k0 + u)) * g.C + c;

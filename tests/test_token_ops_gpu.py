@@ -780,3 +780,24 @@ def test_second_derivatives_refused(ops):
         assert torch.equal(g.detach(), want)
         with pytest.raises(RuntimeError, match="second derivative"):
             (y.sum() + g.square().sum()).backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("size", [(2, 700, 15), (3, 129, 33), (2, 400, 63), (3, 1300, 117), (1, 5000, 65), (2, 9, 7), (1, 4100, 679)])
+def test_linear_recurrence_channels_do_not_depend_on_their_place(ops, size, dtype):
+    """An odd channel count moves the last lanes back by one, so that two of them form the same channel in different
+    places: each channel has the same bits as in a tensor of one channel more, and from call to call."""
+    B, T, C = size
+    x, d, z, h0, dy, dlast = recurrence_inputs(B, T, C + 1, dtype)
+
+    def run(n, gated, reverse):
+        c = lambda t: t[..., :n].contiguous()
+        g = c(z) if gated else None
+        y, last, carry = ops.linear_recurrence_fwd(c(x), c(d), g, c(h0), reverse=reverse)
+        grads = ops.linear_recurrence_bwd(c(x), c(d), carry, c(dy), g, c(dlast), reverse=reverse)
+        return [t[..., :C] for t in (y, last, carry, *grads) if t is not None]
+
+    for gated, reverse in ((True, False), (False, True)):
+        odd = run(C, gated, reverse)
+        for want in (run(C + 1, gated, reverse), run(C, gated, reverse)):
+            assert all(torch.equal(p, q) for p, q in zip(odd, want))
