@@ -16,6 +16,11 @@
 // of 256 MB moves 5.4 TB/s.
 #include "token_ops.h"
 
+// Columns that two lanes share (kOverlap) are formed in different slots of theirs and written by both, so their
+// bits have to be the same in each: the compiler joins no product and sum by itself, fma says where one rounding
+// is meant.
+#pragma clang fp contract(off)
+
 namespace mragan {
 namespace {
 
@@ -124,7 +129,7 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(const T* x, int64_t ro
 #pragma unroll
       for (int j = 0; j < N; j++) {
         const float d = cur[i].get(j) - mu;
-        q += counts<N, END>(at[i], j, C) ? d * d : 0.f;
+        q = counts<N, END>(at[i], j, C) ? fma(d, d, q) : q;
       }
     const float r = rsqrtf(row_sum<G>(q, red[1]) * inv + eps);
 #pragma unroll
@@ -195,9 +200,9 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(con
         const float d = cd[i].get(j), xh = (cx[i].get(j) - mu) * r, p = w ? d * wv[i].get(j) : d;
         if (END != kOverlap || counts<N, END>(at[i], j, C)) {
           s1 += p;
-          s2 += p * xh;
+          s2 = fma(p, xh, s2);
         }
-        aw[i][j] += d * xh;
+        aw[i][j] = fma(d, xh, aw[i][j]);
         ab[i][j] += d;
       }
     if (dx) {
@@ -208,7 +213,7 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(con
 #pragma unroll
         for (int j = 0; j < N; j++) {
           const float d = cd[i].get(j), xh = (cx[i].get(j) - mu) * r, p = w ? d * wv[i].get(j) : d;
-          o.set(j, r * (p - m1 - xh * m2));
+          o.set(j, r * fma(-xh, m2, p - m1));
         }
         vec_store<N, END>(dx + row * C, at[i], C, o);
       }
@@ -304,7 +309,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* x, int64_t r
     const float mu = row_sum<1024>(s, red[0]) / (float)C;
     for (int c = threadIdx.x; c < C; c += 1024) {
       const float d = (float)xr[c] - mu;
-      q += d * d;
+      q = fma(d, d, q);
     }
     const float r = rsqrtf(row_sum<1024>(q, red[1]) / (float)C + eps);
     for (int c = threadIdx.x; c < C; c += 1024)
@@ -326,12 +331,12 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* x, const flo
     for (int c = threadIdx.x; c < C; c += 1024) {
       const float p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
       s1 += p;
-      s2 += p * ((float)x[row * C + c] - mu) * r;
+      s2 = fma(p, ((float)x[row * C + c] - mu) * r, s2);
     }
     const float m1 = row_sum<1024>(s1, red[0]) / (float)C, m2 = row_sum<1024>(s2, red[1]) / (float)C;
     for (int c = threadIdx.x; c < C; c += 1024) {
       const float xh = ((float)x[row * C + c] - mu) * r, p = (float)dy[row * C + c] * (w ? (float)w[c] : 1.f);
-      dx[row * C + c] = (T)(r * (p - m1 - xh * m2));
+      dx[row * C + c] = (T)(r * fma(-xh, m2, p - m1));
     }
     __syncthreads();
   }
@@ -347,7 +352,7 @@ __global__ __launch_bounds__(256) void ln_param_long_kernel(const T* x, const fl
 #pragma unroll 8
   for (int64_t k = k0; k < k1; k++) {
     const float d = (float)dy[k * C + c];
-    sw += d * (((float)x[k * C + c] - mean[k]) * rstd[k]);
+    sw = fma(d, ((float)x[k * C + c] - mean[k]) * rstd[k], sw);
     sb += d;
   }
   float* out = part + (int64_t)blockIdx.y * 2 * C;

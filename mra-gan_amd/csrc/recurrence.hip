@@ -28,8 +28,6 @@
 namespace mragan {
 namespace {
 
-__device__ __forceinline__ float fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
-
 constexpr int kVC = 2;                    // channels a lane
 constexpr int kS = 8;                     // steps of a time lane
 constexpr int kLT = 16;                   // time lanes of a block

@@ -801,3 +801,21 @@ def test_linear_recurrence_channels_do_not_depend_on_their_place(ops, size, dtyp
         odd = run(C, gated, reverse)
         for want in (run(C + 1, gated, reverse), run(C, gated, reverse)):
             assert all(torch.equal(p, q) for p, q in zip(odd, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(700, 9), (300, 33), (90, 515), (70, 1001), (20, 2051), (9, 5003)])
+def test_layer_norm_columns_do_not_depend_on_their_place(ops, shape, dtype):
+    """The last vector of a row of odd length is moved back over columns of the one before, which both write:
+    columns that are alike have the same bits wherever they stand, and from call to call."""
+    R, C = shape
+    x, dy = randn(1, R, 1, dtype=dtype), randn(2, R, 1, dtype=dtype)
+    noise, k = randn(3, R, C // 2, dtype=dtype), C // 2
+    x = torch.cat((noise, x.expand(R, C - k)), 1)                    # columns k … C − 1 are alike
+    dy = torch.cat((noise.flip(0), dy.expand(R, C - k)), 1)
+    w, b = (torch.cat((randn(s, k, dtype=dtype), randn(s + 1, 1, dtype=dtype).expand(C - k))) for s in (4, 6))
+    for _ in range(3):
+        y, mean, rstd = ops.layer_norm_fwd(x, w, b)
+        dx, _, _ = ops.layer_norm_bwd(x, mean, rstd, dy, w, True)
+        for t in (y, dx):
+            assert torch.equal(t[:, k:], t[:, k:k + 1].expand(R, C - k))
