@@ -1167,7 +1167,10 @@ struct Ffn {
       if (planes == 2) ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 2, 2><<<grid, 256, 0, st>>>(a);
       else ffn_gemm_kernel<H, TO, EPI, TA, TB, 64, SN, 2, 2, 2, 3><<<grid, 256, 0, st>>>(a);
     }
-    if (int rc = check_launch(EPI == kEpiStore ? "ffn_gemm" : EPI == kEpiGate ? "ffn_gemm_gate" : "ffn_gemm_gate_bwd")) return rc;
+    static constexpr const char* names[3][3] = {{"ffn_gemm_64", "ffn_gemm_128", "ffn_gemm_256"},
+                                                {"ffn_gemm_gate_64", "ffn_gemm_gate_128", "ffn_gemm_gate_256"},
+                                                {"ffn_gemm_gate_bwd_64", "ffn_gemm_gate_bwd_128", "ffn_gemm_gate_bwd_256"}};
+    if (int rc = check_launch(names[EPI][t.bm / 128])) return rc;
     if (t.splits > 1) {
       const int64_t total = (int64_t)a.M * a.N;
       return reduce(a.partial, t.splits, total, a.N, a.bias, a.out, a.batches == 2 ? a.out2 : nullptr);

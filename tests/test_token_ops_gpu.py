@@ -819,3 +819,39 @@ def test_layer_norm_columns_do_not_depend_on_their_place(ops, shape, dtype):
         dx, _, _ = ops.layer_norm_bwd(x, mean, rstd, dy, w, True)
         for t in (y, dx):
             assert torch.equal(t[:, k:], t[:, k:k + 1].expand(R, C - k))
+
+
+def ffn_tiles(run):
+    """The products' launches of a call and their tiles, in order."""
+    from mragan_hip._lib import lib
+    lib().mragan_launch_log(1)
+    run()
+    return [n[len("ffn_gemm_"):] for n in lib().mragan_launch_log(1).decode().split(";") if n.startswith("ffn_gemm_")]
+
+
+LARGE = {"one plane": [(torch.bfloat16, "f32"), (torch.float16, "f32"), (torch.float32, "bf16"), (torch.float32, "fp16")],
+         "plane pairs": [(torch.float32, "f32"), (torch.float32, "bf16x3")]}
+
+
+@pytest.mark.parametrize("dtype,mode", LARGE["one plane"] + LARGE["plane pairs"], ids=str)
+@pytest.mark.parametrize("size,tiles", [
+    ((4100, 3600, 4104, 3592), (256, 256, 256, 256, 256, 256)),
+    ((4099, 3601, 4101, 3593), (256, 256, 256, 256, 256, 256)),
+    ((4100, 1032, 4104, 1040), (256, 128, 256, 128, 128, 128)),
+    ((2801, 1289, 2051, 1801), (128, 128, 128, 128, 128, 128)),
+    ((200, 2056, 8200, 1000), (128, 64, 64, 64, 256, 128)),
+    ((500, 2056, 8200, 2056), (128, 64, 128, 64, 256, 256)),
+], ids=str)
+def test_gated_ffn_large_tiles(ops, size, tiles, dtype, mode):
+    """Each product (gate and up, down, dg and du, dx, both projections' weights, w_down) on the larger tiles, with
+    remainders along all sides."""
+    a, b, dy = ffn_inputs(*size, dtype)
+    ops.set_conv_precision(mode)
+    _, kept = ops.gated_ffn_fwd(*a, *b, keep=True)
+    names = ["gate_%d", "%d", "gate_bwd_%d", "%d", "%d", "%d"]
+    want = [n % t for n, t in zip(names, tiles)]
+    assert ffn_tiles(lambda: ops.gated_ffn_fwd(*a, *b, keep=True)) == want[:2]
+    assert ffn_tiles(lambda: ops.gated_ffn_bwd(*a, dy, kept, *b)) == want[2:]
+    check_ffn(ops, a, b, dy, "silu", mode=mode)
+    if dtype == torch.bfloat16:
+        check_ffn(ops, a, b, dy, "gelu", mode=mode, keep=False, need=(True, False, True, True) + (True,) * 3)
