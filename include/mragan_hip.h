@@ -425,11 +425,13 @@ int mragan_layer_norm_bwd(const void* x, const float* mean, const float* rstd, c
 /* Gated feed-forward block on x [M][C] with weights w_gate, w_up [F][C] and w_down [O][F]:
  *   g = x·w_gateᵀ + b_gate,  u = x·w_upᵀ + b_up,  h = act(g)·u,  y = h·w_downᵀ + b_down   ([M][O])
  * act: mragan_act or one of the two below (GELU is the erf form).  Biases may be NULL.  One dtype
- * throughout; 16-byte aligned contiguous tensors; C, F and O below 2²².  fp32 tensors are multiplied
- * in the process mode of mragan_set_conv_precision (f32 here: three bf16 planes per operand, six
- * products, fp32 accumulation, ≤ 2⁻²² relative error per product; an infinite operand gives NaN);
- * 16-bit tensors as they are, and what the products take from each other (h, dg, du) is rounded to
- * that type, but h stays in fp32 for up to four rows without kept where C and F are 8 or more.
+ * throughout; 16-byte aligned contiguous tensors; C, F and O up to 2²² − 64, M up to 2³⁰.  fp32
+ * tensors are multiplied in the process mode of mragan_set_conv_precision (f32 here: three bf16 planes
+ * per operand, six products, fp32 accumulation, ≤ 2⁻²² relative error per product); 16-bit tensors as
+ * they are, and what the products take from each other (h, dg, du) is rounded to that type: in fp16,
+ * beyond ±65504 it is infinite.  h stays in fp32 for up to four rows without kept where C and F are 8 or
+ * more, so a row's result may differ in its last bits with the number of rows.  An infinite operand
+ * gives a result that is not finite, an infinity or NaN by the form that the number of rows takes.
  * kept (fp32: [3][M][F], 16-bit types: [4][M][F], the last two factors with 24 bits) holds h,
  * act'(g)·u and act(g): fwd writes it when given, bwd reads it, or recomputes it from x when NULL.
  * bwd: any gradient may be NULL to skip it; the queried workspace is enough for any choice. */

@@ -15,8 +15,9 @@ OBJ = os.environ.get("MRAGAN_OBJ_DIR", os.path.join(HERE, "build"))
 ARCH = os.environ.get("MRAGAN_ARCH", "gfx950")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
          "-Wno-unused-variable", "-Wno-unused-but-set-variable",
-         # no packed fp32 instructions: some of their forms return wrong results now and then on these
-         # cards (hipcc's host pass warns that it does not know the feature)
+         # no packed fp32 instructions: some of their forms have returned wrong results now and then on
+         # these cards, without an error, so this stays also where they would be faster (hipcc's host
+         # pass warns that it does not know the feature)
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("MRAGAN_EXTRA_FLAGS", "").split()
 
 

@@ -17,10 +17,13 @@
 //     lane ends with g and u of the same (m, n) and act(g)·u never leaves the registers.
 // The forward keeps h, act'(g)·u and act(g) for the backward, whose epilogue is then two products
 // with dh; h is the operand of dWd as it stands.
+// Roundings of 16-bit tensors: h, dg and du are operands of the next products and are rounded to the type for
+// them.  A second plane of each would double those products (2.5 of the 4.4 ms below); without one the outputs are
+// off by 0.0023 of their size in bf16, results rounded only once by 0.0017.
 // The matrix units are the bound.  Measured on 16384 rows, 2048 → 8192 → 2048, bf16 (a library product of
-// these sides: 1.3 … 1.6 PFLOP/s): gate and up 1130 us (0.97 PFLOP/s; the epilogue writes 1.07 GB of
-// kept tensors, which one block a CU does not overlap), down 415 us (1.33), dg and du 778 us (0.71; 805 MB
-// read, 537 MB written), dx 850 us (1.29), dWg and dWu 826 us (1.33), dWd 410 us (1.34).
+// these sides: 1.3 … 1.6 PFLOP/s): gate and up 1078 us (1.02 PFLOP/s; the epilogue writes 1.07 GB of
+// kept tensors, which one block a CU does not overlap), down 425 us (1.29), dg and du 787 us (0.70; its epilogue
+// reads 805 MB and writes 537), dx 851 us (1.29), dWg and dWu 820 us (1.34), dWd 400 us (1.37).
 #pragma once
 #include <type_traits>
 
@@ -1039,8 +1042,8 @@ struct Tiling {
 // The largest of three tiles that still gives the 256 CUs a block each: 256×256, 128×128 (two blocks a
 // CU), 64×64 (kEpiGate: half as many columns of g and of u each, 64×64 with 64).  `stages`: of one plane
 // pair; `products`: plane pairs.  Small tiles take all planes of a k run in one stage (NP): they are bound
-// by their loads (fp32 8192 rows, 128 → 512 → 128: forward and backward 145 us, 181 with a plane pair a
-// stage; the forward takes 49 us, 55 with such stages in place of the 128×128 tiles too).
+// by their loads (fp32 8192 rows, 128 → 512 → 128: forward and backward 145 … 150 us back to back, 181 with a plane
+// pair a stage; the forward takes 48 us, 55 with such stages in place of the 128×128 tiles too).
 // A product of small tiles whose partial sums may be stored splits k into runs of at least 4 stages (2 of
 // all planes): up to two blocks a CU where there is not one (one with three planes, whose stages fill its
 // LDS: 512 × 128 from 8192, 21.2 us, 23.6 with two), and with one plane up to three for 64 stages and more,

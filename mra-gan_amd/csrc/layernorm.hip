@@ -4,16 +4,16 @@
 //   bwd   p = dy·w,  x̂ = (x − μ)·rstd,  dx = rstd·(p − mean_c p − x̂·mean_c(p·x̂)),
 //         dw = Σ_rows dy·x̂,  db = Σ_rows dy
 //
-// Both directions are bound by HBM: fwd reads x and writes y, bwd reads x and dy and writes dx, once
-// each.  So a row lives in the registers of the G lanes that own it (G = 4 … 64 lanes of a wave, or a
+// Both directions read and write each tensor once, fwd x and y, bwd x, dy and dx, and HBM is the bound of fwd and
+// of bwd over short rows; over rows that a block shares, bwd waits for the block's barriers, three a row.  So a row lives in the registers of the G lanes that own it (G = 4 … 64 lanes of a wave, or a
 // block of 256 / 1024 threads), every sum is taken from there (the variance as the mean of squared
 // deviations, exact for rows far from zero), a block walks over rows with the next row's loads in
 // flight, and w and b are loaded once per block.  The weight's gradient is summed per lane over the
 // rows of its block in fp32, then over the block's row groups in LDS, then over the blocks by a
 // second launch: a fixed order, no atomics.
-// Measured: 524288 rows of 32 fp32 channels 26 us forward (134 MB, 5.2 TB/s), 33 + 4 us backward (201 MB);
-// 8192 rows of 2048 bf16 channels 14.3 us forward (67 MB, 4.7 TB/s), 27.4 + 4.1 us backward (101 MB).  A copy
-// of 256 MB moves 5.4 TB/s.
+// Measured: 524288 rows of 32 fp32 channels 27 us forward (134 MB, 5.0 TB/s), 33 + 4 us backward (201 MB, 6.1 TB/s:
+// x comes from the cache); 8192 rows of 2048 bf16 channels 14.3 us forward (67 MB, 4.7 TB/s), 28.6 + 4.3 us backward
+// (101 MB, 3.5 TB/s).  A copy of 256 MB moves 5.4 TB/s.
 #include "token_ops.h"
 
 // Columns that two lanes share (kOverlap) are formed in different slots of theirs and written by both, so their
@@ -297,7 +297,8 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* part
 }
 
 // Rows of more channels than the registers of a block hold (C > kMaxRow): the block walks the row
-// in memory, once per sum; the parameter gradients take a column per thread over a run of rows.
+// in memory, once per sum; the parameter gradients take a column per thread over a run of rows.  Loads of single
+// elements: 4096 rows of 16384 bf16 channels take 124 us forward (268 MB, floor 53) and 252 backward (403 MB, 79).
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* x, int64_t rows, int C, const W* w, const W* b, float eps,
                                                            T* y, float* mean, float* rstd) {

@@ -15,9 +15,9 @@
 // Steps behind the end of a sequence enter as d = +inf, x = 0: the identity.
 // The forward leaves the fp32 state entering each chunk; the backward recomputes the states of a
 // chunk from it in registers and walks the chunks backwards, so that no state is read or written.
-// Measured: 16 × 2048 × 1024 bf16 with gate 71 us forward (268 MB, 3.8 TB/s) and 106 us backward (470 MB,
-// 4.4 TB/s), one block of 8 waves a CU; 2 × 32768 × 128 fp32 in segments 14 + 18 us forward (67 MB read
-// twice, 34 MB written) and 16 + 33 us backward.
+// Measured: 16 × 2048 × 1024 bf16 with gate 69 us forward (268 MB, 3.9 TB/s) and 107 us backward (470 MB,
+// 4.4 TB/s), one block of 8 waves a CU; 2 × 32768 × 128 fp32 in segments 15 + 18 us forward (67 MB read
+// twice, 34 MB written) and 17 + 34 us backward.
 #include "token_ops.h"
 
 // A channel may be formed in either slot of a lane, by lanes moved back beside its own (see place), and on a
@@ -129,7 +129,8 @@ __device__ __forceinline__ Place place(const Geo& g) {
 
 // Where this lane's steps of chunk k lie: a wave-uniform address per step (of the chunk's lowest
 // position in memory, which a chunk cut off by the sequence's end may place before the tensor) plus
-// one 32-bit offset of the lane — per-lane 64-bit addresses of every step and tensor would registers.  Steps behind the end (and C = 1's second channel) read as `fill` and are not written.
+// one 32-bit offset of the lane: per-lane 64-bit addresses of every step and tensor would take more registers than
+// there are.  Steps behind the end (and C = 1's second channel) read as `fill` and are not written.
 template <typename T>
 struct Steps {
   T* base;                                                           // step 0 of time lane 0 (reverse: of the last)

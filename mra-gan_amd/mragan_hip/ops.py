@@ -1239,7 +1239,8 @@ def gated_ffn_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_d
                   b_down: Optional[torch.Tensor] = None, act: str = "silu", keep: bool = False):
     """y = (act(x·w_gateᵀ + b_gate) · (x·w_upᵀ + b_up))·w_downᵀ + b_down for x [..., C], w_gate, w_up [F, C],
     w_down [O, F], one type throughout; act: silu, gelu or one of ACT.  float32 tensors are multiplied in
-    set_conv_precision's mode.  Returns (y [..., O], kept): kept ([3, rows, F], 16-bit types [4, rows, F]) spares
+    set_conv_precision's mode; of 16-bit ones the hidden channels are rounded to the type between the products
+    (float16: infinite beyond 65504), but for up to four rows without keep.  Returns (y [..., O], kept): kept ([3, rows, F], 16-bit types [4, rows, F]) spares
     the backward the first two products (keep=True), else None."""
     dt, C, F, O = _ffn_check(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
     x, w_gate, w_up, w_down, b_gate, b_up, b_down = map(_dense, (x, w_gate, w_up, w_down, b_gate, b_up, b_down))
