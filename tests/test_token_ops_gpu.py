@@ -855,3 +855,94 @@ def test_gated_ffn_large_tiles(ops, size, tiles, dtype, mode):
     check_ffn(ops, a, b, dy, "silu", mode=mode)
     if dtype == torch.bfloat16:
         check_ffn(ops, a, b, dy, "gelu", mode=mode, keep=False, need=(True, False, True, True) + (True,) * 3)
+
+
+# ---- tensors whose offsets pass 32 bits -----------------------------------------------------------
+# Each operator on the whole tensors, seen through the rows at their end: only those have a gradient, so the
+# sums over all rows are theirs.
+
+def fresh(seed, *shape, dtype=torch.bfloat16, shift=0.0, scale=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.empty(shape, dtype=dtype, device="cuda").normal_(shift, scale, generator=gen)
+
+
+@pytest.mark.parametrize("rows,C", [((1 << 26) + 3, 70), ((1 << 19) + 1, 8200), ((1 << 23) + 5, 515)])
+def test_layer_norm_far_rows(ops, rows, C):
+    x, w, b = fresh(1, rows, C, scale=2.0), fresh(2, C), fresh(3, C)
+    dy, tail = torch.zeros_like(x), slice(rows - 300, None)
+    dy[tail] = fresh(4, 300, C)
+
+    class Part:
+        def layer_norm_fwd(self, *_):
+            y, *self.stats = ops.layer_norm_fwd(x, w, b, 1e-5)
+            return y[tail], *[t[tail] for t in self.stats]
+
+        def layer_norm_bwd(self, *_, bias):
+            dx, dw, db = ops.layer_norm_bwd(x, *self.stats, dy, w, bias=bias)
+            assert not dx[:1000].any()
+            return dx[tail], dw, db
+
+    check_norm(Part(), x[tail], w, b, dy=dy[tail])
+
+
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("size", [((1 << 20) + 9, 64, 4160, 72), ((1 << 22) + 9, 1032, 40, 1033)])
+def test_gated_ffn_far_rows(ops, size, keep):
+    M, C, F, O = size
+    x, (a, b, _) = fresh(1, M, C), ffn_inputs(1, C, F, O, torch.bfloat16)
+    dy, tail = torch.zeros(M, O, dtype=torch.bfloat16, device="cuda"), slice(M - 300, None)
+    dy[tail] = fresh(2, 300, O)
+
+    class Part:
+        set_conv_precision = staticmethod(ops.set_conv_precision)
+
+        def gated_ffn_fwd(self, *_, act, keep):
+            y, self.kept = ops.gated_ffn_fwd(x, *a[1:], *b, act=act, keep=keep)
+            return y[tail], None
+
+        def gated_ffn_bwd(self, *_, act, need):
+            dx, *rest = ops.gated_ffn_bwd(x, *a[1:], dy, self.kept, *b, act=act, need=need)
+            assert not dx[:1000].any()
+            return [dx[tail], *rest]
+
+    check_ffn(Part(), [x[tail], *a[1:]], b, dy[tail], "silu", keep=keep)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("C", [66, 5])
+def test_linear_recurrence_far_steps(ops, C, reverse):
+    """More than 2^32 elements of one sequence.  The checked steps restart the state, so that they depend on no others;
+    backwards the first steps taken are the far ones, whose bits are those of a short sequence."""
+    T, n = ((1 << 26) if C == 66 else (1 << 28)) + 77, 640
+    x, d, dy = fresh(1, 1, T, C), fresh(2, 1, T, C, shift=2.5), fresh(3, 1, T, C)
+    h0, dlast = fresh(4, 1, C, dtype=torch.float32), fresh(5, 1, C, dtype=torch.float32)
+    sel = slice(0, n) if reverse else slice(T - n, T)
+    d[:, n - 1 if reverse else T - n] = float("-inf")
+
+    class Part:
+        def linear_recurrence_fwd(self, *_, reverse):
+            self.y, last, self.carry = ops.linear_recurrence_fwd(x, d, None, h0, reverse=reverse)
+            return self.y[:, sel], last, None
+
+        def linear_recurrence_bwd(self, *_, reverse):
+            *grads, _ = ops.linear_recurrence_bwd(x, d, self.carry, dy, None, dlast, reverse=reverse)
+            return [t if t is None else t[:, sel] for t in grads] + [torch.zeros(1, C, device="cuda")]   # a restart passes nothing back
+
+    part = Part()
+    check_recurrence(part, x[:, sel], d[:, sel], None, h0, dy[:, sel], dlast, reverse)
+    if reverse:
+        far = slice(T - n, T)
+        assert torch.equal(part.y[:, far], ops.linear_recurrence_fwd(x[:, far], d[:, far], None, h0, reverse=True)[0])
+
+
+LONG = (1 << 22) - 64
+
+
+@pytest.mark.parametrize("size", [(70, LONG, 24, 8), (70, LONG - 3, 16, 9), (33, 16, LONG, 8), (33, 9, LONG - 5, 8), (70, 16, 24, LONG),
+                                  (2, LONG - 1, 9, 8), (300, LONG, 16, 8)])
+def test_gated_ffn_longest_sides(ops, size):
+    M, C, F, O = size
+    a = [fresh(1, M, C), fresh(2, F, C, scale=C ** -0.5), fresh(3, F, C, scale=C ** -0.5), fresh(4, O, F, scale=F ** -0.5)]
+    b = [fresh(5, F), fresh(6, F), fresh(7, O)]
+    for keep in (True, False):
+        check_ffn(ops, a, b, fresh(8, M, O), "silu", keep=keep)
